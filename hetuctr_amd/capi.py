@@ -2,6 +2,7 @@
 not load, importing a table fails loudly."""
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -14,7 +15,9 @@ SYMBOLS = ["hctr_create", "hctr_destroy", "hctr_preprocess", "hctr_preprocess_no
            "hctr_stream", "hctr_call_timing", "hctr_last_times", "hctr_last_push_ms", "hctr_defer_index", "hctr_stage_timing", "hctr_stage_count", "hctr_stage_name",
            "hctr_stage_times", "hctr_copy_probe", "hctr_sample_rows", "hctr_version", "hctr_part_create", "hctr_part_destroy",
            "hctr_part_sizes", "hctr_part_refine_data", "hctr_part_refine_embed", "hctr_part_get_communication",
-           "hctr_part_get_priority", "hctr_part_get_result", "hctr_part_get_counts", "hctr_part_cache_lists"]
+           "hctr_part_get_priority", "hctr_part_get_result", "hctr_part_get_counts", "hctr_part_cache_lists",
+           "hctr_dropout", "hctr_layer_norm", "hctr_dropout_add_layer_norm", "hctr_layer_norm_backward",
+           "hctr_dropout_add_layer_norm_backward", "hctr_layer_norm_workspace"]
 
 # items of hctr_debug_fetch (HCTR_F_*)
 UNIQUE, SORTED_ARG, RUN_START, IDX_MAP, ROOT, OFFSET, SEND_CNT, RECV_CNT = range(8)
@@ -79,6 +82,11 @@ def lib():
         l.hctr_part_get_result.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
         l.hctr_part_get_counts.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
         l.hctr_part_cache_lists.argtypes = [C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p, C.POINTER(C.c_float)]
+        for name in ("hctr_dropout", "hctr_layer_norm", "hctr_dropout_add_layer_norm", "hctr_layer_norm_backward",
+                     "hctr_dropout_add_layer_norm_backward"):
+            getattr(l, name).argtypes = [C.c_char_p]       # the packed argument record
+        l.hctr_layer_norm_workspace.argtypes = [C.c_size_t, C.c_size_t]
+        l.hctr_layer_norm_workspace.restype = C.c_size_t
         _lib = l
     return _lib
 
@@ -102,6 +110,50 @@ def copy_probe(dst_ptr, src_ptr, nbytes, repeats=5):
 def sample_rows(log_ptr, n_samples, n_fields, rows_ptr, n_rows, out_ptr):
     """out[r * n_fields + f] = log[rows[r] * n_fields + f] on the device (all pointers device memory)."""
     _check(lib().hctr_sample_rows(log_ptr, n_samples, n_fields, rows_ptr, n_rows, out_ptr))
+
+
+# The dense operators on raw pointers; hetuctr_amd.nn has them on torch tensors.  A matrix is (pointer, elements between its
+# rows), NO_MATRIX where there is none; `drop` is (p, seed, step, pointer to a number added to step or 0).
+F32, BF16, F16 = range(3)
+NO_MATRIX, NO_DROP = (0, 0), (0.0, 0, 0, 0)
+# the records of include/hetuctr_hip.h, packed in one go: a record built field by field costs several microseconds a call
+_DROPOUT_ARGS = struct.Struct("@QQ" "PqPq" "dQQP" "P" "i4x")
+_NORM_ARGS = struct.Struct("@QQ" "PqPqPqPq" "PPPP" "dQQP" "P" "f3i")
+_NORM_GRAD_ARGS = struct.Struct("@QQ" "PqPqPqPqPq" "PPPPPPQ" "dQQP" "P" "3i4x")
+
+
+def dropout(rows, width, x, y, drop, dtype, stream=0):
+    _check(lib().hctr_dropout(_DROPOUT_ARGS.pack(rows, width, *x, *y, *drop, stream, dtype)))
+
+
+def layer_norm(rows, width, x, y, weight, bias, mean, rstd, drop, eps, dtypes, stream=0):
+    """dtypes: of x, of y, of weight and bias."""
+    _check(lib().hctr_layer_norm(_NORM_ARGS.pack(rows, width, *x, *NO_MATRIX, *NO_MATRIX, *y, weight, bias, mean, rstd, *drop,
+                                                 stream, eps, *dtypes)))
+
+
+def dropout_add_layer_norm(rows, width, x, residual, total, y, weight, bias, mean, rstd, drop, eps, dtypes, stream=0):
+    """dtypes: of residual and total (the sum), of x and y, of weight and bias."""
+    _check(lib().hctr_dropout_add_layer_norm(_NORM_ARGS.pack(rows, width, *x, *residual, *total, *y, weight, bias, mean, rstd,
+                                                             *drop, stream, eps, *dtypes)))
+
+
+def layer_norm_workspace(rows, width):
+    return lib().hctr_layer_norm_workspace(rows, width)
+
+
+def layer_norm_backward(rows, width, dy, x, dx, weight, dweight, dbias, mean, rstd, workspace, workspace_bytes, drop, dtypes,
+                        stream=0):
+    _check(lib().hctr_layer_norm_backward(_NORM_GRAD_ARGS.pack(
+        rows, width, *dy, *x, *NO_MATRIX, *dx, *NO_MATRIX, weight, dweight, dbias, mean, rstd, workspace, workspace_bytes, *drop,
+        stream, *dtypes)))
+
+
+def dropout_add_layer_norm_backward(rows, width, dy, total, dtotal, dx, dresidual, weight, dweight, dbias, mean, rstd, workspace,
+                                    workspace_bytes, drop, dtypes, stream=0):
+    _check(lib().hctr_dropout_add_layer_norm_backward(_NORM_GRAD_ARGS.pack(
+        rows, width, *dy, *total, *dtotal, *dx, *dresidual, weight, dweight, dbias, mean, rstd, workspace, workspace_bytes, *drop,
+        stream, *dtypes)))
 
 
 class Table:

@@ -4,6 +4,7 @@
 #include <cstdio>
 #include <cstring>
 
+#include "dense.h"
 #include "partition.h"
 #include "table.h"
 
@@ -361,6 +362,43 @@ int hctr_part_cache_lists(hctr_partition *h, size_t max_len, int32_t *lists, siz
     h->p->cache_lists(max_len, lists, lens, kernel_ms);
   });
 }
+
+int hctr_dropout(const hctr_dropout_args *a) {
+  return guarded([&] {
+    HCTR_CHECK(a, "null argument");
+    dropout(*a);
+  });
+}
+
+int hctr_layer_norm(const hctr_norm_args *a) {
+  return guarded([&] {
+    HCTR_CHECK(a, "null argument");
+    layer_norm(*a, false);
+  });
+}
+
+int hctr_dropout_add_layer_norm(const hctr_norm_args *a) {
+  return guarded([&] {
+    HCTR_CHECK(a, "null argument");
+    layer_norm(*a, true);
+  });
+}
+
+int hctr_layer_norm_backward(const hctr_norm_grad_args *a) {
+  return guarded([&] {
+    HCTR_CHECK(a, "null argument");
+    layer_norm_backward(*a, false);
+  });
+}
+
+int hctr_dropout_add_layer_norm_backward(const hctr_norm_grad_args *a) {
+  return guarded([&] {
+    HCTR_CHECK(a, "null argument");
+    layer_norm_backward(*a, true);
+  });
+}
+
+size_t hctr_layer_norm_workspace(size_t rows, size_t width) { return layer_norm_workspace(rows, width); }
 
 #pragma GCC visibility pop
 } // extern "C"

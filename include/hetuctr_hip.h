@@ -226,6 +226,92 @@ int hctr_part_get_counts(hctr_partition *h, int32_t *data_cnt, int32_t *embed_cn
  * the device time between the first and the last kernel. */
 int hctr_part_cache_lists(hctr_partition *h, size_t max_len, int32_t *lists, size_t *lens, float *kernel_ms);
 
+/* ---- between the table's rows and a dense model -------------------------------------------------------------------
+ * Dropout, layer normalisation and both in one pass, with their gradients.  No counterpart in the reference, whose dense
+ * model lives outside.  A pull leaves float rows, the model behind it may compute in 16 bits, and a push takes float rows
+ * again: layer_norm reads one type and writes the other, its gradient the other way round.
+ *
+ * Every call launches its kernels on `stream` (a hipStream_t of the current device; NULL: the default stream) and returns;
+ * nothing is allocated, waited for or kept, and a call may be recorded into a HIP graph.  All pointers are DEVICE memory and
+ * have to stay valid until the work is done.  Results do not depend on the device's scheduling: the same call gives the
+ * same bits.  Sums, means and deviations are held in 32 bits whatever the types; a result is rounded once, to nearest even. */
+enum { HCTR_F32 = 0, HCTR_BF16 = 1, HCTR_F16 = 2 };
+
+/* The element in row r, column c lies at data + r * stride + c; stride counts elements.  Rows that are read may overlap or
+ * be one and the same (stride 0), rows that are written may not, nor may a result lie where an input does, but for the y
+ * of hctr_dropout, which may be its x.  Any address an element can have will do. */
+typedef struct hctr_matrix {
+  void *data;
+  int64_t stride;
+} hctr_matrix;
+
+/* The value in row r, column c is dropped (becomes zero, even if it is not finite) if a 32-bit word is less than p * 2^32,
+ * to the nearest integer, and is multiplied by 1 / (1 - p) otherwise.  The word is number c % 4 of Philox4x32 with 7
+ * rounds (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3; SC 2011) with the two 64-bit numbers
+ * (r * ceil(width / 4) + c / 4, step), low words first, as counter, and the seed as key.  No mask is stored: a gradient's
+ * call with the same seed and step drops the same values.  Give every layer a seed and every training step a step.
+ * step_dev: device memory with a number that is added to step, or NULL; a recorded graph draws new numbers as it changes.
+ * p = 0: nothing is dropped.  0 <= p <= 1. */
+typedef struct hctr_drop {
+  double p;
+  uint64_t seed, step;
+  const uint64_t *step_dev;
+} hctr_drop;
+
+/* y = drop(x), rows x width values of type `dtype`; its gradient is the same call on the gradient of y. */
+typedef struct hctr_dropout_args {
+  size_t rows, width;
+  hctr_matrix x, y;
+  hctr_drop drop;
+  void *stream;
+  int dtype;
+} hctr_dropout_args;
+int hctr_dropout(const hctr_dropout_args *a);
+
+/* hctr_layer_norm:              y = drop((x - mean) * rstd * weight + bias)
+ * hctr_dropout_add_layer_norm:  sum = residual + drop(x),  y = (sum - mean) * rstd * weight + bias
+ * where mean and rstd = 1 / sqrt(variance + eps) are those of each row of x, or of sum before it is rounded.
+ * stream_dtype is the type of what is normalised (x, or residual and sum), act_dtype that of the activations (y, and the x
+ * that is added); they are the same, or stream_dtype is HCTR_F32.  weight and bias (`width` elements each, NULL: none) are of
+ * affine_dtype: HCTR_F32 or act_dtype.  mean, rstd: float[rows] for the gradient, or NULL.  residual and sum are read by
+ * the second call alone. */
+typedef struct hctr_norm_args {
+  size_t rows, width;
+  hctr_matrix x, residual, sum, y;
+  const void *weight, *bias;
+  float *mean, *rstd;
+  hctr_drop drop;
+  void *stream;
+  float eps;
+  int stream_dtype, act_dtype, affine_dtype;
+} hctr_norm_args;
+int hctr_layer_norm(const hctr_norm_args *a);
+int hctr_dropout_add_layer_norm(const hctr_norm_args *a);
+
+/* The gradients of the two: dy (act_dtype) is that of y, s (stream_dtype) what was normalised, x or sum.  With
+ * g = drop(dy) * weight for the first and dy * weight for the second, and h = (s - mean) * rstd,
+ *     d = rstd * (g - mean(g) - h * mean(g * h)) [+ dsum],   dweight = sum over the rows of drop(dy) * h,   dbias = of drop(dy)
+ * hctr_layer_norm_backward writes d to dx, of stream_dtype.  hctr_dropout_add_layer_norm_backward adds dsum (stream_dtype, the
+ * gradient that sum has from elsewhere; data NULL: none), writes d to dresidual (stream_dtype) and drop(d) to dx
+ * (act_dtype); either result's data may be NULL.  dweight and dbias (affine_dtype, NULL: not wanted) are written, not
+ * added to.  workspace: hctr_layer_norm_workspace(rows, width) bytes of device memory, 16-byte aligned, in use until the
+ * work is done; needed if dweight or dbias is wanted. */
+typedef struct hctr_norm_grad_args {
+  size_t rows, width;
+  hctr_matrix dy, s, dsum, dx, dresidual;
+  const void *weight;
+  void *dweight, *dbias;
+  const float *mean, *rstd;
+  void *workspace;
+  size_t workspace_bytes;
+  hctr_drop drop;
+  void *stream;
+  int stream_dtype, act_dtype, affine_dtype;
+} hctr_norm_grad_args;
+int hctr_layer_norm_backward(const hctr_norm_grad_args *a);
+int hctr_dropout_add_layer_norm_backward(const hctr_norm_grad_args *a);
+size_t hctr_layer_norm_workspace(size_t rows, size_t width);
+
 /* Version string of the library. */
 const char *hctr_version(void);
 
