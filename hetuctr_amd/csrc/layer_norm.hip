@@ -60,9 +60,105 @@ __global__ __launch_bounds__(kBlock) void norm_wide(NormForward a) {
   }
 }
 
+// ITEMS pieces of V columns per lane of a row that LANES lanes hold in registers: the row is read once.  Up to a wave's
+// lanes, a group of lanes has a row to itself and a block as many rows as it has groups; beyond that the waves of a block share
+// a row, each a stretch of neighbouring columns, and join what they found: a wave's sum and its squares around its own
+// mean.  (Squares around a mean that is not the row's would cancel; put together as n * (wave's mean - mean)^2 they do not,
+// and the block waits once instead of twice.)
+template <typename S, typename A, bool ADD, bool DROP, int LANES, int ITEMS>
+__global__ __launch_bounds__(block_of<LANES>) void norm_rows(NormForward a) {
+  constexpr int V = kVec<S>, BLOCK = block_of<LANES>, GROUP = LANES < kWave ? LANES : kWave, WAVES = LANES / GROUP;
+  constexpr uint32_t STRETCH = GROUP * V * ITEMS; // columns of a group, or wave
+  __shared__ float2 found[WAVES];
+  const uint32_t lane = threadIdx.x % GROUP, wave = WAVES > 1 ? threadIdx.x / kWave : 0, first = wave * STRETCH + lane * V;
+  const bool even = a.width % V == 0;
+  const uint64_t step = DROP ? step_of(a.drop) : 0;
+  for (uint64_t r = (uint64_t)blockIdx.x * (BLOCK / LANES) + threadIdx.x / LANES; r < a.rows; r += (uint64_t)gridDim.x * (BLOCK / LANES)) {
+    Floats<V> f[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) {
+      const uint32_t c = first + i * GROUP * V;
+      if constexpr (ADD) f[i] = load_columns<V>((const A *)a.x + (int64_t)r * a.x_stride, c, a.width);
+      else f[i] = load_columns<V>((const S *)a.x + (int64_t)r * a.x_stride, c, a.width);
+    }
+    if constexpr (ADD) {
+#pragma unroll
+      for (int i = 0; i < ITEMS; i++) {
+        const uint32_t c = first + i * GROUP * V;
+        const Floats<V> g = load_columns<V>((const S *)a.residual + (int64_t)r * a.residual_stride, c, a.width);
+        if constexpr (DROP) drop_columns(f[i], a.drop, step, r * a.drop.quads + c / 4);
+#pragma unroll
+        for (int j = 0; j < V; j++) f[i].v[j] += g.v[j];
+        store_columns((S *)a.sum + (int64_t)r * a.sum_stride, c, a.width, f[i]);
+      }
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++)
+#pragma unroll
+      for (int j = 0; j < V; j++) sum += f[i].v[j];
+    sum = group_sum<GROUP>(sum);
+    // columns behind the end hold zeros and have to add nothing to the squares
+    const float n = WAVES > 1 ? (float)min(a.width - min(a.width, wave * STRETCH), STRETCH) : 0.f;
+    const float middle = WAVES > 1 ? sum / fmaxf(n, 1.f) : sum * a.inv_width;
+    float square = 0.f;
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) {
+      const uint32_t c = first + i * GROUP * V;
+      if (even) {
+        const float m = c < a.width ? middle : 0.f;
+#pragma unroll
+        for (int j = 0; j < V; j++) square = fmaf(f[i].v[j] - m, f[i].v[j] - m, square);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          const float d = f[i].v[j] - (c + j < a.width ? middle : 0.f);
+          square = fmaf(d, d, square);
+        }
+      }
+    }
+    square = group_sum<GROUP>(square);
+    float mean = middle;
+    if constexpr (WAVES > 1) {
+      __syncthreads(); // the row before has been read
+      if (lane == 0) found[wave] = make_float2(sum, square);
+      __syncthreads();
+      sum = square = 0.f;
+#pragma unroll
+      for (int w = 0; w < WAVES; w++) sum += found[w].x;
+      mean = sum * a.inv_width;
+#pragma unroll
+      for (int w = 0; w < WAVES; w++) {
+        const float k = (float)min(a.width - min(a.width, w * STRETCH), STRETCH), off = found[w].x / fmaxf(k, 1.f) - mean;
+        square += fmaf(k * off, off, found[w].y);
+      }
+    }
+    const float rstd = rsqrtf(fmaf(square, a.inv_width, a.eps));
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) {
+      const uint32_t c = first + i * GROUP * V;
+      const Floats<V> w = load_affine<V, A>(a.weight, a.narrow, c, a.width, 1.f), b = load_affine<V, A>(a.bias, a.narrow, c, a.width, 0.f);
+#pragma unroll
+      for (int j = 0; j < V; j++) f[i].v[j] = fmaf((f[i].v[j] - mean) * rstd, w.v[j], b.v[j]);
+      if constexpr (DROP && !ADD) drop_columns(f[i], a.drop, step, r * a.drop.quads + c / 4);
+      store_columns((A *)a.y + (int64_t)r * a.y_stride, c, a.width, f[i]);
+    }
+    if (threadIdx.x % LANES == 0) {
+      if (a.mean) a.mean[r] = mean;
+      if (a.rstd) a.rstd[r] = rstd;
+    }
+  }
+}
+
 template <typename S, typename A, bool ADD, bool DROP> void launch(const NormForward &p, hipStream_t s) {
-  const unsigned blocks = (unsigned)std::min<uint64_t>(p.rows, 1u << 20);
-  hipLaunchKernelGGL((norm_wide<S, A, ADD, DROP>), dim3(blocks), dim3(kBlock), 0, s, p);
+  const bool held = rows_in_registers<S>(p.width, [&](auto lanes, auto items) {
+    constexpr int LANES = decltype(lanes)::value, ITEMS = decltype(items)::value, BLOCK = block_of<LANES>;
+    const uint64_t blocks = (p.rows + BLOCK / LANES - 1) / (BLOCK / LANES);
+    hipLaunchKernelGGL((norm_rows<S, A, ADD, DROP, LANES, ITEMS>), dim3((unsigned)std::min<uint64_t>(blocks, (1u << 31) / BLOCK)),
+                       dim3(BLOCK), 0, s, p);
+  });
+  if (!held)
+    hipLaunchKernelGGL((norm_wide<S, A, ADD, DROP>), dim3((unsigned)std::min<uint64_t>(p.rows, 1u << 20)), dim3(kBlock), 0, s, p);
   HCTR_HIP(hipGetLastError());
 }
 

@@ -7,11 +7,11 @@ namespace hctr {
 typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 
-// Columns a lane moves at a time: 16 bytes of the narrower of the types that a kernel moves, as long as the wider ones take at most
-// two such pieces.  Always a multiple of four, the columns that one draw of the generator serves.
+// Columns a lane moves at a time: 16 bytes of the type that is normalised or dropped.  Always a multiple of four, the columns
+// that one draw of the generator serves.
 template <typename T> constexpr int kVec = 16 / (int)sizeof(T);
 
-template <typename T, int V> struct alignas(sizeof(T)) Packed {
+template <typename T, int V> struct Packed {
   typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)))); // any address a T can have
 };
 template <int V> struct Floats {
@@ -20,15 +20,23 @@ template <int V> struct Floats {
 
 // Columns c .. c + V - 1 of a row of `width` columns, those behind its end as zeros.  A row may start at any multiple of its
 // element's size (gfx950 moves up to 16 bytes from any address in one instruction), and nothing outside it is read.
-template <int V, typename T> __device__ __forceinline__ Floats<V> load_columns(const T *row, uint32_t c, uint32_t width) {
+// ONCE: nothing reads them again soon.
+template <int V, bool ONCE = true, typename T>
+__device__ __forceinline__ Floats<V> load_columns(const T *row, uint32_t c, uint32_t width) {
   Floats<V> f;
   if (c + V <= width) {
-    const auto x = __builtin_nontemporal_load((const typename Packed<T, V>::type *)(row + c));
+    typedef const typename Packed<T, V>::type *Vector;
+    const auto x = ONCE ? __builtin_nontemporal_load((Vector)(row + c)) : *(Vector)(row + c);
 #pragma unroll
     for (int j = 0; j < V; j++) f.v[j] = (float)x[j];
   } else {
 #pragma unroll
-    for (int j = 0; j < V; j++) f.v[j] = c + j < width ? (float)row[c + j] : 0.f;
+    for (int j = 0; j < V; j++) f.v[j] = 0.f;
+    if (c < width) {
+#pragma unroll
+      for (int j = 0; j + 1 < V; j++)
+        if (c + j < width) f.v[j] = (float)row[c + j];
+    }
   }
   return f;
 }
@@ -40,9 +48,9 @@ template <int V, typename T> __device__ __forceinline__ void store_columns(T *ro
 #pragma unroll
     for (int j = 0; j < V; j++) x[j] = (T)f.v[j];
     __builtin_nontemporal_store(x, (typename Packed<T, V>::type *)(row + c));
-  } else {
+  } else if (c < width) {
 #pragma unroll
-    for (int j = 0; j < V; j++)
+    for (int j = 0; j + 1 < V; j++)
       if (c + j < width) row[c + j] = (T)f.v[j];
   }
 }
