@@ -14,8 +14,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "build")
 LIBDIR = os.path.join(HERE, "lib")
-HIP_SOURCES = ["radix_sort.hip", "tile_sort.hip", "preprocess.hip", "push.hip", "pull.hip", "init.hip", "table.hip", "checkpoint.hip", "loader.hip", "partition.hip", "host_copy.hip", "dropout.hip", "layer_norm.hip", "layer_norm_grad.hip", "c_api.hip"]
-HEADERS = ["common.h", "host_copy.h", "kernels.h", "radix_sort.h", "tile_sort.h", "run_lists.h", "row_slices.h", "launch_cut.h", "unique_tile.h", "table.h", "partition.h", "dense.h", "layer_norm.h", "philox.h", "values.h", os.path.join("..", "..", "include", "hetuctr_hip.h")]
+HIP_SOURCES = ["radix_sort.hip", "tile_sort.hip", "preprocess.hip", "push.hip", "pull.hip", "init.hip", "table.hip", "checkpoint.hip", "loader.hip", "partition.hip", "host_copy.hip", "dropout.hip", "layer_norm_f32.hip", "layer_norm_f32_bf16.hip", "layer_norm_f32_f16.hip", "layer_norm_bf16.hip", "layer_norm_f16.hip", "layer_norm.hip", "c_api.hip"]
+HEADERS = ["common.h", "host_copy.h", "kernels.h", "radix_sort.h", "tile_sort.h", "run_lists.h", "row_slices.h", "launch_cut.h", "unique_tile.h", "table.h", "partition.h", "dense.h", "layer_norm.h", "layer_norm_forward.h", "layer_norm_backward.h", "philox.h", "values.h", os.path.join("..", "..", "include", "hetuctr_hip.h")]
 # packed-fp32 instruction selection is switched off for all device code; no fused multiply-add contraction, so
 # that "sum * -lr" then "row + that" rounds twice like the CPU restatement it is checked against (fused
 # operations are written explicitly where they are meant)

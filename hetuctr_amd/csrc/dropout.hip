@@ -16,9 +16,9 @@ __global__ __launch_bounds__(kBlock) void dropout_rows(const T *__restrict__ x, 
   const uint64_t i = (uint64_t)blockIdx.x * kBlock + threadIdx.x, row = i / pieces;
   if (row >= rows) return;
   const uint32_t c = (uint32_t)(i - row * pieces) * V;
-  Floats<V> f = load_columns<V>(x + (int64_t)row * x_stride, c, width);
+  Floats<V> f = load_columns<V, Rows::kLong>(x + (int64_t)row * x_stride, c, width);
   if constexpr (ON) drop_columns(f, d, step_of(d), row * d.quads + c / 4);
-  store_columns(y + (int64_t)row * y_stride, c, width, f);
+  store_columns<V, Rows::kLong>(y + (int64_t)row * y_stride, c, width, f);
 }
 
 template <typename T> void launch(const hctr_dropout_args &a, const Dropping &d, bool on) {

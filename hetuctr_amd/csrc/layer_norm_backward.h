@@ -1,0 +1,239 @@
+// The kernels of the gradient of layer normalisation: of the rows, and of weight and bias.
+//
+// The rows' gradients need two sums over each row.  Those of weight and bias are sums over all rows: every block adds up the rows
+// that it works on, writes one row of partial sums, and a second kernel adds those up in the order of the blocks, so that the
+// result does not depend on which block is done first.
+#pragma once
+#include <algorithm>
+
+#include "layer_norm.h"
+
+namespace hctr {
+namespace {
+
+// One block per row at a time, which it reads twice; its sums for weight and bias lie in its row of `partial` from the first row
+// on: rows of any width.
+template <typename S, typename A, bool ADD, bool DROP>
+__global__ __launch_bounds__(kWideBlock) void grad_wide(NormBackward a) {
+  constexpr int V = kVec<S>;
+  __shared__ float smem[kWideBlock / kWave];
+  const uint64_t step = DROP ? step_of(a.drop) : 0;
+  float *dweight = a.partial ? a.partial + (uint64_t)blockIdx.x * 2 * a.width : nullptr, *dbias = dweight + a.width;
+  for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const float mean = a.mean[r], rstd = a.rstd[r];
+    const auto gradient = [&](uint32_t c) { // of y, before what was dropped behind the normalisation
+      Floats<V> f = load_columns<V, Rows::kLong>((const A *)a.dy + (int64_t)r * a.dy_stride, c, a.width);
+      if constexpr (DROP && !ADD) drop_columns(f, a.drop, step, r * a.drop.quads + c / 4);
+      return f;
+    };
+    const auto normal = [&](uint32_t c) {
+      Floats<V> f = load_columns<V, Rows::kLong>((const S *)a.s + (int64_t)r * a.s_stride, c, a.width);
+#pragma unroll
+      for (int j = 0; j < V; j++) f.v[j] = (f.v[j] - mean) * rstd;
+      return f;
+    };
+    float sum_g = 0.f, sum_gh = 0.f;
+    for (uint32_t c = threadIdx.x * V; c < a.width; c += kWideBlock * V) {
+      const Floats<V> g = gradient(c), h = normal(c);
+      Floats<V> w[1];
+      load_affine<V, A, Rows::kLong>(w, a.weight, a.narrow, c, 0, a.width, 1.f);
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const float gw = g.v[j] * w[0].v[j];
+        if (c + j < a.width) {
+          sum_g += gw;
+          sum_gh = fmaf(gw, h.v[j], sum_gh);
+        }
+      }
+      if (dweight) {
+        const bool first = r == blockIdx.x;
+#pragma unroll
+        for (int j = 0; j < V; j++)
+          if (c + j < a.width) {
+            dweight[c + j] = fmaf(g.v[j], h.v[j], first ? 0.f : dweight[c + j]);
+            dbias[c + j] = g.v[j] + (first ? 0.f : dbias[c + j]);
+          }
+      }
+    }
+    const float mean_g = block_sum<kWideBlock>(sum_g, smem) * a.inv_width, mean_gh = block_sum<kWideBlock>(sum_gh, smem) * a.inv_width;
+    for (uint32_t c = threadIdx.x * V; c < a.width; c += kWideBlock * V) {
+      const Floats<V> g = gradient(c), h = normal(c);
+      Floats<V> w[1];
+      load_affine<V, A, Rows::kLong>(w, a.weight, a.narrow, c, 0, a.width, 1.f);
+      Floats<V> d;
+#pragma unroll
+      for (int j = 0; j < V; j++) d.v[j] = rstd * (fmaf(g.v[j], w[0].v[j], -mean_g) - h.v[j] * mean_gh);
+      if constexpr (ADD) {
+        if (a.ds) {
+          const Floats<V> more = load_columns<V, Rows::kLong>((const S *)a.ds + (int64_t)r * a.ds_stride, c, a.width);
+#pragma unroll
+          for (int j = 0; j < V; j++) d.v[j] += more.v[j];
+        }
+        if (a.dresidual) store_columns<V, Rows::kLong>((S *)a.dresidual + (int64_t)r * a.dresidual_stride, c, a.width, d);
+        if (a.dx) {
+          if constexpr (DROP) drop_columns(d, a.drop, step, r * a.drop.quads + c / 4);
+          store_columns<V, Rows::kLong>((A *)a.dx + (int64_t)r * a.dx_stride, c, a.width, d);
+        }
+      } else {
+        store_columns<V, Rows::kLong>((S *)a.dx + (int64_t)r * a.dx_stride, c, a.width, d);
+      }
+    }
+  }
+}
+
+// The rows that a block works on, held in registers as by the forward pass (rows_in_registers): each is read once.  A lane has the
+// same columns of every row, so it keeps their sums for weight and bias in registers too, and the block's groups join theirs at
+// the end.  The next row is on its way while this one is worked on; where the waves of a block share a row, their two
+// sums go through LDS, in two places by turns, so that one barrier per row will do.
+template <typename S, typename A, bool ADD, bool DROP, Rows R, int LANES, int ITEMS>
+__global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
+  constexpr int V = kVec<S>, BLOCK = block_of<LANES>, GROUP = LANES < kWave ? LANES : kWave, WAVES = LANES / GROUP, GROUPS = BLOCK / LANES;
+  constexpr bool TIGHT = LANES == 1024; // 128 registers: the row's own values and sums are all that fits
+  __shared__ float2 found[2][WAVES];
+  __shared__ float joined[GROUPS > 1 ? GROUPS * LANES * ITEMS * V : 1];
+  const uint32_t lane = threadIdx.x % GROUP, wave = WAVES > 1 ? threadIdx.x / kWave : 0;
+  uint32_t first = wave * GROUP * V * ITEMS + lane * V;
+  const uint64_t step = DROP ? step_of(a.drop) : 0, stride = (uint64_t)gridDim.x * GROUPS;
+  Floats<V> w[ITEMS], dweight[ITEMS], dbias[ITEMS];
+  if constexpr (!TIGHT) load_affine<V, A, R>(w, a.weight, a.narrow, first, GROUP * V, a.width, 1.f);
+#pragma unroll
+  for (int i = 0; i < ITEMS; i++) {
+#pragma unroll
+    for (int j = 0; j < V; j++) dweight[i].v[j] = dbias[i].v[j] = 0.f;
+  }
+  typename Packed<A, V>::type dy[ITEMS];
+  typename Packed<S, V>::type s[ITEMS];
+  typename Packed<S, V>::type ds[ITEMS];
+  float mean = 0.f, rstd = 0.f;
+  const auto fetch = [&](uint64_t r) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) {
+      const uint32_t c = first + i * GROUP * V;
+      dy[i] = load_raw<V, R>((const A *)a.dy + (int64_t)r * a.dy_stride, c, a.width);
+      s[i] = load_raw<V, R>((const S *)a.s + (int64_t)r * a.s_stride, c, a.width);
+      if constexpr (ADD && !TIGHT)
+        if (a.ds) ds[i] = load_raw<V, R>((const S *)a.ds + (int64_t)r * a.ds_stride, c, a.width);
+    }
+    mean = a.mean[r];
+    rstd = a.rstd[r];
+  };
+  uint64_t r = (uint64_t)blockIdx.x * GROUPS + threadIdx.x / LANES;
+  if (!TIGHT && r < a.rows) fetch(r);
+  int turn = 0;
+  for (; r < a.rows; r += stride) {
+    if constexpr (TIGHT) {
+      asm volatile("" : "+v"(first)); // no address is worked out, and kept, before the loop
+      fetch(r);
+      load_affine<V, A, R>(w, a.weight, a.narrow, first, GROUP * V, a.width, 1.f);
+    }
+    Floats<V> g[ITEMS], h[ITEMS];
+    typename Packed<S, V>::type more[ITEMS];
+    float sum_g = 0.f, sum_gh = 0.f;
+    const float scale = rstd;
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) {
+      const uint32_t c = first + i * GROUP * V;
+      g[i] = floats<V>(settled<V, R>(dy[i], c, a.width));
+      h[i] = floats<V>(settled<V, R>(s[i], c, a.width));
+      if constexpr (ADD && !TIGHT) more[i] = ds[i];
+#pragma unroll
+      for (int j = 0; j < V; j++) h[i].v[j] = (h[i].v[j] - mean) * scale;
+    }
+    if (!TIGHT && r + stride < a.rows) fetch(r + stride);
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) {
+      if constexpr (DROP && !ADD) drop_columns(g[i], a.drop, step, r * a.drop.quads + (first + i * GROUP * V) / 4);
+#pragma unroll
+      for (int j = 0; j < V; j++) { // columns behind the end have no gradient, and add nothing
+        dweight[i].v[j] = fmaf(g[i].v[j], h[i].v[j], dweight[i].v[j]);
+        dbias[i].v[j] += g[i].v[j];
+        g[i].v[j] *= w[i].v[j];
+        sum_g += g[i].v[j];
+        sum_gh = fmaf(g[i].v[j], h[i].v[j], sum_gh);
+      }
+    }
+    sum_g = group_sum<GROUP>(sum_g);
+    sum_gh = group_sum<GROUP>(sum_gh);
+    if constexpr (WAVES > 1) {
+      if (lane == 0) found[turn][wave] = make_float2(sum_g, sum_gh);
+      __syncthreads();
+      const float2 other = found[turn][lane % WAVES]; // every lane takes one wave's
+      sum_g = group_sum<WAVES>(other.x);
+      sum_gh = group_sum<WAVES>(other.y);
+      turn ^= 1;
+    }
+    const float mean_g = sum_g * a.inv_width, mean_gh = sum_gh * a.inv_width;
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) {
+      if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
+      const uint32_t c = first + i * GROUP * V;
+      Floats<V> d;
+#pragma unroll
+      for (int j = 0; j < V; j++) d.v[j] = scale * (fmaf(-h[i].v[j], mean_gh, g[i].v[j]) - mean_g);
+      if constexpr (ADD) {
+        if (a.ds) {
+          if constexpr (TIGHT) more[i] = load_raw<V, R>((const S *)a.ds + (int64_t)r * a.ds_stride, c, a.width);
+          const Floats<V> e = floats<V>(settled<V, R>(more[i], c, a.width));
+#pragma unroll
+          for (int j = 0; j < V; j++) d.v[j] += e.v[j];
+        }
+        if (a.dresidual) store_columns<V, R>((S *)a.dresidual + (int64_t)r * a.dresidual_stride, c, a.width, d);
+        if (a.dx) {
+          if constexpr (DROP) drop_columns(d, a.drop, step, r * a.drop.quads + c / 4);
+          store_columns<V, R>((A *)a.dx + (int64_t)r * a.dx_stride, c, a.width, d);
+        }
+      } else {
+        store_columns<V, R>((S *)a.dx + (int64_t)r * a.dx_stride, c, a.width, d);
+      }
+    }
+  }
+  if (!a.partial) return;
+  float *out = a.partial + (uint64_t)blockIdx.x * 2 * a.width;
+  const auto join = [&](Floats<V> (&sums)[ITEMS], float *row) { // in the order of the groups, and one row of results
+    if constexpr (GROUPS > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < ITEMS; i++)
+#pragma unroll
+        for (int j = 0; j < V; j++) joined[threadIdx.x / LANES * (LANES * ITEMS * V) + (i * GROUP + lane) * V + j] = sums[i].v[j];
+      __syncthreads();
+      for (uint32_t c = threadIdx.x; c < a.width; c += BLOCK) {
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < GROUPS; k++) sum += joined[k * (LANES * ITEMS * V) + c];
+        row[c] = sum;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < ITEMS; i++)
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          const uint32_t c = first + i * GROUP * V + j;
+          if (c < a.width) row[c] = sums[i].v[j];
+        }
+    }
+  };
+  join(dweight, out);
+  join(dbias, out + a.width);
+}
+
+template <typename S, typename A, bool ADD, bool DROP> unsigned launch_grad(const NormBackward &p, hipStream_t s) {
+  unsigned blocks = norm_grad_blocks(p.rows, p.width, ADD, p.width % kVec<S> != 0);
+  const bool held = rows_in_registers<S>(p.width, [&](auto how, auto lanes, auto items) {
+    constexpr int LANES = decltype(lanes)::value, ITEMS = decltype(items)::value, BLOCK = block_of<LANES>;
+    blocks = (unsigned)std::min<uint64_t>(blocks, (p.rows + BLOCK / LANES - 1) / (BLOCK / LANES));
+    hipLaunchKernelGGL((grad_rows<S, A, ADD, DROP, decltype(how)::value, LANES, ITEMS>), dim3(blocks), dim3(BLOCK), 0, s, p);
+  });
+  if (!held) hipLaunchKernelGGL((grad_wide<S, A, ADD, DROP>), dim3(blocks), dim3(kWideBlock), 0, s, p);
+  HCTR_HIP(hipGetLastError());
+  return blocks;
+}
+
+} // namespace
+
+template <typename S, typename A> unsigned launch_norm_grad(const NormBackward &p, bool add, bool dropped, hipStream_t s) {
+  if (add) return dropped ? launch_grad<S, A, true, true>(p, s) : launch_grad<S, A, true, false>(p, s);
+  return dropped ? launch_grad<S, A, false, true>(p, s) : launch_grad<S, A, false, false>(p, s);
+}
+
+} // namespace hctr

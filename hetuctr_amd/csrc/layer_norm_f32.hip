@@ -1,0 +1,7 @@
+#include "layer_norm_backward.h"
+#include "layer_norm_forward.h"
+
+namespace hctr {
+template void launch_norm<float, float>(const NormForward &, bool, bool, hipStream_t);
+template unsigned launch_norm_grad<float, float>(const NormBackward &, bool, bool, hipStream_t);
+} // namespace hctr

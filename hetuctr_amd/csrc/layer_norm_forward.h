@@ -1,0 +1,193 @@
+// The kernels of layer normalisation, with dropout behind it or a dropped-out branch added before it.
+#pragma once
+#include <algorithm>
+
+#include "layer_norm.h"
+
+namespace hctr {
+namespace {
+
+// One block per row at a time, which it reads again for each of mean, variance and result: rows of any width.
+template <typename S, typename A, bool ADD, bool DROP>
+__global__ __launch_bounds__(kWideBlock) void norm_wide(NormForward a) {
+  constexpr int V = kVec<S>;
+  __shared__ float smem[kWideBlock / kWave];
+  const uint64_t step = DROP ? step_of(a.drop) : 0;
+  for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const auto value = [&](uint32_t c) { // what is normalised, in 32 bits
+      if constexpr (ADD) {
+        Floats<V> f = load_columns<V, Rows::kLong>((const A *)a.x + (int64_t)r * a.x_stride, c, a.width);
+        if constexpr (DROP) drop_columns(f, a.drop, step, r * a.drop.quads + c / 4);
+        const Floats<V> g = load_columns<V, Rows::kLong>((const S *)a.residual + (int64_t)r * a.residual_stride, c, a.width);
+#pragma unroll
+        for (int j = 0; j < V; j++) f.v[j] += g.v[j];
+        return f;
+      } else {
+        return load_columns<V, Rows::kLong>((const S *)a.x + (int64_t)r * a.x_stride, c, a.width);
+      }
+    };
+    float sum = 0.f;
+    for (uint32_t c = threadIdx.x * V; c < a.width; c += kWideBlock * V) {
+      const Floats<V> f = value(c);
+      if constexpr (ADD) store_columns<V, Rows::kLong>((S *)a.sum + (int64_t)r * a.sum_stride, c, a.width, f);
+#pragma unroll
+      for (int j = 0; j < V; j++) sum += f.v[j];
+    }
+    const float mean = block_sum<kWideBlock>(sum, smem) * a.inv_width;
+    float square = 0.f;
+    for (uint32_t c = threadIdx.x * V; c < a.width; c += kWideBlock * V) {
+      const Floats<V> f = value(c);
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const float d = c + j < a.width ? f.v[j] - mean : 0.f;
+        square = fmaf(d, d, square);
+      }
+    }
+    const float rstd = rsqrtf(block_sum<kWideBlock>(square, smem) * a.inv_width + a.eps);
+    for (uint32_t c = threadIdx.x * V; c < a.width; c += kWideBlock * V) {
+      Floats<V> f = value(c);
+      Floats<V> w[1], b[1];
+      load_affine<V, A, Rows::kLong>(w, a.weight, a.narrow, c, 0, a.width, 1.f);
+      load_affine<V, A, Rows::kLong>(b, a.bias, a.narrow, c, 0, a.width, 0.f);
+#pragma unroll
+      for (int j = 0; j < V; j++) f.v[j] = fmaf((f.v[j] - mean) * rstd, w[0].v[j], b[0].v[j]);
+      if constexpr (DROP && !ADD) drop_columns(f, a.drop, step, r * a.drop.quads + c / 4);
+      store_columns<V, Rows::kLong>((A *)a.y + (int64_t)r * a.y_stride, c, a.width, f);
+    }
+    if (threadIdx.x == 0) {
+      if (a.mean) a.mean[r] = mean;
+      if (a.rstd) a.rstd[r] = rstd;
+    }
+  }
+}
+
+// ITEMS pieces of V columns per lane of a row that LANES lanes hold in registers: the row is read once.  Up to a wave's
+// lanes, a group of lanes has a row to itself, ROWS of them at a time, and a block as many as it has groups; beyond that the waves of a
+// block share a row, each a stretch of neighbouring columns, and join what they found: a wave's sum and its squares around
+// its own mean.  (Squares around a mean that is not the row's would cancel; put together as n * (wave's mean - mean)^2 they do
+// not, and the block waits once instead of twice.)
+template <typename S, typename A, bool ADD, bool DROP, Rows R, int LANES, int ITEMS, int ROWS>
+__global__ __launch_bounds__(block_of<LANES>) void norm_rows(NormForward a) {
+  constexpr int V = kVec<S>, BLOCK = block_of<LANES>, GROUP = LANES < kWave ? LANES : kWave, WAVES = LANES / GROUP, GROUPS = BLOCK / LANES;
+  constexpr uint32_t STRETCH = GROUP * V * ITEMS; // columns of a group, or wave
+  static_assert(WAVES == 1 || ROWS == 1, "a block that shares a row has one at a time");
+  __shared__ float2 found[WAVES];
+  const uint32_t lane = threadIdx.x % GROUP, wave = WAVES > 1 ? threadIdx.x / kWave : 0;
+  const uint64_t step = DROP ? step_of(a.drop) : 0;
+  for (uint64_t r0 = (uint64_t)blockIdx.x * (GROUPS * ROWS) + threadIdx.x / LANES; r0 < a.rows; r0 += (uint64_t)gridDim.x * (GROUPS * ROWS)) {
+    uint32_t first = wave * STRETCH + lane * V;
+    asm volatile("" : "+v"(first)); // no address is worked out, and kept, before the loop
+    typedef std::conditional_t<ADD, A, S> X;
+    typename Packed<X, V>::type x[ROWS][ITEMS];
+    typename Packed<S, V>::type residual[ROWS][ITEMS];
+    Floats<V> f[ROWS][ITEMS], w[ITEMS], b[ITEMS];
+    const auto row = [&](int k) { return r0 + (uint64_t)(k * GROUPS); };
+    // a row that is not there is one of no columns
+    const auto width = [&](int k) { return k == 0 || row(k) < a.rows ? a.width : 0; };
+#pragma unroll
+    for (int k = 0; k < ROWS; k++)
+#pragma unroll
+      for (int i = 0; i < ITEMS; i++) {
+        const uint32_t c = first + i * GROUP * V;
+        x[k][i] = load_raw<V, R>((const X *)a.x + (int64_t)row(k) * a.x_stride, c, width(k));
+        if constexpr (ADD) residual[k][i] = load_raw<V, R>((const S *)a.residual + (int64_t)row(k) * a.residual_stride, c, width(k));
+      }
+    load_affine<V, A, R>(w, a.weight, a.narrow, first, GROUP * V, a.width, 1.f);
+    load_affine<V, A, R>(b, a.bias, a.narrow, first, GROUP * V, a.width, 0.f);
+#pragma unroll
+    for (int k = 0; k < ROWS; k++)
+#pragma unroll
+      for (int i = 0; i < ITEMS; i++) {
+        const uint32_t c = first + i * GROUP * V;
+        f[k][i] = floats<V>(settled<V, R>(x[k][i], c, a.width));
+        if constexpr (ADD) {
+          const Floats<V> g = floats<V>(settled<V, R>(residual[k][i], c, a.width));
+          if constexpr (DROP) drop_columns(f[k][i], a.drop, step, row(k) * a.drop.quads + c / 4);
+#pragma unroll
+          for (int j = 0; j < V; j++) f[k][i].v[j] += g.v[j];
+          store_columns<V, R>((S *)a.sum + (int64_t)row(k) * a.sum_stride, c, width(k), f[k][i]);
+        }
+      }
+    float mean[ROWS], rstd[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; k++) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < ITEMS; i++)
+#pragma unroll
+        for (int j = 0; j < V; j++) sum += f[k][i].v[j];
+      sum = group_sum<GROUP>(sum);
+      const float n = WAVES > 1 ? (float)min(a.width - min(a.width, wave * STRETCH), STRETCH) : 0.f;
+      mean[k] = WAVES > 1 ? sum / fmaxf(n, 1.f) : sum * a.inv_width;
+      // columns behind the end hold zeros and have to add nothing to the squares
+      float square = 0.f;
+#pragma unroll
+      for (int i = 0; i < ITEMS; i++) {
+        const uint32_t c = first + i * GROUP * V;
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          const float d = f[k][i].v[j] - ((R == Rows::kEven ? c : c + j) < a.width ? mean[k] : 0.f);
+          square = fmaf(d, d, square);
+        }
+      }
+      square = group_sum<GROUP>(square);
+      if constexpr (WAVES > 1) {
+        __syncthreads(); // the row before has been read
+        if (lane == 0) found[wave] = make_float2(sum, square);
+        __syncthreads();
+        // every lane takes one wave's
+        const float2 other = found[lane % WAVES];
+        const float m = (float)min(a.width - min(a.width, lane % WAVES * STRETCH), STRETCH);
+        mean[k] = group_sum<WAVES>(other.x) * a.inv_width;
+        const float off = other.x / fmaxf(m, 1.f) - mean[k];
+        square = group_sum<WAVES>(fmaf(m * off, off, other.y));
+      }
+      rstd[k] = rsqrtf(fmaf(square, a.inv_width, a.eps));
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) {
+      const uint32_t c = first + i * GROUP * V;
+#pragma unroll
+      for (int k = 0; k < ROWS; k++) {
+#pragma unroll
+        for (int j = 0; j < V; j++) f[k][i].v[j] = fmaf((f[k][i].v[j] - mean[k]) * rstd[k], w[i].v[j], b[i].v[j]);
+        if constexpr (DROP && !ADD) drop_columns(f[k][i], a.drop, step, row(k) * a.drop.quads + c / 4);
+        store_columns<V, R>((A *)a.y + (int64_t)row(k) * a.y_stride, c, width(k), f[k][i]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < ROWS; k++)
+      if (threadIdx.x % LANES == 0 && width(k)) {
+        if (a.mean) a.mean[row(k)] = mean[k];
+        if (a.rstd) a.rstd[row(k)] = rstd[k];
+      }
+  }
+}
+
+template <typename S, typename A, bool ADD, bool DROP> void launch(const NormForward &p, hipStream_t s) {
+  const bool held = rows_in_registers<S>(p.width, [&](auto rows, auto lanes, auto items) {
+    constexpr Rows R = decltype(rows)::value;
+    constexpr int LANES = decltype(lanes)::value, ITEMS = decltype(items)::value, BLOCK = block_of<LANES>;
+    // Four rows at a time where the memory would wait for the lanes: they draw, convert two values a register, or leave some of
+    // their loads empty.  us with one row and with four, 2^27 values: float to bfloat16, dropped, 16 columns 155, 131, 64
+    // columns 156, 132, 256 columns 160, 139; float, 37 columns 313, 226; bfloat16, 64 columns 96, 92.  Elsewhere four are no
+    // better or worse: float, 64 columns 175, 179, 256 columns 179, 194; a branch added, float and bfloat16, 256 columns 265, 283.
+    constexpr bool FOUR = LANES <= kWave && ITEMS == 1 && (R == Rows::kRagged || (!ADD && (DROP || sizeof(S) == 2)));
+    constexpr int ROWS = FOUR ? 4 : 1, PER = BLOCK / LANES * ROWS;
+    const uint64_t blocks = (p.rows + PER - 1) / PER;
+    hipLaunchKernelGGL((norm_rows<S, A, ADD, DROP, R, LANES, ITEMS, ROWS>), dim3((unsigned)std::min<uint64_t>(blocks, (1u << 31) / BLOCK)),
+                       dim3(BLOCK), 0, s, p);
+  });
+  if (!held)
+    hipLaunchKernelGGL((norm_wide<S, A, ADD, DROP>), dim3((unsigned)std::min<uint64_t>(p.rows, 1u << 20)), dim3(kWideBlock), 0, s, p);
+  HCTR_HIP(hipGetLastError());
+}
+
+} // namespace
+
+template <typename S, typename A> void launch_norm(const NormForward &p, bool add, bool dropped, hipStream_t s) {
+  if (add) dropped ? launch<S, A, true, true>(p, s) : launch<S, A, true, false>(p, s);
+  else dropped ? launch<S, A, false, true>(p, s) : launch<S, A, false, false>(p, s);
+}
+
+} // namespace hctr
