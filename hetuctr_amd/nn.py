@@ -36,6 +36,11 @@ class Drop(NamedTuple):
     step_tensor: Optional[torch.Tensor] = None
 
 
+# The host's share of a call is several microseconds, more than a small kernel takes (1.9 of them torch.cuda.current_stream
+# alone): what follows keeps to torch's cheaper calls.
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _drop(drop, device):
     if drop is None:
         return capi.NO_DROP
@@ -75,43 +80,55 @@ def _same(t, like, dtype, what):
         raise RuntimeError("hetuctr_amd.nn: %s must be %s of shape %s on %s" % (what, dtype, tuple(like.shape), like.device))
 
 
+def _per_column(t, width, act, device, what):
+    """weight or bias, ready to be read"""
+    if t is None:
+        return None
+    if t.shape != (width,) or t.device != device or (t.dtype != torch.float32 and t.dtype != act):
+        raise RuntimeError("hetuctr_amd.nn: %s must hold %d values of float32 or %s on %s" % (what, width, act, device))
+    return t if t.is_contiguous() else t.contiguous()
+
+
 def _affine(weight, bias, width, act, device):
     """weight and bias (or None) ready to be read, and the code of their type"""
-    code = capi.F32
-    given = []
-    for t, what in ((weight, "weight"), (bias, "bias")):
-        if t is not None:
-            if t.shape != (width,) or t.device != device or (t.dtype != torch.float32 and t.dtype != act):
-                raise RuntimeError("hetuctr_amd.nn: %s must hold %d values of float32 or %s on %s" % (what, width, act, device))
-            code = _DTYPES[t.dtype]
-            t = t.contiguous()
-        given.append(t)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise RuntimeError("hetuctr_amd.nn: weight and bias must be of one type")
-    return given[0], given[1], code
+    weight, bias = _per_column(weight, width, act, device, "weight"), _per_column(bias, width, act, device, "bias")
+    if weight is not None:
+        if bias is not None and weight.dtype != bias.dtype:
+            raise RuntimeError("hetuctr_amd.nn: weight and bias must be of one type")
+        return weight, bias, _DTYPES[weight.dtype]
+    return weight, bias, capi.F32 if bias is None else _DTYPES[bias.dtype]
 
 
 def _pointer(t):
     return 0 if t is None else t.data_ptr()
 
 
+def _result(like, dtype):
+    return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 def _call(device, f, *args):
     """f on torch's current stream of `device`"""
-    if device.index == torch.cuda.current_device():
-        f(*args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        f(*args, _stream_of(index))
     else:
-        with torch.cuda.device(device):
-            f(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(index):
+            f(*args, _stream_of(index))
 
 
 def _wants_gradient(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # ---- dropout ----------------------------------------------------------------------------------------------------------
 def _dropout(x, drop):
     m, at = _matrix(x, "x")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _result(x, x.dtype)
     _call(x.device, capi.dropout, m.shape[0], m.shape[1], at, (y.data_ptr(), m.shape[1]), _drop(drop, x.device), _type(x.dtype, "x"))
     return y
 
@@ -139,8 +156,8 @@ def dropout(x, drop):
 
 
 # ---- layer normalisation ------------------------------------------------------------------------------------------------
-def _statistics(rows, device):
-    return torch.empty(rows, dtype=torch.float32, device=device), torch.empty(rows, dtype=torch.float32, device=device)
+def _statistics(rows, like):
+    return like.new_empty(rows, dtype=torch.float32), like.new_empty(rows, dtype=torch.float32)
 
 
 def _norm(x, weight, bias, eps, drop, dtype, stats):
@@ -148,8 +165,8 @@ def _norm(x, weight, bias, eps, drop, dtype, stats):
     m, at = _matrix(x, "x")
     rows, width = m.shape
     weight, bias, affine = _affine(weight, bias, width, dtype, x.device)
-    y = torch.empty(x.shape, dtype=dtype, device=x.device)
-    mean, rstd = _statistics(rows, x.device) if stats else (None, None)
+    y = _result(x, dtype)
+    mean, rstd = _statistics(rows, x) if stats else (None, None)
     _call(x.device, capi.layer_norm, rows, width, at, (y.data_ptr(), width), _pointer(weight), _pointer(bias), _pointer(mean),
           _pointer(rstd), _drop(drop, x.device), eps, (_type(x.dtype, "x"), _type(dtype, "the result"), affine))
     return y, mean, rstd
@@ -166,13 +183,13 @@ def _columns(dy, rows, width, weight, bias, need_weight, need_bias):
     dweight = torch.empty_like(weight) if weight is not None and need_weight else None
     dbias = torch.empty_like(bias) if bias is not None and need_bias else None
     need = capi.layer_norm_workspace(rows, width) if dweight is not None or dbias is not None else 0
-    return dweight, dbias, torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None, need
+    return dweight, dbias, dy.new_empty(need, dtype=torch.uint8) if need else None, need
 
 
 def _statistic(t, rows, like, what):
     if t.numel() != rows or t.dtype != torch.float32 or t.device != like.device:
         raise RuntimeError("hetuctr_amd.nn: %s must hold a float32 for each of the %d rows on %s" % (what, rows, like.device))
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _norm_backward(dy, x, mean, rstd, weight, bias, drop, need_weight, need_bias):
@@ -182,7 +199,7 @@ def _norm_backward(dy, x, mean, rstd, weight, bias, drop, need_weight, need_bias
     rows, width = m.shape
     weight, bias, affine = _affine(weight, bias, width, dy.dtype, x.device)
     mean, rstd = _statistic(mean, rows, x, "mean"), _statistic(rstd, rows, x, "rstd")
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = _result(x, x.dtype)
     dweight, dbias, space, need = _columns(dy, rows, width, weight, bias, need_weight, need_bias)
     _call(x.device, capi.layer_norm_backward, rows, width, g_at, at, (dx.data_ptr(), width), _pointer(weight), _pointer(dweight),
           _pointer(dbias), mean.data_ptr(), rstd.data_ptr(), _pointer(space), need, _drop(drop, x.device),
@@ -225,9 +242,9 @@ def _add_norm(x, residual, weight, bias, eps, drop, stats):
     r, r_at = _matrix(residual, "residual")
     rows, width = m.shape
     weight, bias, affine = _affine(weight, bias, width, x.dtype, x.device)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    s = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-    mean, rstd = _statistics(rows, x.device) if stats else (None, None)
+    y = _result(x, x.dtype)
+    s = _result(x, residual.dtype)
+    mean, rstd = _statistics(rows, x) if stats else (None, None)
     _call(x.device, capi.dropout_add_layer_norm, rows, width, at, r_at, (s.data_ptr(), width), (y.data_ptr(), width),
           _pointer(weight), _pointer(bias), _pointer(mean), _pointer(rstd), _drop(drop, x.device), eps,
           (_type(residual.dtype, "residual"), _type(x.dtype, "x"), affine))
@@ -252,9 +269,9 @@ def _add_norm_backward(dy, ds, s, mean, rstd, weight, bias, drop, need_x, need_w
     rows, width = m.shape
     weight, bias, affine = _affine(weight, bias, width, dy.dtype, s.device)
     mean, rstd = _statistic(mean, rows, s, "mean"), _statistic(rstd, rows, s, "rstd")
-    dresidual = torch.empty(s.shape, dtype=s.dtype, device=s.device)
+    dresidual = _result(s, s.dtype)
     one = dy.dtype == s.dtype and (drop is None or drop.p == 0)
-    dx = torch.empty(s.shape, dtype=dy.dtype, device=s.device) if need_x and not one else None
+    dx = _result(s, dy.dtype) if need_x and not one else None
     dweight, dbias, space, need = _columns(dy, rows, width, weight, bias, need_weight, need_bias)
     _call(s.device, capi.dropout_add_layer_norm_backward, rows, width, g_at, at, d_at,
           capi.NO_MATRIX if dx is None else (dx.data_ptr(), width), (dresidual.data_ptr(), width), _pointer(weight),
