@@ -1,5 +1,6 @@
 // Device code that layer normalisation and its gradient share.
 #pragma once
+#include <algorithm>
 #include <type_traits>
 
 #include "dense.h"
@@ -68,43 +69,60 @@ constexpr int kWideBlock = 256; // threads of a block that reads its row again a
 // threads of a block whose rows are held by LANES lanes each: 256, or those of one row if they are more than a wave
 template <int LANES> constexpr int block_of = LANES <= kWave ? 256 : LANES;
 
-// f(rows, lanes, items), constants: how rows of `width` columns are read, the lanes that hold one in registers, and the pieces of
-// kVec<S> columns that each of them holds: as few lanes as can read the row at once, up to a wave of them, then up to 16
-// columns a lane (32 do not fit beside weight and bias into the 128 registers of a block of 1024).  False: the row is wider
-// than 16384 columns.
-template <Rows R, typename S, typename F> bool lanes_of_rows(uint32_t pieces, F &&f) {
-  constexpr int MOST = 16 / kVec<S>;
-  constexpr std::integral_constant<Rows, R> rows;
-  using std::integral_constant;
-  if (pieces <= 2) f(rows, integral_constant<int, 2>(), integral_constant<int, 1>());
-  else if (pieces <= 4) f(rows, integral_constant<int, 4>(), integral_constant<int, 1>());
-  else if (pieces <= 8) f(rows, integral_constant<int, 8>(), integral_constant<int, 1>());
-  else if (pieces <= 16) f(rows, integral_constant<int, 16>(), integral_constant<int, 1>());
-  else if (pieces <= 32) f(rows, integral_constant<int, 32>(), integral_constant<int, 1>());
-  else if (pieces <= 64) f(rows, integral_constant<int, 64>(), integral_constant<int, 1>());
-  else if (pieces <= 128) f(rows, integral_constant<int, 64>(), integral_constant<int, 2>());
-  else if (pieces <= 64 * MOST) f(rows, integral_constant<int, 64>(), integral_constant<int, MOST>());
-  else if (pieces <= 128 * MOST) f(rows, integral_constant<int, 128>(), integral_constant<int, MOST>());
-  else if (pieces <= 256 * MOST) f(rows, integral_constant<int, 256>(), integral_constant<int, MOST>());
-  else if (pieces <= 512 * MOST) f(rows, integral_constant<int, 512>(), integral_constant<int, MOST>());
-  else if (pieces <= 1024 * MOST) f(rows, integral_constant<int, 1024>(), integral_constant<int, MOST>());
-  else return false;
-  return true;
+// The lanes that hold a row of `width` columns in registers, and the pieces of V columns that each of them holds: as few lanes as
+// can read the row at once, up to a wave of them; then up to 16 columns a lane (32 do not fit beside weight and bias into the
+// 128 registers of a block of 1024).  A block that shares a row has four waves at least: with two, half of a CU's four SIMDs
+// had no work (the gradient of 2^27 values, a branch added and dropped, 2048 columns: 405 us with 128 lanes, 354 with 256).
+// No lanes: the row is wider than 16384 columns.
+struct Held {
+  int lanes, items;
+};
+constexpr Held held_by(uint32_t width, int V) {
+  const uint32_t pieces = (width - 1) / V + 1;
+  const int most = 16 / V;
+  for (int lanes = 2; lanes <= kWave; lanes *= 2)
+    if (pieces <= (uint32_t)lanes) return {lanes, 1};
+  for (int items = 2; items <= most; items *= 2)
+    if (pieces <= (uint32_t)(kWave * items)) return {kWave, items};
+  if (pieces <= (uint32_t)(256 * most / 2)) return {256, most / 2};
+  for (int lanes = 256; lanes <= 1024; lanes *= 2)
+    if (pieces <= (uint32_t)(lanes * most)) return {lanes, most};
+  return {0, 0};
 }
+// f(rows, lanes, items), constants, for how rows of `width` columns are read and held; false: they are not held
 template <typename S, typename F> bool rows_in_registers(uint32_t width, F &&f) {
-  const uint32_t pieces = div_up(width, kVec<S>);
-  return width % kVec<S> ? lanes_of_rows<Rows::kRagged, S>(pieces, f) : lanes_of_rows<Rows::kEven, S>(pieces, f);
+  constexpr int V = kVec<S>, MOST = 16 / V;
+  const Held h = held_by(width, V);
+  const auto with = [&](auto lanes, auto items) {
+    if (h.lanes != lanes || h.items != items) return false;
+    if (width % V) f(std::integral_constant<Rows, Rows::kRagged>(), lanes, items);
+    else f(std::integral_constant<Rows, Rows::kEven>(), lanes, items);
+    return true;
+  };
+  using std::integral_constant;
+  constexpr integral_constant<int, 1> one;
+  constexpr integral_constant<int, MOST / 2> half;
+  constexpr integral_constant<int, MOST> most;
+  constexpr integral_constant<int, 64> wave;
+  constexpr integral_constant<int, 256> four;
+  bool done = with(integral_constant<int, 2>(), one) || with(integral_constant<int, 4>(), one) || with(integral_constant<int, 8>(), one) ||
+              with(integral_constant<int, 16>(), one) || with(integral_constant<int, 32>(), one) || with(wave, one) || with(wave, most) ||
+              with(four, half) || with(four, most) || with(integral_constant<int, 512>(), most) || with(integral_constant<int, 1024>(), most);
+  if constexpr (MOST > 2) done = done || with(wave, half);
+  return done;
 }
 
-// Blocks of the gradient's kernels, each of which writes a row of sums for weight and bias: few of them, since the sums are written
-// and read beside the data, but enough loads under way to fill the memory, and a multiple of the 256 CUs.  us on an MI355X
-// with 256, 512, 768, 1280 blocks, 2^27 values: float, 64 columns 411, 283, 277, 302; float and bfloat16, dropped, 128
-// columns -, 262, 230, 256; a branch added (its sum's gradient is loaded ahead too) 64 columns -, 356, 385, 425; float, 2048
-// columns 308, 274, 283, 298; 4096 columns 276, 281, 284, 284; 4096 rows of 8192 halves 52, 66, 78, 103.  Narrow rows that
-// leave lanes idle want more: 37 columns, dropped, -, 647, 493, 351, a branch added -, 740, 560, 470.
-constexpr unsigned norm_grad_blocks(uint64_t rows, uint32_t width, bool add, bool ragged) {
-  const unsigned most = width > 4096 ? 256 : width > 1024 ? 512 : ragged ? 1280 : add ? 512 : 768;
-  return rows < most ? (unsigned)rows : most;
+// Blocks of the gradient's kernels, each of which writes a row of sums for weight and bias: as many per CU as fetch 18 KiB at a
+// time (bytes: of a column's values, read), so few that the memory sees long stretches and the rows of sums are little beside the data, at
+// least one and at most eight.  us on an MI355X for 2^27 values with 256, 512, 768, 1024 blocks (chosen: *): float, 64
+// columns 411, 287, 274*, 290; 1024 columns 268*, 286, 282, 286; bfloat16, 4096 columns 152, 151*, 160, 159; float and bfloat16,
+// dropped, 128 columns 665, 262, 230*, 244; the same with a branch added, 512 columns 354*, 386, 408, 423; 2048 columns 354*, 377,
+// 411, 431; 4096 rows of 8192 halves 51*, 63, 74, 86; 37 columns, dropped, with 768, 1536, 2048 493, 323*, 401.
+inline unsigned norm_grad_blocks(uint64_t rows, uint32_t width, int V, int bytes) {
+  const Held h = held_by(width, V);
+  const uint64_t groups = h.lanes && h.lanes < 256 ? 256 / h.lanes : 1, fetch = groups * width * bytes;
+  const uint64_t per_cu = std::min<uint64_t>((18 * 1024 - 1) / fetch + 1, 8);
+  return (unsigned)std::min(256 * per_cu, (rows + groups - 1) / groups);
 }
 
 // The kernels' launches, one instance per pair of types in a file of its own (layer_norm_*.hip); add, dropped: which of the four

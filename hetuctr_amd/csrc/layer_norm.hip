@@ -43,7 +43,9 @@ template <typename W> void launch_sum(const hctr_norm_grad_args &a, unsigned blo
 
 // The most that norm_grad_blocks says for any form and pair of types.
 size_t layer_norm_workspace(size_t rows, size_t width) {
-  return std::min<size_t>(rows, width <= 1024 ? 1280 : width <= 4096 ? 512 : 256) * 2 * width * sizeof(float);
+  if (!rows || !width || width >= (1u << 31)) return 0;
+  const uint32_t w = (uint32_t)width;
+  return (size_t)std::max(norm_grad_blocks(rows, w, kVec<float>, 6), norm_grad_blocks(rows, w, kVec<bf16_t>, 4)) * 2 * width * sizeof(float);
 }
 
 void check_types(int stream, int act, int affine, bool has_affine) {

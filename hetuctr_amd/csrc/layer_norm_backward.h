@@ -4,8 +4,6 @@
 // that it works on, writes one row of partial sums, and a second kernel adds those up in the order of the blocks, so that the
 // result does not depend on which block is done first.
 #pragma once
-#include <algorithm>
-
 #include "layer_norm.h"
 
 namespace hctr {
@@ -88,7 +86,7 @@ __global__ __launch_bounds__(kWideBlock) void grad_wide(NormBackward a) {
 template <typename S, typename A, bool ADD, bool DROP, Rows R, int LANES, int ITEMS>
 __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
   constexpr int V = kVec<S>, BLOCK = block_of<LANES>, GROUP = LANES < kWave ? LANES : kWave, WAVES = LANES / GROUP, GROUPS = BLOCK / LANES;
-  constexpr bool TIGHT = LANES == 1024; // 128 registers: the row's own values and sums are all that fits
+  constexpr bool TIGHT = LANES == 1024 && ITEMS * V == 16; // 128 registers: the row's own values and sums are all that fits
   __shared__ float2 found[2][WAVES];
   __shared__ float joined[GROUPS > 1 ? GROUPS * LANES * ITEMS * V : 1];
   const uint32_t lane = threadIdx.x % GROUP, wave = WAVES > 1 ? threadIdx.x / kWave : 0;
@@ -218,10 +216,9 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
 }
 
 template <typename S, typename A, bool ADD, bool DROP> unsigned launch_grad(const NormBackward &p, hipStream_t s) {
-  unsigned blocks = norm_grad_blocks(p.rows, p.width, ADD, p.width % kVec<S> != 0);
+  const unsigned blocks = norm_grad_blocks(p.rows, p.width, kVec<S>, (int)(sizeof(A) + sizeof(S) * (p.ds ? 2 : 1)));
   const bool held = rows_in_registers<S>(p.width, [&](auto how, auto lanes, auto items) {
     constexpr int LANES = decltype(lanes)::value, ITEMS = decltype(items)::value, BLOCK = block_of<LANES>;
-    blocks = (unsigned)std::min<uint64_t>(blocks, (p.rows + BLOCK / LANES - 1) / (BLOCK / LANES));
     hipLaunchKernelGGL((grad_rows<S, A, ADD, DROP, decltype(how)::value, LANES, ITEMS>), dim3(blocks), dim3(BLOCK), 0, s, p);
   });
   if (!held) hipLaunchKernelGGL((grad_wide<S, A, ADD, DROP>), dim3(blocks), dim3(kWideBlock), 0, s, p);

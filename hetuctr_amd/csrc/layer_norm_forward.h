@@ -1,7 +1,5 @@
 // The kernels of layer normalisation, with dropout behind it or a dropped-out branch added before it.
 #pragma once
-#include <algorithm>
-
 #include "layer_norm.h"
 
 namespace hctr {
@@ -61,6 +59,10 @@ __global__ __launch_bounds__(kWideBlock) void norm_wide(NormForward a) {
   }
 }
 
+// Rows of more than 512 columns, but for those that leave no registers for the next one: a block stays for several.
+template <typename S, int LANES, int ITEMS>
+constexpr bool stays = LANES * ITEMS * kVec<S> > 512 && !(LANES == 1024 && ITEMS * kVec<S> == 16);
+
 // ITEMS pieces of V columns per lane of a row that LANES lanes hold in registers: the row is read once.  Up to a wave's
 // lanes, a group of lanes has a row to itself, ROWS of them at a time, and a block as many as it has groups; beyond that the waves of a
 // block share a row, each a stretch of neighbouring columns, and join what they found: a wave's sum and its squares around
@@ -71,19 +73,21 @@ __global__ __launch_bounds__(block_of<LANES>) void norm_rows(NormForward a) {
   constexpr int V = kVec<S>, BLOCK = block_of<LANES>, GROUP = LANES < kWave ? LANES : kWave, WAVES = LANES / GROUP, GROUPS = BLOCK / LANES;
   constexpr uint32_t STRETCH = GROUP * V * ITEMS; // columns of a group, or wave
   static_assert(WAVES == 1 || ROWS == 1, "a block that shares a row has one at a time");
-  __shared__ float2 found[WAVES];
+  // Wide rows: a block stays for several, weight and bias in its registers, the next row on its way while one is worked on.
+  constexpr bool STAYS = stays<S, LANES, ITEMS>;
+  __shared__ float2 found[2][WAVES]; // by turns, so that one barrier per row will do
   const uint32_t lane = threadIdx.x % GROUP, wave = WAVES > 1 ? threadIdx.x / kWave : 0;
-  const uint64_t step = DROP ? step_of(a.drop) : 0;
-  for (uint64_t r0 = (uint64_t)blockIdx.x * (GROUPS * ROWS) + threadIdx.x / LANES; r0 < a.rows; r0 += (uint64_t)gridDim.x * (GROUPS * ROWS)) {
-    uint32_t first = wave * STRETCH + lane * V;
-    asm volatile("" : "+v"(first)); // no address is worked out, and kept, before the loop
-    typedef std::conditional_t<ADD, A, S> X;
-    typename Packed<X, V>::type x[ROWS][ITEMS];
-    typename Packed<S, V>::type residual[ROWS][ITEMS];
-    Floats<V> f[ROWS][ITEMS], w[ITEMS], b[ITEMS];
-    const auto row = [&](int k) { return r0 + (uint64_t)(k * GROUPS); };
-    // a row that is not there is one of no columns
-    const auto width = [&](int k) { return k == 0 || row(k) < a.rows ? a.width : 0; };
+  uint32_t first = wave * STRETCH + lane * V;
+  const uint64_t step = DROP ? step_of(a.drop) : 0, stride = (uint64_t)gridDim.x * (GROUPS * ROWS);
+  uint64_t r0 = (uint64_t)blockIdx.x * (GROUPS * ROWS) + threadIdx.x / LANES;
+  typedef std::conditional_t<ADD, A, S> X;
+  typename Packed<X, V>::type x[ROWS][ITEMS];
+  typename Packed<S, V>::type residual[ROWS][ITEMS];
+  Floats<V> w[ITEMS], b[ITEMS];
+  const auto row = [&](int k) { return r0 + (uint64_t)(k * GROUPS); };
+  // a row that is not there is one of no columns
+  const auto width = [&](int k) { return k == 0 || row(k) < a.rows ? a.width : 0; };
+  const auto fetch = [&] {
 #pragma unroll
     for (int k = 0; k < ROWS; k++)
 #pragma unroll
@@ -92,8 +96,22 @@ __global__ __launch_bounds__(block_of<LANES>) void norm_rows(NormForward a) {
         x[k][i] = load_raw<V, R>((const X *)a.x + (int64_t)row(k) * a.x_stride, c, width(k));
         if constexpr (ADD) residual[k][i] = load_raw<V, R>((const S *)a.residual + (int64_t)row(k) * a.residual_stride, c, width(k));
       }
+  };
+  const auto fetch_affine = [&] {
     load_affine<V, A, R>(w, a.weight, a.narrow, first, GROUP * V, a.width, 1.f);
     load_affine<V, A, R>(b, a.bias, a.narrow, first, GROUP * V, a.width, 0.f);
+  };
+  if (STAYS && r0 < a.rows) {
+    fetch();
+    fetch_affine();
+  }
+  for (int turn = 0; r0 < a.rows; r0 += stride, turn ^= 1) {
+    if constexpr (!STAYS) {
+      asm volatile("" : "+v"(first)); // no address is worked out, and kept, before the loop
+      fetch();
+      fetch_affine();
+    }
+    Floats<V> f[ROWS][ITEMS];
 #pragma unroll
     for (int k = 0; k < ROWS; k++)
 #pragma unroll
@@ -108,6 +126,11 @@ __global__ __launch_bounds__(block_of<LANES>) void norm_rows(NormForward a) {
           store_columns<V, R>((S *)a.sum + (int64_t)row(k) * a.sum_stride, c, width(k), f[k][i]);
         }
       }
+    if (STAYS && r0 + stride < a.rows) {
+      r0 += stride;
+      fetch();
+      r0 -= stride;
+    }
     float mean[ROWS], rstd[ROWS];
 #pragma unroll
     for (int k = 0; k < ROWS; k++) {
@@ -132,11 +155,10 @@ __global__ __launch_bounds__(block_of<LANES>) void norm_rows(NormForward a) {
       }
       square = group_sum<GROUP>(square);
       if constexpr (WAVES > 1) {
-        __syncthreads(); // the row before has been read
-        if (lane == 0) found[wave] = make_float2(sum, square);
+        if (lane == 0) found[turn][wave] = make_float2(sum, square);
         __syncthreads();
         // every lane takes one wave's
-        const float2 other = found[lane % WAVES];
+        const float2 other = found[turn][lane % WAVES];
         const float m = (float)min(a.width - min(a.width, lane % WAVES * STRETCH), STRETCH);
         mean[k] = group_sum<WAVES>(other.x) * a.inv_width;
         const float off = other.x / fmaxf(m, 1.f) - mean[k];
@@ -174,9 +196,18 @@ template <typename S, typename A, bool ADD, bool DROP> void launch(const NormFor
     // better or worse: float, 64 columns 175, 179, 256 columns 179, 194; a branch added, float and bfloat16, 256 columns 265, 283.
     constexpr bool FOUR = LANES <= kWave && ITEMS == 1 && (R == Rows::kRagged || (!ADD && (DROP || sizeof(S) == 2)));
     constexpr int ROWS = FOUR ? 4 : 1, PER = BLOCK / LANES * ROWS;
-    const uint64_t blocks = (p.rows + PER - 1) / PER;
-    hipLaunchKernelGGL((norm_rows<S, A, ADD, DROP, R, LANES, ITEMS, ROWS>), dim3((unsigned)std::min<uint64_t>(blocks, (1u << 31) / BLOCK)),
-                       dim3(BLOCK), 0, s, p);
+    // Blocks that stay: as many per CU as fetch 16 KiB at a time, or sixteen where the draws' arithmetic wants them.  us for 2^27
+    // values with 256, 512, 1024, 4096 blocks and with one for each row (chosen: *): float, 4096 columns 176*, 179, 184, 182, 195;
+    // bfloat16, 2048 columns 197, 120, 92*, 98, 111, 8192 columns 90*, 91, 92, 93, 117; a branch added, float and bfloat16, 1024
+    // columns 269*, 292, 286, 278, 272, 4096 columns 269*, 285, 284, 278, 282; float to bfloat16, dropped, 4096 columns 176, 141,
+    // 145, 137*, 157.  Two pieces a lane of a wave: 297 with 512 blocks, 272 with one for each row*.
+    uint64_t most = (1u << 31) / BLOCK;
+    if constexpr (stays<S, LANES, ITEMS>) {
+      const uint64_t fetch = (uint64_t)PER * p.width * (ADD ? sizeof(A) + sizeof(S) : sizeof(S));
+      most = 256 * (DROP && !ADD ? 16 : (16 * 1024 - 1) / fetch + 1);
+    }
+    const uint64_t blocks = std::min<uint64_t>((p.rows + PER - 1) / PER, most);
+    hipLaunchKernelGGL((norm_rows<S, A, ADD, DROP, R, LANES, ITEMS, ROWS>), dim3((unsigned)blocks), dim3(BLOCK), 0, s, p);
   });
   if (!held)
     hipLaunchKernelGGL((norm_wide<S, A, ADD, DROP>), dim3((unsigned)std::min<uint64_t>(p.rows, 1u << 20)), dim3(kWideBlock), 0, s, p);
