@@ -1,5 +1,7 @@
 // Rows of float, bfloat16 or half values as the dense operators read and write them: a few columns at a time, in 32 bits.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 namespace hctr {
@@ -81,13 +83,25 @@ __device__ __forceinline__ Floats<V> load_columns(const T *row, uint32_t c, uint
   return floats<V>(settled<V, R>(load_raw<V, R, ONCE>(row, c, width), c, width));
 }
 
-// Columns c .. c + V - 1 written, rounded to the nearest value of T (ties to even) if that is narrower.  The last columns of a
+// Values rounded to T, to nearest, ties to even.  The compiler may put the product or sum that made a value and its rounding to half
+// into one instruction, which does not round to 32 bits in between, in one kernel and not in another: it is kept from that,
+// so that a value does not depend on where its row lies.
+template <typename T, int V> __device__ __forceinline__ typename Packed<T, V>::type rounded(const Floats<V> &f) {
+  typename Packed<T, V>::type x;
+#pragma unroll
+  for (int j = 0; j < V; j++) {
+    float v = f.v[j];
+    if constexpr (std::is_same_v<T, f16_t>) asm("" : "+v"(v));
+    x[j] = (T)v;
+  }
+  return x;
+}
+
+// Columns c .. c + V - 1 written, rounded to the nearest value of T.  The last columns of a
 // ragged row go out in pieces of a power of two.
 template <int V, Rows R, typename T>
 __device__ __forceinline__ void store_columns(T *row, uint32_t c, uint32_t width, const Floats<V> &f) {
-  typename Packed<T, V>::type x;
-#pragma unroll
-  for (int j = 0; j < V; j++) x[j] = (T)f.v[j];
+  typename Packed<T, V>::type x = rounded<T>(f);
   T *p = at_column<R>(row, c);
   if constexpr (R == Rows::kEven) {
     if (c < width) __builtin_nontemporal_store(x, (typename Packed<T, V>::memory *)p);
