@@ -7,24 +7,30 @@ namespace hctr {
 namespace {
 
 // The blocks' rows of sums (dweight's columns, then dbias's), added up: COLUMNS neighbouring columns per block, whose threads share
-// out the rows and join their sums through LDS, in an order that depends on nothing but the sizes.
-constexpr int kSumColumns = 32, kSumRows = 32;
-template <typename W>
-__global__ __launch_bounds__(kSumColumns * kSumRows) void sum_partial(const float *__restrict__ partial, uint32_t blocks, uint32_t width,
-                                                                      W *dweight, W *dbias) {
-  __shared__ float sums[kSumRows][kSumColumns + 1];
-  const uint32_t x = threadIdx.x % kSumColumns, y = threadIdx.x / kSumColumns;
-  const uint64_t c = (uint64_t)blockIdx.x * kSumColumns + x, columns = 2 * (uint64_t)width;
+// out the rows and join their sums through LDS, in an order that depends on nothing but the sizes.  A thread has eight loads under
+// way: what it waits for is the memory, the rows having been written by other XCDs.  With few columns a block takes 16 of them,
+// to have more threads per column; with many 32, whole cache lines.
+constexpr int kSumThreads = 1024;
+template <typename W, int COLUMNS>
+__global__ __launch_bounds__(kSumThreads) void sum_partial(const float *__restrict__ partial, uint32_t blocks, uint32_t width, W *dweight, W *dbias) {
+  constexpr uint32_t ROWS = kSumThreads / COLUMNS, LOADS = 8;
+  __shared__ float sums[ROWS][COLUMNS + 1];
+  const uint32_t x = threadIdx.x % COLUMNS, y = threadIdx.x / COLUMNS;
+  const uint64_t c = (uint64_t)blockIdx.x * COLUMNS + x, columns = 2 * (uint64_t)width;
   float sum = 0.f;
-  if (c < columns) {
-#pragma unroll 8
-    for (uint32_t i = y; i < blocks; i += kSumRows) sum += partial[i * columns + c];
+  for (uint32_t i = y; i < blocks; i += ROWS * LOADS) {
+    float v[LOADS];
+#pragma unroll
+    for (uint32_t k = 0; k < LOADS; k++) v[k] = c < columns && i + k * ROWS < blocks ? partial[(i + k * ROWS) * columns + c] : 0.f;
+#pragma unroll
+    for (uint32_t k = 0; k < LOADS; k++) sum += v[k];
   }
   sums[y][x] = sum;
   __syncthreads();
   if (y || c >= columns) return;
+  sum = 0.f;
 #pragma unroll
-  for (int i = 1; i < kSumRows; i++) sum += sums[i][x];
+  for (uint32_t i = 0; i < ROWS; i++) sum += sums[i][x];
   if (c < width) {
     if (dweight) dweight[c] = (W)sum;
   } else if (dbias) {
@@ -33,9 +39,12 @@ __global__ __launch_bounds__(kSumColumns * kSumRows) void sum_partial(const floa
 }
 
 template <typename W> void launch_sum(const hctr_norm_grad_args &a, unsigned blocks, hipStream_t s) {
-  hipLaunchKernelGGL(sum_partial<W>, dim3(div_up(2 * a.width, kSumColumns)), dim3(kSumColumns * kSumRows), 0, s,
-                     (const float *)a.workspace, blocks,
-                     (uint32_t)a.width, (W *)a.dweight, (W *)a.dbias);
+  const auto launch = [&](auto kernel, unsigned columns) {
+    hipLaunchKernelGGL(kernel, dim3(div_up(2 * a.width, columns)), dim3(kSumThreads), 0, s, (const float *)a.workspace, blocks, (uint32_t)a.width,
+                       (W *)a.dweight, (W *)a.dbias);
+  };
+  if (a.width <= 2048) launch(sum_partial<W, 16>, 16);
+  else launch(sum_partial<W, 32>, 32);
   HCTR_HIP(hipGetLastError());
 }
 

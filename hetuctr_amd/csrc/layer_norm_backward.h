@@ -203,12 +203,7 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < ITEMS; i++)
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-          const uint32_t c = first + i * GROUP * V + j;
-          if (c < a.width) row[c] = sums[i].v[j];
-        }
+      for (int i = 0; i < ITEMS; i++) store_columns<V, R>(row, first + i * GROUP * V, a.width, sums[i]);
     }
   };
   join(dweight, out);
