@@ -1,5 +1,6 @@
 """Builds the native parts in-tree: libhetuctr_hip.so (HIP kernels + C ABI, gfx950) and the pybind11 module
-`hetuCTR` that mirrors the reference's python surface (csrc/pybind/pybind.cu:42-79) on top of the C ABI.
+`hetuCTR` that mirrors the reference's python surface (csrc/pybind/pybind.cu:42-79) on top of the C ABI, and the module
+`hetuctr_nn` with the dense operators on torch tensors.
 
     python -m hetuctr_amd.build            # build what is missing or out of date
     python -m hetuctr_amd.build --force    # rebuild everything
@@ -24,6 +25,7 @@ HIPFLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contrac
 # host code of the partitioner's sweeps: AVX2 (no fused multiply-add is formed: contraction is off above)
 EXTRA_FLAGS = {"partition.hip": ["-Xarch_host", "-march=x86-64-v3"], "host_copy.hip": ["-Xarch_host", "-march=x86-64-v3"]}
 LIB = os.path.join(LIBDIR, "libhetuctr_hip.so")
+NNMOD = os.path.join(LIBDIR, "hetuctr_nn" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 PYMOD = os.path.join(LIBDIR, "hetuCTR" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 
@@ -83,9 +85,29 @@ def build_pymod(force=False, verbose=True):
     return PYMOD
 
 
+def build_nn(force=False, verbose=True):
+    src = os.path.join(CSRC, "nn_module.cpp")
+    if force or not _newer(NNMOD, [src, os.path.join(HERE, "..", "include", "hetuctr_hip.h")]):
+        import torch
+        from torch.utils import cpp_extension
+        inc = ["-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(HERE, "..", "include")]
+        inc += [x for path in cpp_extension.include_paths() for x in ("-isystem", path)]
+        lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+              "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch.compiled_with_cxx11_abi()] + inc +
+             [src, "-o", NNMOD, "-L" + LIBDIR, "-lhetuctr_hip", "-Wl,-rpath,$ORIGIN", "-L" + lib, "-ltorch_python", "-ltorch_cpu",
+              "-lc10", "-Wl,-rpath," + lib])
+        if verbose:
+            print("built", NNMOD, flush=True)
+    return NNMOD
+
+
 def build_all(force=False, verbose=True):
-    build_hip(force, verbose)
-    build_pymod(force, verbose)
+    with ThreadPoolExecutor(max_workers=1) as ex:
+        build_hip(force, verbose)
+        nn = ex.submit(build_nn, force, verbose)
+        build_pymod(force, verbose)
+        nn.result()
 
 
 if __name__ == "__main__":

@@ -15,6 +15,7 @@ from tests import dense_reference as ref
 
 gpu = pytest.mark.gpu
 TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+CODES = {"f32": capi.F32, "bf16": capi.BF16, "f16": capi.F16}
 PAIRS = [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("f32", "bf16"), ("f32", "f16")]
 ROW, COLUMN = 64 * 2.0 ** -24, 256 * 2.0 ** -24
 EPS = 1e-5
@@ -448,7 +449,7 @@ def test_norms_of_any_layout(width, stream, act):
     # results of the C entry point that are columns of a wider matrix leave the rest of it alone
     wider = torch.full((rows, width + 5), 7.0, dtype=TYPES[act], device="cuda")
     capi.layer_norm(rows, width, (r.data_ptr(), width), (wider[:, 2:].data_ptr(), width + 5), w.data_ptr(), b.data_ptr(), 0, 0,
-                    (0.3, 4, 4, 0), 1e-5, (nn._DTYPES[r.dtype], nn._DTYPES[TYPES[act]], capi.F32), torch.cuda.current_stream().cuda_stream)
+                    (0.3, 4, 4, 0), 1e-5, (CODES[stream], CODES[act], capi.F32), torch.cuda.current_stream().cuda_stream)
     assert torch.equal(wider[:, 2:width + 2], want[0]) and (wider[:, :2] == 7).all() and (wider[:, width + 2:] == 7).all()
 
 
