@@ -568,6 +568,21 @@ def test_rows_of_a_table_through_the_norm_and_back():
     t.close()
 
 
+@gpu
+def test_the_example_learns():
+    # the labels are a function of the ids: a model that gets the table's rows, and sends it their gradients, learns them; one that
+    # could not would stay at log 2
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "examples", "train_dense.py")
+    spec = importlib.util.spec_from_file_location("train_dense", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses = example.train(steps=60, samples=1024)
+    assert np.isfinite(losses).all()
+    assert np.mean(losses[-10:]) < 0.9 * np.log(2) < np.mean(losses[:3])
+
+
 # ---- refusals ---------------------------------------------------------------------------------------------------------------
 
 def test_the_c_entry_points_refuse_what_they_cannot_do():
