@@ -16,14 +16,18 @@ struct Dropping {
   uint32_t last;            // words up to this one drop their value
 };
 
-// V values that begin at column c (a multiple of four) of row r, dropped or scaled.  A dropped value becomes zero whatever it
-// was: it is never multiplied.
-template <int V> __device__ __forceinline__ void drop_columns(Floats<V> &f, const Dropping &d, uint64_t step, uint64_t quad) {
+// V values that begin at column c (a multiple of four) of row r, quad = r * quads + c / 4: dropped, or kept and, if SCALED,
+// multiplied by the scale.  A dropped value becomes zero whatever it was: it is never multiplied.
+template <bool SCALED = true, int V>
+__device__ __forceinline__ void drop_columns(Floats<V> &f, const Dropping &d, uint64_t step, uint64_t quad) {
 #pragma unroll
   for (int q = 0; q < V / 4; q++) {
     const Quad w = philox(quad + q, step, d.seed);
 #pragma unroll
-    for (int j = 0; j < 4; j++) f.v[4 * q + j] = w.w[j] > d.last ? f.v[4 * q + j] * d.scale : 0.f;
+    for (int j = 0; j < 4; j++) {
+      const float kept = SCALED ? f.v[4 * q + j] * d.scale : f.v[4 * q + j];
+      f.v[4 * q + j] = w.w[j] > d.last ? kept : 0.f;
+    }
   }
 }
 

@@ -7,29 +7,36 @@
 
 namespace hctr {
 
-// The sum of v over each group of LANES neighbouring lanes, the same bits in all of them: every step adds what two halves
-// hold, in either order.  Quads and rows of 16 lanes take it in data-parallel moves, wider groups by swapping rows or halves
-// of the wave between two registers; none of it goes through LDS.
-template <int LANES> __device__ __forceinline__ float group_sum(float v) {
+// The sums of v[0], v[1], .. over each group of LANES neighbouring lanes, the same bits in all of them: every step adds what two
+// halves hold, in either order.  Quads and rows of 16 lanes take it in data-parallel moves, wider groups by swapping rows or
+// halves of the wave between two registers; none of it goes through LDS, and the sums fill each other's waits.
+template <int LANES, int N> __device__ __forceinline__ void group_sums(float (&v)[N]) {
   static_assert(LANES >= 2 && LANES <= kWave && (LANES & (LANES - 1)) == 0, "lanes of a group");
-  const auto moved = [](float x, auto ctrl) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true));
+  const auto move = [&](auto ctrl) {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+      v[i] += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v[i]), decltype(ctrl)::value, 0xf, 0xf, true));
   };
-  v += moved(v, std::integral_constant<int, 0xB1>()); // lane ^ 1
-  if constexpr (LANES >= 4) v += moved(v, std::integral_constant<int, 0x4E>()); // lane ^ 2
-  if constexpr (LANES >= 8) v += moved(v, std::integral_constant<int, 0x141>()); // 7 - lane, of 8
-  if constexpr (LANES >= 16) v += moved(v, std::integral_constant<int, 0x140>()); // 15 - lane, of 16
-  if constexpr (LANES >= 32) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
-    const unsigned low = r[0], high = r[1]; // (the cast of an element itself takes the first one)
-    v = __builtin_bit_cast(float, low) + __builtin_bit_cast(float, high);
-  }
-  if constexpr (LANES >= 64) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
-    const unsigned low = r[0], high = r[1]; // (the cast of an element itself takes the first one)
-    v = __builtin_bit_cast(float, low) + __builtin_bit_cast(float, high);
-  }
-  return v;
+  // (r[0] and r[1] go through integers of their own: the cast of an element itself takes the first one)
+  const auto swap = [&](auto f) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const auto r = f(__builtin_bit_cast(unsigned, v[i]));
+      const unsigned low = r[0], high = r[1];
+      v[i] = __builtin_bit_cast(float, low) + __builtin_bit_cast(float, high);
+    }
+  };
+  move(std::integral_constant<int, 0xB1>());                            // lane ^ 1
+  if constexpr (LANES >= 4) move(std::integral_constant<int, 0x4E>());  // lane ^ 2
+  if constexpr (LANES >= 8) move(std::integral_constant<int, 0x141>()); // 7 - lane, of 8
+  if constexpr (LANES >= 16) move(std::integral_constant<int, 0x140>()); // 15 - lane, of 16
+  if constexpr (LANES >= 32) swap([](unsigned x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false); });
+  if constexpr (LANES >= 64) swap([](unsigned x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false); });
+}
+template <int LANES> __device__ __forceinline__ float group_sum(float v) {
+  float one[1] = {v};
+  group_sums<LANES>(one);
+  return one[0];
 }
 
 // The sum of v over the NT threads of a block, the same in all of them.  `smem` needs NT / 64 floats; the barriers inside keep
@@ -43,6 +50,16 @@ template <int NT> __device__ __forceinline__ float block_sum(float v, float *sme
 #pragma unroll
   for (int i = 0; i < NT / kWave; i++) v += smem[i];
   return v;
+}
+
+// (first + group) * stride, where first and stride are the same in all lanes, and the group is too if UNIFORM.  The lanes are spared
+// the product of two 64-bit numbers that scalar arithmetic can do (it takes them nine multiplications' time, as much as a
+// round of the draws), and kept apart, so that the compiler does not put the two products together again.
+template <bool UNIFORM> __device__ __forceinline__ int64_t rows_away(uint64_t first, uint32_t group, int64_t stride) {
+  int64_t own = (int64_t)group * stride;
+  if constexpr (UNIFORM) asm("" : "+s"(own));
+  else asm("" : "+v"(own));
+  return (int64_t)first * stride + own;
 }
 
 // Columns of weight or bias, ITEMS pieces that lie `apart` columns from each other: `narrow`, they are of type A, else float;
@@ -62,6 +79,13 @@ __device__ __forceinline__ void load_affine(Floats<V> (&f)[ITEMS], const void *p
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) f[i] = load_columns<V, R, false>((const float *)p, c + i * apart, width);
   }
+}
+
+template <int V, int ITEMS> __device__ __forceinline__ void scale_all(Floats<V> (&f)[ITEMS], float scale) {
+#pragma unroll
+  for (int i = 0; i < ITEMS; i++)
+#pragma unroll
+    for (int j = 0; j < V; j++) f[i].v[j] *= scale;
 }
 
 constexpr int kWideBlock = 256; // threads of a block that reads its row again and again
@@ -95,7 +119,8 @@ template <typename S, typename F> bool rows_in_registers(uint32_t width, F &&f) 
   const Held h = held_by(width, V);
   const auto with = [&](auto lanes, auto items) {
     if (h.lanes != lanes || h.items != items) return false;
-    if (width % V) f(std::integral_constant<Rows, Rows::kRagged>(), lanes, items);
+    // (what more than two lanes hold has more than two pieces)
+    if (width % V) f(std::integral_constant<Rows, decltype(lanes)::value == 2 ? Rows::kTiny : Rows::kRagged>(), lanes, items);
     else f(std::integral_constant<Rows, Rows::kEven>(), lanes, items);
     return true;
   };

@@ -93,7 +93,11 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
   uint32_t first = wave * GROUP * V * ITEMS + lane * V;
   const uint64_t step = DROP ? step_of(a.drop) : 0, stride = (uint64_t)gridDim.x * GROUPS;
   Floats<V> w[ITEMS], dweight[ITEMS], dbias[ITEMS];
-  if constexpr (!TIGHT) load_affine<V, A, R>(w, a.weight, a.narrow, first, GROUP * V, a.width, 1.f);
+  const auto fetch_weight = [&] {
+    load_affine<V, A, R>(w, a.weight, a.narrow, first, GROUP * V, a.width, 1.f);
+    if constexpr (DROP && !ADD) scale_all(w, a.drop.scale); // what is kept is scaled with it
+  };
+  if constexpr (!TIGHT) fetch_weight();
 #pragma unroll
   for (int i = 0; i < ITEMS; i++) {
 #pragma unroll
@@ -122,11 +126,11 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
     if constexpr (TIGHT) {
       asm volatile("" : "+v"(first)); // no address is worked out, and kept, before the loop
       fetch(r);
-      load_affine<V, A, R>(w, a.weight, a.narrow, first, GROUP * V, a.width, 1.f);
+      fetch_weight();
     }
     Floats<V> g[ITEMS], h[ITEMS];
     typename Packed<S, V>::type more[ITEMS];
-    float sum_g = 0.f, sum_gh = 0.f;
+    float sums[2] = {0.f, 0.f}; // of g and of g * h
     const float scale = rstd;
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
@@ -140,27 +144,26 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
     if (!TIGHT && r + stride < a.rows) fetch(r + stride);
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
-      if constexpr (DROP && !ADD) drop_columns(g[i], a.drop, step, r * a.drop.quads + (first + i * GROUP * V) / 4);
+      if constexpr (DROP && !ADD) drop_columns<false>(g[i], a.drop, step, r * a.drop.quads + (first + i * GROUP * V) / 4);
 #pragma unroll
       for (int j = 0; j < V; j++) { // columns behind the end have no gradient, and add nothing
         dweight[i].v[j] = fmaf(g[i].v[j], h[i].v[j], dweight[i].v[j]);
         dbias[i].v[j] += g[i].v[j];
         g[i].v[j] *= w[i].v[j];
-        sum_g += g[i].v[j];
-        sum_gh = fmaf(g[i].v[j], h[i].v[j], sum_gh);
+        sums[0] += g[i].v[j];
+        sums[1] = fmaf(g[i].v[j], h[i].v[j], sums[1]);
       }
     }
-    sum_g = group_sum<GROUP>(sum_g);
-    sum_gh = group_sum<GROUP>(sum_gh);
+    group_sums<GROUP>(sums);
     if constexpr (WAVES > 1) {
-      if (lane == 0) found[turn][wave] = make_float2(sum_g, sum_gh);
+      if (lane == 0) found[turn][wave] = make_float2(sums[0], sums[1]);
       __syncthreads();
       const float2 other = found[turn][lane % WAVES]; // every lane takes one wave's
-      sum_g = group_sum<WAVES>(other.x);
-      sum_gh = group_sum<WAVES>(other.y);
+      sums[0] = other.x, sums[1] = other.y;
+      group_sums<WAVES>(sums);
       turn ^= 1;
     }
-    const float mean_g = sum_g * a.inv_width, mean_gh = sum_gh * a.inv_width;
+    const float mean_g = sums[0] * a.inv_width, mean_gh = sums[1] * a.inv_width;
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
       if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
@@ -186,14 +189,18 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
     }
   }
   if (!a.partial) return;
+  if constexpr (DROP && !ADD) {
+    scale_all(dweight, a.drop.scale);
+    scale_all(dbias, a.drop.scale);
+  }
   float *out = a.partial + (uint64_t)blockIdx.x * 2 * a.width;
-  const auto join = [&](Floats<V> (&sums)[ITEMS], float *row) { // in the order of the groups, and one row of results
+  const auto join = [&](Floats<V> (&own)[ITEMS], float *row) { // in the order of the groups, and one row of results
     if constexpr (GROUPS > 1) {
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < ITEMS; i++)
 #pragma unroll
-        for (int j = 0; j < V; j++) joined[threadIdx.x / LANES * (LANES * ITEMS * V) + (i * GROUP + lane) * V + j] = sums[i].v[j];
+        for (int j = 0; j < V; j++) joined[threadIdx.x / LANES * (LANES * ITEMS * V) + (i * GROUP + lane) * V + j] = own[i].v[j];
       __syncthreads();
       for (uint32_t c = threadIdx.x; c < a.width; c += BLOCK) {
         float sum = 0.f;
@@ -203,7 +210,7 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < ITEMS; i++) store_columns<V, R>(row, first + i * GROUP * V, a.width, sums[i]);
+      for (int i = 0; i < ITEMS; i++) store_columns<V, R>(row, first + i * GROUP * V, a.width, own[i]);
     }
   };
   join(dweight, out);

@@ -78,37 +78,54 @@ __global__ __launch_bounds__(block_of<LANES>) void norm_rows(NormForward a) {
   __shared__ float2 found[2][WAVES]; // by turns, so that one barrier per row will do
   const uint32_t lane = threadIdx.x % GROUP, wave = WAVES > 1 ? threadIdx.x / kWave : 0;
   uint32_t first = wave * STRETCH + lane * V;
-  const uint64_t step = DROP ? step_of(a.drop) : 0, stride = (uint64_t)gridDim.x * (GROUPS * ROWS);
-  uint64_t r0 = (uint64_t)blockIdx.x * (GROUPS * ROWS) + threadIdx.x / LANES;
+  const uint64_t step = DROP ? step_of(a.drop) : 0;
   typedef std::conditional_t<ADD, A, S> X;
   typename Packed<X, V>::type x[ROWS][ITEMS];
   typename Packed<S, V>::type residual[ROWS][ITEMS];
   Floats<V> w[ITEMS], b[ITEMS];
-  const auto row = [&](int k) { return r0 + (uint64_t)(k * GROUPS); };
+  // The group's rows are r0, r0 + GROUPS, .., and r0 moves on by `stride`; their addresses move with it.
+  const uint64_t block0 = (uint64_t)blockIdx.x * (GROUPS * ROWS), stride = (uint64_t)gridDim.x * (GROUPS * ROWS);
+  constexpr bool UNIFORM = LANES >= kWave;
+  const uint32_t group = GROUPS == 1 ? 0 : UNIFORM ? __builtin_amdgcn_readfirstlane(threadIdx.x / LANES) : threadIdx.x / LANES;
+  uint64_t r0 = block0 + group, quad = DROP ? rows_away<UNIFORM>(block0, group, a.drop.quads) : 0;
+  S *ps = ADD ? (S *)a.sum + rows_away<UNIFORM>(block0, group, a.sum_stride) : nullptr;
+  A *py = (A *)a.y + rows_away<UNIFORM>(block0, group, a.y_stride);
   // a row that is not there is one of no columns
-  const auto width = [&](int k) { return k == 0 || row(k) < a.rows ? a.width : 0; };
-  const auto fetch = [&] {
+  const auto width = [&](int k, uint64_t r) { return k == 0 || r + k * GROUPS < a.rows ? a.width : 0; };
+  const X *px = (const X *)a.x + rows_away<UNIFORM>(block0, group, a.x_stride);
+  const S *pr = ADD ? (const S *)a.residual + rows_away<UNIFORM>(block0, group, a.residual_stride) : nullptr;
+  const auto fetch = [&](uint64_t r) {
+    if constexpr (STAYS) { // ahead of the loop
+      px = (const X *)a.x + (int64_t)r * a.x_stride;
+      pr = ADD ? (const S *)a.residual + (int64_t)r * a.residual_stride : nullptr;
+    }
 #pragma unroll
     for (int k = 0; k < ROWS; k++)
 #pragma unroll
       for (int i = 0; i < ITEMS; i++) {
         const uint32_t c = first + i * GROUP * V;
-        x[k][i] = load_raw<V, R>((const X *)a.x + (int64_t)row(k) * a.x_stride, c, width(k));
-        if constexpr (ADD) residual[k][i] = load_raw<V, R>((const S *)a.residual + (int64_t)row(k) * a.residual_stride, c, width(k));
+        x[k][i] = load_raw<V, R>(px + k * GROUPS * a.x_stride, c, width(k, r));
+        if constexpr (ADD) residual[k][i] = load_raw<V, R>(pr + k * GROUPS * a.residual_stride, c, width(k, r));
       }
+    px += (int64_t)stride * a.x_stride;
+    if constexpr (ADD) pr += (int64_t)stride * a.residual_stride;
   };
   const auto fetch_affine = [&] {
     load_affine<V, A, R>(w, a.weight, a.narrow, first, GROUP * V, a.width, 1.f);
     load_affine<V, A, R>(b, a.bias, a.narrow, first, GROUP * V, a.width, 0.f);
+    if constexpr (DROP && !ADD) { // what is kept is scaled with them
+      scale_all(w, a.drop.scale);
+      scale_all(b, a.drop.scale);
+    }
   };
   if (STAYS && r0 < a.rows) {
-    fetch();
+    fetch(r0);
     fetch_affine();
   }
   for (int turn = 0; r0 < a.rows; r0 += stride, turn ^= 1) {
     if constexpr (!STAYS) {
       asm volatile("" : "+v"(first)); // no address is worked out, and kept, before the loop
-      fetch();
+      fetch(r0);
       fetch_affine();
     }
     Floats<V> f[ROWS][ITEMS];
@@ -120,69 +137,79 @@ __global__ __launch_bounds__(block_of<LANES>) void norm_rows(NormForward a) {
         f[k][i] = floats<V>(settled<V, R>(x[k][i], c, a.width));
         if constexpr (ADD) {
           const Floats<V> g = floats<V>(settled<V, R>(residual[k][i], c, a.width));
-          if constexpr (DROP) drop_columns(f[k][i], a.drop, step, row(k) * a.drop.quads + c / 4);
+          if constexpr (DROP) drop_columns(f[k][i], a.drop, step, quad + k * GROUPS * a.drop.quads + c / 4);
 #pragma unroll
           for (int j = 0; j < V; j++) f[k][i].v[j] += g.v[j];
-          store_columns<V, R>((S *)a.sum + (int64_t)row(k) * a.sum_stride, c, width(k), f[k][i]);
+          store_columns<V, R>(ps + k * GROUPS * a.sum_stride, c, width(k, r0), f[k][i]);
         }
       }
-    if (STAYS && r0 + stride < a.rows) {
-      r0 += stride;
-      fetch();
-      r0 -= stride;
-    }
-    float mean[ROWS], rstd[ROWS];
+    if (STAYS && r0 + stride < a.rows) fetch(r0 + stride);
+    float sum[ROWS], square[ROWS], mean[ROWS], rstd[ROWS];
 #pragma unroll
     for (int k = 0; k < ROWS; k++) {
-      float sum = 0.f;
+      sum[k] = 0.f;
 #pragma unroll
       for (int i = 0; i < ITEMS; i++)
 #pragma unroll
-        for (int j = 0; j < V; j++) sum += f[k][i].v[j];
-      sum = group_sum<GROUP>(sum);
-      const float n = WAVES > 1 ? (float)min(a.width - min(a.width, wave * STRETCH), STRETCH) : 0.f;
-      mean[k] = WAVES > 1 ? sum / fmaxf(n, 1.f) : sum * a.inv_width;
-      // columns behind the end hold zeros and have to add nothing to the squares
-      float square = 0.f;
+        for (int j = 0; j < V; j++) sum[k] += f[k][i].v[j];
+    }
+    group_sums<GROUP>(sum);
+    const float n = WAVES > 1 ? (float)min(a.width - min(a.width, wave * STRETCH), STRETCH) : 0.f;
+#pragma unroll
+    for (int k = 0; k < ROWS; k++) {
+      mean[k] = WAVES > 1 ? sum[k] / fmaxf(n, 1.f) : sum[k] * a.inv_width;
+      square[k] = 0.f;
 #pragma unroll
       for (int i = 0; i < ITEMS; i++) {
         const uint32_t c = first + i * GROUP * V;
 #pragma unroll
         for (int j = 0; j < V; j++) {
+          // columns behind the end hold zeros and have to add nothing to the squares
           const float d = f[k][i].v[j] - ((R == Rows::kEven ? c : c + j) < a.width ? mean[k] : 0.f);
-          square = fmaf(d, d, square);
+          square[k] = fmaf(d, d, square[k]);
+          if constexpr (WAVES == 1) f[k][i].v[j] = d;
         }
       }
-      square = group_sum<GROUP>(square);
-      if constexpr (WAVES > 1) {
-        if (lane == 0) found[turn][wave] = make_float2(sum, square);
-        __syncthreads();
-        // every lane takes one wave's
-        const float2 other = found[turn][lane % WAVES];
-        const float m = (float)min(a.width - min(a.width, lane % WAVES * STRETCH), STRETCH);
-        mean[k] = group_sum<WAVES>(other.x) * a.inv_width;
-        const float off = other.x / fmaxf(m, 1.f) - mean[k];
-        square = group_sum<WAVES>(fmaf(m * off, off, other.y));
-      }
-      rstd[k] = rsqrtf(fmaf(square, a.inv_width, a.eps));
     }
+    group_sums<GROUP>(square);
+    if constexpr (WAVES > 1) {
+      if (lane == 0) found[turn][wave] = make_float2(sum[0], square[0]);
+      __syncthreads();
+      // every lane takes one wave's
+      const float2 other = found[turn][lane % WAVES];
+      const float m = (float)min(a.width - min(a.width, lane % WAVES * STRETCH), STRETCH);
+      mean[0] = group_sum<WAVES>(other.x) * a.inv_width;
+      const float off = other.x / fmaxf(m, 1.f) - mean[0];
+      square[0] = group_sum<WAVES>(fmaf(m * off, off, other.y));
+#pragma unroll
+      for (int i = 0; i < ITEMS; i++)
+#pragma unroll
+        for (int j = 0; j < V; j++) f[0][i].v[j] -= mean[0];
+    }
+#pragma unroll
+    for (int k = 0; k < ROWS; k++) rstd[k] = rsqrtf(fmaf(square[k], a.inv_width, a.eps));
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
       const uint32_t c = first + i * GROUP * V;
 #pragma unroll
       for (int k = 0; k < ROWS; k++) {
 #pragma unroll
-        for (int j = 0; j < V; j++) f[k][i].v[j] = fmaf((f[k][i].v[j] - mean[k]) * rstd[k], w[i].v[j], b[i].v[j]);
-        if constexpr (DROP && !ADD) drop_columns(f[k][i], a.drop, step, row(k) * a.drop.quads + c / 4);
-        store_columns<V, R>((A *)a.y + (int64_t)row(k) * a.y_stride, c, width(k), f[k][i]);
+        for (int j = 0; j < V; j++) f[k][i].v[j] = fmaf(f[k][i].v[j] * rstd[k], w[i].v[j], b[i].v[j]);
+        if constexpr (DROP && !ADD) drop_columns<false>(f[k][i], a.drop, step, quad + k * GROUPS * a.drop.quads + c / 4);
+        store_columns<V, R>(py + k * GROUPS * a.y_stride, c, width(k, r0), f[k][i]);
       }
     }
+    if (threadIdx.x % LANES == 0) {
 #pragma unroll
-    for (int k = 0; k < ROWS; k++)
-      if (threadIdx.x % LANES == 0 && width(k)) {
-        if (a.mean) a.mean[row(k)] = mean[k];
-        if (a.rstd) a.rstd[row(k)] = rstd[k];
-      }
+      for (int k = 0; k < ROWS; k++)
+        if (width(k, r0)) {
+          if (a.mean) a.mean[r0 + k * GROUPS] = mean[k];
+          if (a.rstd) a.rstd[r0 + k * GROUPS] = rstd[k];
+        }
+    }
+    quad += stride * a.drop.quads;
+    py += (int64_t)stride * a.y_stride;
+    if constexpr (ADD) ps += (int64_t)stride * a.sum_stride;
   }
 }
 
@@ -194,8 +221,8 @@ template <typename S, typename A, bool ADD, bool DROP> void launch(const NormFor
     // their loads empty.  us with one row and with four, 2^27 values: float to bfloat16, dropped, 16 columns 155, 131, 64
     // columns 156, 132, 256 columns 160, 139; float, 37 columns 313, 226; bfloat16, 64 columns 96, 92.  Elsewhere four are no
     // better or worse: float, 64 columns 175, 179, 256 columns 179, 194; a branch added, float and bfloat16, 256 columns 265, 283.
-    constexpr bool FOUR = LANES <= kWave && ITEMS == 1 && (R == Rows::kRagged || (!ADD && (DROP || sizeof(S) == 2)));
-    constexpr int ROWS = FOUR ? 4 : 1, PER = BLOCK / LANES * ROWS;
+    constexpr bool FOUR = LANES <= kWave && ITEMS == 1 && (R != Rows::kEven || (!ADD && (DROP || sizeof(S) == 2)));
+    constexpr int ROWS = FOUR ? 4 : LANES <= kWave && ITEMS == 2 && R == Rows::kRagged && !stays<S, LANES, ITEMS> ? 2 : 1, PER = BLOCK / LANES * ROWS;
     // Blocks that stay: as many per CU as fetch 16 KiB at a time, or sixteen where the draws' arithmetic wants them.  us for 2^27
     // values with 256, 512, 1024, 4096 blocks and with one for each row (chosen: *): float, 4096 columns 176*, 179, 184, 182, 195;
     // bfloat16, 2048 columns 197, 120, 92*, 98, 111, 8192 columns 90*, 91, 92, 93, 117; a branch added, float and bfloat16, 1024

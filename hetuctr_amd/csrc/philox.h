@@ -18,6 +18,15 @@ struct Quad {
   uint32_t w[4];
 };
 
+// a ^ b ^ c (one instruction, where the compiler makes two)
+__host__ __device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+#ifdef __HIP_DEVICE_COMPILE__
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);
+#else
+  return a ^ b ^ c;
+#endif
+}
+
 // the words of counter (quad, step), low words first, under `key`
 __host__ __device__ __forceinline__ Quad philox(uint64_t quad, uint64_t step, uint64_t key) {
   uint32_t c0 = (uint32_t)quad, c1 = (uint32_t)(quad >> 32), c2 = (uint32_t)step, c3 = (uint32_t)(step >> 32);
@@ -25,9 +34,9 @@ __host__ __device__ __forceinline__ Quad philox(uint64_t quad, uint64_t step, ui
 #pragma unroll
   for (int r = 0; r < kPhiloxRounds; r++) {
     const uint64_t a = kPhiloxMul0 * c0, b = kPhiloxMul1 * c2;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c0 = xor3((uint32_t)(b >> 32), c1, k0);
     c1 = (uint32_t)b;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c2 = xor3((uint32_t)(a >> 32), c3, k1);
     c3 = (uint32_t)a;
     k0 += kPhiloxKey0;
     k1 += kPhiloxKey1;

@@ -24,7 +24,8 @@ template <int V> struct Floats {
 // How a kernel reads and writes rows of `width` columns, V at a time.
 enum class Rows {
   kEven,   // short (their bytes can be counted in 32 bits), the width a multiple of V: past the caches, nothing reads them again
-  kRagged, // short, any width: rows share cache lines with their neighbours, which the caches put together
+  kRagged, // short, at least V columns: rows share cache lines with their neighbours, which the caches put together
+  kTiny,   // the same, any width
   kLong,   // any length and width
 };
 
@@ -51,7 +52,7 @@ __device__ __forceinline__ typename Packed<T, V>::type load_raw(const T *row, ui
   if constexpr (R == Rows::kEven) {
     if (c < width) load(c);
   } else if (c < width) {
-    if (width >= V) load(min(c, width - V));
+    if (R == Rows::kRagged || width >= V) load(min(c, width - V));
     else
 #pragma unroll
       for (int j = 0; j + 1 < V; j++)
@@ -61,7 +62,7 @@ __device__ __forceinline__ typename Packed<T, V>::type load_raw(const T *row, ui
 }
 template <int V, Rows R, typename X> __device__ __forceinline__ X settled(X x, uint32_t c, uint32_t width) {
   if constexpr (R != Rows::kEven)
-    if (c < width && c + V > width && width >= V) {
+    if (c < width && c + V > width && (R == Rows::kRagged || width >= V)) {
       const uint32_t by = V - width % V;
 #pragma unroll
       for (int k = 1; k < V; k *= 2)
