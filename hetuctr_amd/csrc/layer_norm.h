@@ -137,16 +137,17 @@ template <typename S, typename F> bool rows_in_registers(uint32_t width, F &&f) 
   return done;
 }
 
-// Blocks of the gradient's kernels, each of which writes a row of sums for weight and bias: as many per CU as fetch 18 KiB at a
+// Blocks of the gradient's kernels, each of which writes a row of sums for weight and bias: as many per CU as fetch 17 KiB at a
 // time (bytes: of a column's values, read), so few that the memory sees long stretches and the rows of sums are little beside the data, at
 // least one and at most eight.  us on an MI355X for 2^27 values with 256, 512, 768, 1024 blocks (chosen: *): float, 64
 // columns 411, 287, 274*, 290; 1024 columns 268*, 286, 282, 286; bfloat16, 4096 columns 152, 151*, 160, 159; float and bfloat16,
 // dropped, 128 columns 665, 262, 230*, 244; the same with a branch added, 512 columns 354*, 386, 408, 423; 2048 columns 354*, 377,
-// 411, 431; 4096 rows of 8192 halves 51*, 63, 74, 86; 37 columns, dropped, with 768, 1536, 2048 493, 323*, 401.
+// 411, 431; 4096 rows of 8192 halves 51*, 63, 74, 86; 1.2e8 values in rows of 37
+// with 768, 1024, 1280, 1536: dropped 299, 287, 274*, 288, a branch added 420*, 466, 463, 475.
 inline unsigned norm_grad_blocks(uint64_t rows, uint32_t width, int V, int bytes) {
   const Held h = held_by(width, V);
   const uint64_t groups = h.lanes && h.lanes < 256 ? 256 / h.lanes : 1, fetch = groups * width * bytes;
-  const uint64_t per_cu = std::min<uint64_t>((18 * 1024 - 1) / fetch + 1, 8);
+  const uint64_t per_cu = std::min<uint64_t>((17 * 1024 - 1) / fetch + 1, 8);
   return (unsigned)std::min(256 * per_cu, (rows + groups - 1) / groups);
 }
 

@@ -160,6 +160,40 @@ def test_dropout_in_place_and_of_rows_far_apart():
 
 
 @gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows, width", [(50, 3), (40, 37), (7, 1443), (300, 12), (1, 1001)])
+def test_dropout_in_place_of_ragged_rows(rows, width, kind):
+    x = values((rows, width + 2), kind, 7)[:, :width]
+    drop = (0.4, 8, 2)
+    want = nn.dropout(x, nn.Drop(*drop))
+    at = (x.data_ptr(), width + 2)
+    capi.dropout(rows, width, at, at, drop + (0,), CODES[kind], torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(x, want)
+
+
+@gpu
+def test_counters_beyond_32_bits():
+    # 2^34 values and some: their quads, and with them the counter's low word, pass 2^32 in the last rows
+    width, rows = 1024, 2 ** 24 + 3
+    drop, quads = (0.3, 77, 5), width // 4
+    at = np.arange((rows - 4) * quads, rows * quads, dtype=np.uint64)
+    words = ref.philox([at & np.uint64(0xFFFFFFFF), at >> np.uint64(32), np.uint64(5), np.uint64(0)], (77, 0), 7)
+    keep = torch.from_numpy(words.T.reshape(4, width) >= np.uint64(round(0.3 * 2 ** 32)))
+    assert (at >> np.uint64(32)).max() == 1 and (at >> np.uint64(32)).min() == 0
+    want = torch.where(keep, torch.tensor(1 / 0.7, dtype=torch.float32).half(), torch.tensor(0.0).half())
+    x = torch.ones((rows, width), dtype=torch.float16, device="cuda")
+    place = (x.data_ptr(), width)
+    capi.dropout(rows, width, place, place, drop + (0,), capi.F16, torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(x[-4:].cpu(), want)
+    # rows without spread become their bias, which is dropped likewise
+    x.zero_()
+    y = nn.layer_norm(x, None, torch.ones(width, dtype=torch.float16, device="cuda"), drop=nn.Drop(*drop))
+    assert torch.equal(y[-4:].cpu(), want)
+    del x, y
+    torch.cuda.empty_cache()
+
+
+@gpu
 def test_step_tensor_is_added_to_the_step():
     x = values((20, 40), "f32", 6)
     for base, more in ((3, 4), (0, 2 ** 40), (2 ** 64 - 1, 2)):
