@@ -59,9 +59,11 @@ __global__ __launch_bounds__(kWideBlock) void norm_wide(NormForward a) {
   }
 }
 
-// Rows of more than 512 columns, but for those that leave no registers for the next one: a block stays for several.
-template <typename S, int LANES, int ITEMS>
-constexpr bool stays = LANES * ITEMS * kVec<S> > 512 && !(LANES == 1024 && ITEMS * kVec<S> == 16);
+// Rows of more than 512 columns: a block stays for several.
+template <typename S, int LANES, int ITEMS> constexpr bool stays = LANES * ITEMS * kVec<S> > 512;
+// The widest leave no registers for weight and bias beside the next row: every lane puts what it needs of them in LDS, 128 KiB
+// in all.  (Read again for every row they are more bytes than the row: 1.2e8 bfloat16 values in rows of 16384 124 us, 83 this way.)
+template <typename S, int LANES, int ITEMS> constexpr bool shelved = LANES == 1024 && ITEMS * kVec<S> == 16;
 
 // ITEMS pieces of V columns per lane of a row that LANES lanes hold in registers: the row is read once.  Up to a wave's
 // lanes, a group of lanes has a row to itself, ROWS of them at a time, and a block as many as it has groups; beyond that the waves of a
@@ -75,6 +77,8 @@ __global__ __launch_bounds__(block_of<LANES>) void norm_rows(NormForward a) {
   static_assert(WAVES == 1 || ROWS == 1, "a block that shares a row has one at a time");
   // Wide rows: a block stays for several, weight and bias in its registers, the next row on its way while one is worked on.
   constexpr bool STAYS = stays<S, LANES, ITEMS>;
+  constexpr bool SHELVED = shelved<S, LANES, ITEMS>;
+  __shared__ float4 shelf[SHELVED ? 2 * ITEMS * V / 4 * BLOCK : 1];
   __shared__ float2 found[2][WAVES]; // by turns, so that one barrier per row will do
   const uint32_t lane = threadIdx.x % GROUP, wave = WAVES > 1 ? threadIdx.x / kWave : 0;
   uint32_t first = wave * STRETCH + lane * V;
@@ -116,6 +120,16 @@ __global__ __launch_bounds__(block_of<LANES>) void norm_rows(NormForward a) {
     if constexpr (DROP && !ADD) { // what is kept is scaled with them
       scale_all(w, a.drop.scale);
       scale_all(b, a.drop.scale);
+    }
+    if constexpr (SHELVED) {
+#pragma unroll
+      for (int i = 0; i < ITEMS; i++)
+#pragma unroll
+        for (int q = 0; q < V / 4; q++) {
+          float4 *place = shelf + ((i * (V / 4) + q) * 2) * BLOCK + threadIdx.x; // no other lane's
+          place[0] = make_float4(w[i].v[4 * q], w[i].v[4 * q + 1], w[i].v[4 * q + 2], w[i].v[4 * q + 3]);
+          place[BLOCK] = make_float4(b[i].v[4 * q], b[i].v[4 * q + 1], b[i].v[4 * q + 2], b[i].v[4 * q + 3]);
+        }
     }
   };
   if (STAYS && r0 < a.rows) {
@@ -191,6 +205,14 @@ __global__ __launch_bounds__(block_of<LANES>) void norm_rows(NormForward a) {
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
       const uint32_t c = first + i * GROUP * V;
+      if constexpr (SHELVED) {
+#pragma unroll
+        for (int q = 0; q < V / 4; q++) {
+          const float4 *place = shelf + ((i * (V / 4) + q) * 2) * BLOCK + threadIdx.x, x4 = place[0], y4 = place[BLOCK];
+          w[i].v[4 * q] = x4.x, w[i].v[4 * q + 1] = x4.y, w[i].v[4 * q + 2] = x4.z, w[i].v[4 * q + 3] = x4.w;
+          b[i].v[4 * q] = y4.x, b[i].v[4 * q + 1] = y4.y, b[i].v[4 * q + 2] = y4.z, b[i].v[4 * q + 3] = y4.w;
+        }
+      }
 #pragma unroll
       for (int k = 0; k < ROWS; k++) {
 #pragma unroll
@@ -231,7 +253,7 @@ template <typename S, typename A, bool ADD, bool DROP> void launch(const NormFor
     uint64_t most = (1u << 31) / BLOCK;
     if constexpr (stays<S, LANES, ITEMS>) {
       const uint64_t fetch = (uint64_t)PER * p.width * (ADD ? sizeof(A) + sizeof(S) : sizeof(S));
-      most = 256 * (DROP && !ADD ? 16 : (16 * 1024 - 1) / fetch + 1);
+      most = 256 * (DROP && !ADD && !shelved<S, LANES, ITEMS> ? 16 : (16 * 1024 - 1) / fetch + 1);
     }
     const uint64_t blocks = std::min<uint64_t>((p.rows + PER - 1) / PER, most);
     hipLaunchKernelGGL((norm_rows<S, A, ADD, DROP, R, LANES, ITEMS, ROWS>), dim3((unsigned)blocks), dim3(BLOCK), 0, s, p);
