@@ -6,6 +6,8 @@ reference's table interface.
                         top-level ``hetuCTR`` after ``hetuctr_amd.install_as_hetuCTR()``)
 ``hetuctr_amd.partition`` the offline partitioner with the surface of the reference's ``hetuCTR_partition`` module
                         (importable under that name after ``hetuctr_amd.install_as_hetuCTR_partition()``)
+``hetuctr_amd.nn``      operators between the table's rows and a dense model on torch tensors: dropout, layer normalisation,
+                        both in one pass, and their gradients
 """
 import importlib
 import os
