@@ -56,7 +56,9 @@ struct NormBackward {
   const float *mean, *rstd;
   const void *weight;
   bool narrow;
-  float *partial; // [blocks][2][width] sums for weight and bias, or null
+  float *partial;       // [blocks][2][width] sums for weight and bias, or null
+  void *dweight, *dbias; // where blocks of their own make them (few rows); either may be null
+  uint32_t row_blocks;   // blocks behind these are the columns'
   Dropping drop;
 };
 

@@ -50,9 +50,15 @@ template <typename W> void launch_sum(const hctr_norm_grad_args &a, unsigned blo
 
 } // namespace
 
+// Few rows: weight and bias get blocks of their own, one launch does it all, and no workspace is needed.  A call's time in us with
+// two launches and with one, dropped (the draws, made again for every column, are what many rows cost): 128 columns, 1 to 512
+// rows 11.0, 6.8, 1024 rows 11.1, 10.3, 2048 rows 11.0, 18.3; 1024 columns, 512 rows 11.0, 6.9, 1024 rows 11.1, 18.2; 4096 columns,
+// 128 rows 11.1, 6.9, 512 rows 11.6, 20.7; 16384 columns, 1 row 10.8, 26.8.
+static bool few(size_t rows, size_t width) { return rows <= 512 && width <= 4096 && rows * width <= (1u << 19); }
+
 // The most that norm_grad_blocks says for any form and pair of types.
 size_t layer_norm_workspace(size_t rows, size_t width) {
-  if (!rows || !width || width >= (1u << 31)) return 0;
+  if (!rows || !width || width >= (1u << 31) || few(rows, width)) return 0;
   const uint32_t w = (uint32_t)width;
   return (size_t)std::max(norm_grad_blocks(rows, w, kVec<float>, 6), norm_grad_blocks(rows, w, kVec<bf16_t>, 4)) * 2 * width * sizeof(float);
 }
@@ -111,7 +117,7 @@ void layer_norm_backward(const hctr_norm_grad_args &a, bool add) {
     HCTR_CHECK(a.mean && a.rstd, "layer norm: mean and rstd of the forward pass are needed");
     if (!add || a.dx.data) check_matrix(a.dx, a.rows, a.width, true, "layer norm: dx");
     if (add && a.dresidual.data) check_matrix(a.dresidual, a.rows, a.width, true, "layer norm: dresidual");
-    HCTR_CHECK(!columns || (a.workspace && (uintptr_t)a.workspace % 16 == 0 && a.workspace_bytes >= layer_norm_workspace(a.rows, a.width)),
+    HCTR_CHECK(!columns || few(a.rows, a.width) || (a.workspace && (uintptr_t)a.workspace % 16 == 0 && a.workspace_bytes >= layer_norm_workspace(a.rows, a.width)),
                "layer norm: the workspace is missing, too small or not 16-byte aligned");
   }
   p.rows = a.rows;
@@ -127,7 +133,9 @@ void layer_norm_backward(const hctr_norm_grad_args &a, bool add) {
   p.mean = a.mean, p.rstd = a.rstd;
   p.weight = a.weight;
   p.narrow = a.affine_dtype != HCTR_F32;
-  p.partial = columns ? (float *)a.workspace : nullptr;
+  const bool alone = columns && a.rows && few(a.rows, a.width); // one launch does it all
+  if (alone) p.dweight = a.dweight, p.dbias = a.dbias;
+  else if (columns) p.partial = (float *)a.workspace;
   unsigned blocks = 0;
   if (a.rows) {
     if (a.stream_dtype == HCTR_BF16) blocks = launch_norm_grad<bf16_t, bf16_t>(p, add, on, s);
@@ -136,7 +144,7 @@ void layer_norm_backward(const hctr_norm_grad_args &a, bool add) {
     else if (a.act_dtype == HCTR_F16) blocks = launch_norm_grad<float, f16_t>(p, add, on, s);
     else blocks = launch_norm_grad<float, float>(p, add, on, s);
   }
-  if (!columns) return;
+  if (!columns || alone) return;
   if (a.affine_dtype == HCTR_F32) launch_sum<float>(a, blocks, s);
   else if (a.affine_dtype == HCTR_BF16) launch_sum<bf16_t>(a, blocks, s);
   else launch_sum<f16_t>(a, blocks, s);

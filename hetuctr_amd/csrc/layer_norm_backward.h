@@ -79,6 +79,49 @@ __global__ __launch_bounds__(kWideBlock) void grad_wide(NormBackward a) {
   }
 }
 
+// The gradients of weight and bias, of few rows: kColumns columns per block, whose threads share out the rows, read them for
+// themselves beside the blocks of rows, and join their sums through LDS.  Nothing has to be written in between, and no second
+// launch adds it up.
+constexpr uint32_t kColumns = 8;
+template <typename S, typename A, bool DROPPED, int BLOCK> __device__ __forceinline__ void sum_columns(const NormBackward &a, uint32_t block) {
+  constexpr uint32_t ROWS = BLOCK / kColumns, LOADS = 8;
+  __shared__ float2 sums[ROWS][kColumns];
+  const uint32_t x = threadIdx.x % kColumns, y = threadIdx.x / kColumns, c = block * kColumns + x;
+  const uint64_t step = DROPPED ? step_of(a.drop) : 0;
+  float w = 0.f, b = 0.f;
+  for (uint64_t r = y; r < a.rows; r += ROWS * LOADS) {
+    float g[LOADS], s[LOADS], mean[LOADS], rstd[LOADS];
+#pragma unroll
+    for (uint32_t k = 0; k < LOADS; k++) {
+      const uint64_t at = r + k * ROWS;
+      const bool there = at < a.rows && c < a.width;
+      g[k] = there ? (float)((const A *)a.dy)[(int64_t)at * a.dy_stride + c] : 0.f;
+      s[k] = there ? (float)((const S *)a.s)[(int64_t)at * a.s_stride + c] : 0.f;
+      mean[k] = there ? a.mean[at] : 0.f;
+      rstd[k] = there ? a.rstd[at] : 0.f;
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < LOADS; k++) {
+      if constexpr (DROPPED) {
+        const Quad q = philox((r + k * ROWS) * a.drop.quads + c / 4, step, a.drop.seed);
+        const uint32_t word = c % 4 < 2 ? (c % 4 == 0 ? q.w[0] : q.w[1]) : (c % 4 == 2 ? q.w[2] : q.w[3]);
+        g[k] = word > a.drop.last ? g[k] * a.drop.scale : 0.f;
+      }
+      w = fmaf(g[k], (s[k] - mean[k]) * rstd[k], w);
+      b += g[k];
+    }
+  }
+  sums[y][x] = make_float2(w, b);
+  __syncthreads();
+  if (threadIdx.x >= 2 * kColumns || c >= a.width) return; // the first kColumns threads add up dweight, the next dbias
+  float sum = 0.f;
+  for (uint32_t i = 0; i < ROWS; i++) sum += y ? sums[i][x].y : sums[i][x].x;
+  void *out = y ? a.dbias : a.dweight;
+  if (!out) return;
+  if (a.narrow) ((A *)out)[c] = (A)sum;
+  else ((float *)out)[c] = sum;
+}
+
 // The rows that a block works on, held in registers as by the forward pass (rows_in_registers): each is read once.  A lane has the
 // same columns of every row, so it keeps their sums for weight and bias in registers too, and the block's groups join theirs at
 // the end.  The next row is on its way while this one is worked on; where the waves of a block share a row, their two
@@ -86,12 +129,13 @@ __global__ __launch_bounds__(kWideBlock) void grad_wide(NormBackward a) {
 template <typename S, typename A, bool ADD, bool DROP, Rows R, int LANES, int ITEMS>
 __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
   constexpr int V = kVec<S>, BLOCK = block_of<LANES>, GROUP = LANES < kWave ? LANES : kWave, WAVES = LANES / GROUP, GROUPS = BLOCK / LANES;
+  if (blockIdx.x >= a.row_blocks) return sum_columns<S, A, DROP && !ADD, BLOCK>(a, blockIdx.x - a.row_blocks);
   constexpr bool TIGHT = LANES == 1024 && ITEMS * V == 16; // 128 registers: the row's own values and sums are all that fits
   __shared__ float2 found[2][WAVES];
   __shared__ float joined[GROUPS > 1 ? GROUPS * LANES * ITEMS * V : 1];
   const uint32_t lane = threadIdx.x % GROUP, wave = WAVES > 1 ? threadIdx.x / kWave : 0;
   uint32_t first = wave * GROUP * V * ITEMS + lane * V;
-  const uint64_t step = DROP ? step_of(a.drop) : 0, stride = (uint64_t)gridDim.x * GROUPS;
+  const uint64_t step = DROP ? step_of(a.drop) : 0, stride = (uint64_t)a.row_blocks * GROUPS;
   Floats<V> w[ITEMS], dweight[ITEMS], dbias[ITEMS];
   const auto fetch_weight = [&] {
     load_affine<V, A, R>(w, a.weight, a.narrow, first, GROUP * V, a.width, 1.f);
@@ -219,9 +263,12 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
 
 template <typename S, typename A, bool ADD, bool DROP> unsigned launch_grad(const NormBackward &p, hipStream_t s) {
   const unsigned blocks = norm_grad_blocks(p.rows, p.width, kVec<S>, (int)(sizeof(A) + sizeof(S) * (p.ds ? 2 : 1)));
+  NormBackward q = p;
+  q.row_blocks = blocks;
   const bool held = rows_in_registers<S>(p.width, [&](auto how, auto lanes, auto items) {
     constexpr int LANES = decltype(lanes)::value, ITEMS = decltype(items)::value, BLOCK = block_of<LANES>;
-    hipLaunchKernelGGL((grad_rows<S, A, ADD, DROP, decltype(how)::value, LANES, ITEMS>), dim3(blocks), dim3(BLOCK), 0, s, p);
+    const unsigned columns = p.dweight || p.dbias ? div_up(p.width, kColumns) : 0;
+    hipLaunchKernelGGL((grad_rows<S, A, ADD, DROP, decltype(how)::value, LANES, ITEMS>), dim3(blocks + columns), dim3(BLOCK), 0, s, q);
   });
   if (!held) hipLaunchKernelGGL((grad_wide<S, A, ADD, DROP>), dim3(blocks), dim3(kWideBlock), 0, s, p);
   HCTR_HIP(hipGetLastError());

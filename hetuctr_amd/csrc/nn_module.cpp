@@ -254,8 +254,10 @@ PyObject *backward(const Arguments &a) {
   r.dweight = pointer(dweight), r.dbias = pointer(dbias);
   if (dweight || dbias) {
     r.workspace_bytes = hctr_layer_norm_workspace(m.rows, m.width);
-    space = result({(int64_t)r.workspace_bytes}, s, at::kByte);
-    r.workspace = space->data_ptr();
+    if (r.workspace_bytes) {
+      space = result({(int64_t)r.workspace_bytes}, s, at::kByte);
+      r.workspace = space->data_ptr();
+    }
   }
   r.stream = a.stream(12);
   done(add ? hctr_dropout_add_layer_norm_backward(&r) : hctr_layer_norm_backward(&r));

@@ -294,8 +294,8 @@ int hctr_dropout_add_layer_norm(const hctr_norm_args *a);
  * hctr_layer_norm_backward writes d to dx, of stream_dtype.  hctr_dropout_add_layer_norm_backward adds dsum (stream_dtype, the
  * gradient that sum has from elsewhere; data NULL: none), writes d to dresidual (stream_dtype) and drop(d) to dx
  * (act_dtype); either result's data may be NULL.  dweight and dbias (affine_dtype, NULL: not wanted) are written, not
- * added to.  workspace: hctr_layer_norm_workspace(rows, width) bytes of device memory, 16-byte aligned, in use until the
- * work is done; needed if dweight or dbias is wanted. */
+ * added to.  workspace: hctr_layer_norm_workspace(rows, width) bytes of device memory (0 for few rows), 16-byte aligned, in
+ * use until the work is done; needed if dweight or dbias is wanted. */
 typedef struct hctr_norm_grad_args {
   size_t rows, width;
   hctr_matrix dy, s, dsum, dx, dresidual;

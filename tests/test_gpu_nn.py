@@ -344,6 +344,25 @@ def test_weight_gradient_over_many_rows_or_few(rows, width):
     assert last[1] is None and torch.equal(last[2], dbias)
 
 
+@gpu
+@pytest.mark.parametrize("stream, act", PAIRS)
+@pytest.mark.parametrize("rows, width", [(513, 3), (900, 12), (2000, 37), (1500, 64), (700, 333), (600, 1000), (530, 1443), (520, 2056),
+                                         (140, 4100), (100, 8192), (66, 16388)])
+def test_gradients_of_more_rows_than_one_launch_takes(rows, width, stream, act):
+    x, dy = values((rows, width), stream, 1, 0.5, 0.1), values((rows, width), act, 2, 0.01)
+    mean, rstd = (torch.from_numpy(t).float().cuda() for t in ref.statistics(wide(x), EPS))
+    weight, bias = affine("act", width, act)
+    drop = (0.25, 3, width)
+    f = ref.factors(rows, width, drop)
+    for g, got in ((wide(dy) * f, nn.layer_norm_backward(dy, x, mean, rstd, weight, bias, drop=nn.Drop(*drop))),
+                   (wide(dy), nn.dropout_add_layer_norm_backward(dy, x, x, mean, rstd, weight, bias, drop=nn.Drop(*drop))[1:])):
+        want, size = ref.gradient(g, wide(x), wide(mean), wide(rstd), wide(weight))
+        more = 0 if g.shape == f.shape and np.array_equal(g, wide(dy) * f) else wide(x)
+        check(got[0], want[0] + more, size[0] + np.abs(want[0] + more), ROW, "rows")
+        check(got[1], want[1], size[1], COLUMN, "dweight")
+        check(got[2], want[2], size[2], COLUMN, "dbias")
+
+
 # ---- gradients against differences ------------------------------------------------------------------------------------------
 def test_reference_gradient_against_differences():
     rng = np.random.default_rng(3)
@@ -643,13 +662,14 @@ def test_the_c_entry_points_refuse_what_they_cannot_do():
     for residual, total in ((none, m), (m, none), (m, (4096, 1))):
         with pytest.raises(RuntimeError, match="null|overlap"):
             capi.dropout_add_layer_norm(2, 8, m, residual, total, m, 0, 0, 0, 0, drop, EPS, types)
-    need = capi.layer_norm_workspace(2, 8)
+    rows = 100_000                                  # few rows need no workspace
+    need = capi.layer_norm_workspace(rows, 8)
     assert need >= 2 * 8 * 4
     for args, match in [
             ((2, 8, none, m, m, 0, 0, 0, 16, 16, 0, 0, drop, types), "null"), ((2, 8, m, m, m, 0, 0, 0, 0, 16, 0, 0, drop, types), "mean and rstd"),
-            ((2, 8, m, m, m, 0, 4096, 0, 16, 16, 0, 0, drop, types), "workspace"),
-            ((2, 8, m, m, m, 0, 4096, 0, 16, 16, 4096, need - 1, drop, types), "workspace"),
-            ((2, 8, m, m, m, 0, 4096, 0, 16, 16, 4100, need, drop, types), "workspace"),
+            ((rows, 8, m, m, m, 0, 4096, 0, 16, 16, 0, 0, drop, types), "workspace"),
+            ((rows, 8, m, m, m, 0, 4096, 0, 16, 16, 4096, need - 1, drop, types), "workspace"),
+            ((rows, 8, m, m, m, 0, 4096, 0, 16, 16, 4100, need, drop, types), "workspace"),
             ((2, 8, m, m, (4096, 2), 0, 0, 0, 16, 16, 0, 0, drop, types), "overlap"),
             ((2, 8, m, m, m, 4096, 0, 0, 16, 16, 0, 0, drop, (f32, f32, bf16)), "weight and bias")]:
         with pytest.raises(RuntimeError, match=match):
