@@ -88,8 +88,12 @@ def build_pymod(force=False, verbose=True):
 def build_nn(force=False, verbose=True):
     src = os.path.join(CSRC, "nn_module.cpp")
     if force or not _newer(NNMOD, [src, os.path.join(HERE, "..", "include", "hetuctr_hip.h")]):
-        import torch
-        from torch.utils import cpp_extension
+        try:
+            import torch
+            from torch.utils import cpp_extension
+        except ImportError:
+            print("torch is not installed: hetuctr_nn (hetuctr_amd.nn) is not built", flush=True)
+            return None
         inc = ["-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(HERE, "..", "include")]
         inc += [x for path in cpp_extension.include_paths() for x in ("-isystem", path)]
         lib = os.path.join(os.path.dirname(torch.__file__), "lib")

@@ -7,7 +7,8 @@ import struct
 import numpy as np
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
-# HETUCTR_LIB points at another build of the same library (kernel tuning experiments)
+# HETUCTR_LIB points at another build of the same library (kernel tuning experiments; the extension under hetuctr_amd.nn takes
+# the library beside it, or the one that LD_LIBRARY_PATH finds)
 LIB_PATH = os.environ.get("HETUCTR_LIB") or os.path.join(_HERE, "lib", "libhetuctr_hip.so")
 INIT = {"Zero": 0, "Normal": 1, "Uniform": 2, "TruncatedNormal": 3}
 SYMBOLS = ["hctr_create", "hctr_destroy", "hctr_preprocess", "hctr_preprocess_noalloc", "hctr_push_pull", "hctr_push_pull_pooled",
