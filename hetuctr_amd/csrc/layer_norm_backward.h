@@ -130,7 +130,10 @@ template <typename S, typename A, bool ADD, bool DROP, Rows R, int LANES, int IT
 __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
   constexpr int V = kVec<S>, BLOCK = block_of<LANES>, GROUP = LANES < kWave ? LANES : kWave, WAVES = LANES / GROUP, GROUPS = BLOCK / LANES;
   if (blockIdx.x >= a.row_blocks) return sum_columns<S, A, DROP && !ADD, BLOCK>(a, blockIdx.x - a.row_blocks);
-  constexpr bool TIGHT = LANES == 1024 && ITEMS * V == 16; // 128 registers: the row's own values and sums are all that fits
+  // The widest rows leave 128 registers: the row's own values and sums, the next row if it is two matrices of 16-bit values, and no weight,
+  // of which every lane puts its columns in LDS.  (1.2e8 bfloat16 values in rows of 11381: 219 us with neither, 182 this way.)
+  constexpr bool TIGHT = LANES == 1024 && ITEMS * V == 16, AHEAD = !TIGHT || (sizeof(S) == 2 && !ADD);
+  __shared__ float4 shelf[TIGHT ? ITEMS * V / 4 * BLOCK : 1];
   __shared__ float2 found[2][WAVES];
   __shared__ float joined[GROUPS > 1 ? GROUPS * LANES * ITEMS * V : 1];
   const uint32_t lane = threadIdx.x % GROUP, wave = WAVES > 1 ? threadIdx.x / kWave : 0;
@@ -140,8 +143,15 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
   const auto fetch_weight = [&] {
     load_affine<V, A, R>(w, a.weight, a.narrow, first, GROUP * V, a.width, 1.f);
     if constexpr (DROP && !ADD) scale_all(w, a.drop.scale); // what is kept is scaled with it
+    if constexpr (TIGHT) {
+#pragma unroll
+      for (int i = 0; i < ITEMS; i++)
+#pragma unroll
+        for (int q = 0; q < V / 4; q++)
+          shelf[(i * (V / 4) + q) * BLOCK + threadIdx.x] = make_float4(w[i].v[4 * q], w[i].v[4 * q + 1], w[i].v[4 * q + 2], w[i].v[4 * q + 3]);
+    }
   };
-  if constexpr (!TIGHT) fetch_weight();
+  fetch_weight();
 #pragma unroll
   for (int i = 0; i < ITEMS; i++) {
 #pragma unroll
@@ -157,21 +167,18 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
       const uint32_t c = first + i * GROUP * V;
       dy[i] = load_raw<V, R>((const A *)a.dy + (int64_t)r * a.dy_stride, c, a.width);
       s[i] = load_raw<V, R>((const S *)a.s + (int64_t)r * a.s_stride, c, a.width);
-      if constexpr (ADD && !TIGHT)
+      if constexpr (ADD && AHEAD)
         if (a.ds) ds[i] = load_raw<V, R>((const S *)a.ds + (int64_t)r * a.ds_stride, c, a.width);
     }
     mean = a.mean[r];
     rstd = a.rstd[r];
   };
   uint64_t r = (uint64_t)blockIdx.x * GROUPS + threadIdx.x / LANES;
-  if (!TIGHT && r < a.rows) fetch(r);
+  if (AHEAD && r < a.rows) fetch(r);
   int turn = 0;
   for (; r < a.rows; r += stride) {
-    if constexpr (TIGHT) {
-      asm volatile("" : "+v"(first)); // no address is worked out, and kept, before the loop
-      fetch(r);
-      fetch_weight();
-    }
+    if constexpr (TIGHT) asm volatile("" : "+v"(first)); // no address is worked out, and kept, before the loop
+    if constexpr (!AHEAD) fetch(r);
     Floats<V> g[ITEMS], h[ITEMS];
     typename Packed<S, V>::type more[ITEMS];
     float sums[2] = {0.f, 0.f}; // of g and of g * h
@@ -181,14 +188,21 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
       const uint32_t c = first + i * GROUP * V;
       g[i] = floats<V>(settled<V, R>(dy[i], c, a.width));
       h[i] = floats<V>(settled<V, R>(s[i], c, a.width));
-      if constexpr (ADD && !TIGHT) more[i] = ds[i];
+      if constexpr (ADD && AHEAD) more[i] = ds[i];
 #pragma unroll
       for (int j = 0; j < V; j++) h[i].v[j] = (h[i].v[j] - mean) * scale;
     }
-    if (!TIGHT && r + stride < a.rows) fetch(r + stride);
+    if (AHEAD && r + stride < a.rows) fetch(r + stride);
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
       if constexpr (DROP && !ADD) drop_columns<false>(g[i], a.drop, step, r * a.drop.quads + (first + i * GROUP * V) / 4);
+      if constexpr (TIGHT) {
+#pragma unroll
+        for (int q = 0; q < V / 4; q++) {
+          const float4 x4 = shelf[(i * (V / 4) + q) * BLOCK + threadIdx.x];
+          w[i].v[4 * q] = x4.x, w[i].v[4 * q + 1] = x4.y, w[i].v[4 * q + 2] = x4.z, w[i].v[4 * q + 3] = x4.w;
+        }
+      }
 #pragma unroll
       for (int j = 0; j < V; j++) { // columns behind the end have no gradient, and add nothing
         dweight[i].v[j] = fmaf(g[i].v[j], h[i].v[j], dweight[i].v[j]);
@@ -217,7 +231,7 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
       for (int j = 0; j < V; j++) d.v[j] = scale * (fmaf(-h[i].v[j], mean_gh, g[i].v[j]) - mean_g);
       if constexpr (ADD) {
         if (a.ds) {
-          if constexpr (TIGHT) more[i] = load_raw<V, R>((const S *)a.ds + (int64_t)r * a.ds_stride, c, a.width);
+          if constexpr (!AHEAD) more[i] = load_raw<V, R>((const S *)a.ds + (int64_t)r * a.ds_stride, c, a.width);
           const Floats<V> e = floats<V>(settled<V, R>(more[i], c, a.width));
 #pragma unroll
           for (int j = 0; j < V; j++) d.v[j] += e.v[j];
