@@ -88,7 +88,8 @@ template <int V, int ITEMS> __device__ __forceinline__ void scale_all(Floats<V> 
     for (int j = 0; j < V; j++) f[i].v[j] *= scale;
 }
 
-constexpr int kWideBlock = 256; // threads of a block that reads its row again and again
+// threads of a block that reads its row again and again; the gradient has few blocks, for the sake of their sums
+constexpr int kWideBlock = 256, kWideGradBlock = 1024;
 
 // threads of a block whose rows are held by LANES lanes each: 256, or those of one row if they are more than a wave
 template <int LANES> constexpr int block_of = LANES <= kWave ? 256 : LANES;
@@ -139,11 +140,10 @@ template <typename S, typename F> bool rows_in_registers(uint32_t width, F &&f) 
 
 // Blocks of the gradient's kernels, each of which writes a row of sums for weight and bias: as many per CU as fetch 17 KiB at a
 // time (bytes: of a column's values, read), so few that the memory sees long stretches and the rows of sums are little beside the data, at
-// least one and at most eight.  us on an MI355X for 2^27 values with 256, 512, 768, 1024 blocks (chosen: *): float, 64
-// columns 411, 287, 274*, 290; 1024 columns 268*, 286, 282, 286; bfloat16, 4096 columns 152, 151*, 160, 159; float and bfloat16,
-// dropped, 128 columns 665, 262, 230*, 244; the same with a branch added, 512 columns 354*, 386, 408, 423; 2048 columns 354*, 377,
-// 411, 431; 4096 rows of 8192 halves 51*, 63, 74, 86; 1.2e8 values in rows of 37
-// with 768, 1024, 1280, 1536: dropped 299, 287, 274*, 288, a branch added 420*, 466, 463, 475.
+// least one and at most eight.  us on an MI355X for 1.2e8 values with 256, 512, 768, 1024 blocks (chosen: *): float, 64 columns
+// 371, 253, 243*, 255; 1024 columns 240*, 258, 256, 259; bfloat16, 4096 columns 135, 127*, 141, 150; float and bfloat16, dropped, 128
+// columns 370, 234, 204*, 214; a branch added, 37 columns 741, 468, 403*, 469, 64 columns 431, 321*, 344, 367, 512 columns 324*, 358,
+// 364, 379, 2048 columns 324*, 335, 369, 384; 4096 rows of 8192 halves 46*, 54, 61, 69.
 inline unsigned norm_grad_blocks(uint64_t rows, uint32_t width, int V, int bytes) {
   const Held h = held_by(width, V);
   const uint64_t groups = h.lanes && h.lanes < 256 ? 256 / h.lanes : 1, fetch = groups * width * bytes;

@@ -5,7 +5,8 @@
 namespace hctr {
 namespace {
 
-// One block per row at a time, which it reads again for each of mean, variance and result: rows of any width.
+// One block per row at a time, which it reads again for each of mean, variance and result: rows of any width.  What it reads again
+// bounds it: 1.2e8 floats in rows of 20000 313 us (3.1 TB/s of what the operator has to move), bfloat16 162.
 template <typename S, typename A, bool ADD, bool DROP>
 __global__ __launch_bounds__(kWideBlock) void norm_wide(NormForward a) {
   constexpr int V = kVec<S>;
@@ -69,7 +70,9 @@ template <typename S, int LANES, int ITEMS> constexpr bool shelved = LANES == 10
 // lanes, a group of lanes has a row to itself, ROWS of them at a time, and a block as many as it has groups; beyond that the waves of a
 // block share a row, each a stretch of neighbouring columns, and join what they found: a wave's sum and its squares around
 // its own mean.  (Squares around a mean that is not the row's would cancel; put together as n * (wave's mean - mean)^2 they do
-// not, and the block waits once instead of twice.)
+// not, and the block waits once instead of twice.)  Bound by memory, and by arithmetic as much where values are drawn: 1.7 M rows
+// of 128, float to bfloat16, dropped, 214 us (1.3 GB, 6.2 TB/s; a plain copy reaches 6.5); 16384 rows of 4096, a branch dropped
+// and added, 131 us (6.1 TB/s).
 template <typename S, typename A, bool ADD, bool DROP, Rows R, int LANES, int ITEMS, int ROWS>
 __global__ __launch_bounds__(block_of<LANES>) void norm_rows(NormForward a) {
   constexpr int V = kVec<S>, BLOCK = block_of<LANES>, GROUP = LANES < kWave ? LANES : kWave, WAVES = LANES / GROUP, GROUPS = BLOCK / LANES;
@@ -239,17 +242,19 @@ template <typename S, typename A, bool ADD, bool DROP> void launch(const NormFor
   const bool held = rows_in_registers<S>(p.width, [&](auto rows, auto lanes, auto items) {
     constexpr Rows R = decltype(rows)::value;
     constexpr int LANES = decltype(lanes)::value, ITEMS = decltype(items)::value, BLOCK = block_of<LANES>;
-    // Four rows at a time where the memory would wait for the lanes: they draw, convert two values a register, or leave some of
-    // their loads empty.  us with one row and with four, 2^27 values: float to bfloat16, dropped, 16 columns 155, 131, 64
-    // columns 156, 132, 256 columns 160, 139; float, 37 columns 313, 226; bfloat16, 64 columns 96, 92.  Elsewhere four are no
-    // better or worse: float, 64 columns 175, 179, 256 columns 179, 194; a branch added, float and bfloat16, 256 columns 265, 283.
+    // Four rows at a time (two, if each is two pieces a lane) where the memory would wait for the lanes: they draw, convert two values
+    // a register, or leave some of their loads empty.  us with one row and with four, 1.2e8 values: float to bfloat16, dropped, 16
+    // columns 147, 126, 256 columns 152, 121, 37 columns 326, 209, 333 columns 224, 188; float, 37 columns 271, 191; bfloat16, 64
+    // columns 87, 81, 333 columns 166, 107; a branch added, bfloat16, dropped, 37 columns 319, 280.  Elsewhere four are no better or
+    // worse: float, 64 columns 157, 157, 256 columns 157, 165; a branch added, float and bfloat16, 256 columns 236, 245, bfloat16,
+    // dropped, 16 columns 154, 161.
     constexpr bool FOUR = LANES <= kWave && ITEMS == 1 && (R != Rows::kEven || (!ADD && (DROP || sizeof(S) == 2)));
     constexpr int ROWS = FOUR ? 4 : LANES <= kWave && ITEMS == 2 && R == Rows::kRagged && !stays<S, LANES, ITEMS> ? 2 : 1, PER = BLOCK / LANES * ROWS;
-    // Blocks that stay: as many per CU as fetch 16 KiB at a time, or sixteen where the draws' arithmetic wants them.  us for 2^27
-    // values with 256, 512, 1024, 4096 blocks and with one for each row (chosen: *): float, 4096 columns 176*, 179, 184, 182, 195;
-    // bfloat16, 2048 columns 197, 120, 92*, 98, 111, 8192 columns 90*, 91, 92, 93, 117; a branch added, float and bfloat16, 1024
-    // columns 269*, 292, 286, 278, 272, 4096 columns 269*, 285, 284, 278, 282; float to bfloat16, dropped, 4096 columns 176, 141,
-    // 145, 137*, 157.  Two pieces a lane of a wave: 297 with 512 blocks, 272 with one for each row*.
+    // Blocks that stay: as many per CU as fetch 16 KiB at a time, or sixteen where the draws' arithmetic wants them.  us for 1.2e8
+    // values with 256, 512, 1024, 4096 blocks and with one for each row (chosen: *): float, 4096 columns 161*, 162, 165, 163, 176;
+    // bfloat16, 2048 columns 166, 106, 82*, 87, 102, 8192 columns 81*, 82, 90, 85, 108; a branch added, float and bfloat16, 1024
+    // columns 244*, 262, 256, 250, 241, 4096 columns 241*, 257, 255, 250, 250; float to bfloat16, dropped, 4096 columns 150, 121,
+    // 127, 123*, 142.
     uint64_t most = (1u << 31) / BLOCK;
     if constexpr (stays<S, LANES, ITEMS>) {
       const uint64_t fetch = (uint64_t)PER * p.width * (ADD ? sizeof(A) + sizeof(S) : sizeof(S));
