@@ -551,6 +551,30 @@ def test_autograd_gives_the_gradients(stream, act):
 
 
 @gpu
+@pytest.mark.parametrize("wanted", [(0,), (1,), (2,), (3,), (0, 3), (1, 2)])
+def test_autograd_of_some_of_the_inputs(wanted):
+    x, r, dy = (values((700, 48), "f32", i) for i in range(3))
+    w, b = affine("f32", 48, "f32")
+    drop = nn.Drop(0.3, 4, 4)
+    y, s, mean, rstd = nn.dropout_add_layer_norm(x, r, w, b, drop=drop, stats=True)
+    want = nn.dropout_add_layer_norm_backward(dy, None, s, mean, rstd, w, b, drop=drop)
+    _, mean, rstd = nn.layer_norm(r, w, b, drop=drop, stats=True)
+    plain = (None,) + nn.layer_norm_backward(dy, r, mean, rstd, w, b, drop=drop)
+    inputs = [t.clone().requires_grad_(i in wanted) for i, t in enumerate((x, r, w, b))]
+    leaves = [inputs[i] for i in wanted]
+    out = nn.dropout_add_layer_norm(*inputs, drop=drop)[0]
+    for i, g in zip(wanted, torch.autograd.grad(out, leaves, dy)):
+        assert torch.equal(g, want[i])
+    if 0 not in wanted:
+        out, mean, rstd = nn.layer_norm(*inputs[1:], drop=drop, stats=True)
+        assert not mean.requires_grad and not rstd.requires_grad
+        for i, g in zip(wanted, torch.autograd.grad(out, leaves, dy)):
+            assert torch.equal(g, plain[i])
+    with torch.no_grad():
+        assert not nn.layer_norm(*inputs[1:]).requires_grad
+
+
+@gpu
 def test_a_step_that_changed_before_its_gradient_is_an_error():
     x = values((4, 16), "f32", 1).requires_grad_()
     step = torch.zeros(1, dtype=torch.int64, device="cuda")
