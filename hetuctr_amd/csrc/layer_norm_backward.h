@@ -145,6 +145,9 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
   const uint32_t lane = threadIdx.x % GROUP, wave = WAVES > 1 ? threadIdx.x / kWave : 0;
   uint32_t first = wave * GROUP * V * ITEMS + lane * V;
   const uint64_t step = DROP ? step_of(a.drop) : 0, stride = (uint64_t)a.row_blocks * GROUPS;
+  // whether the wave has columns in its piece i: if not, nothing is drawn or worked out for it
+  const uint32_t begin = WAVES > 1 ? __builtin_amdgcn_readfirstlane(wave * GROUP * V * ITEMS) : 0;
+  const auto used = [&](int i) { return (WAVES == 1 && i == 0) || begin + i * GROUP * V < a.width; };
   Floats<V> w[ITEMS], dweight[ITEMS], dbias[ITEMS];
   const auto fetch_weight = [&] {
     load_affine<V, A, R>(w, a.weight, a.narrow, first, GROUP * V, a.width, 1.f);
@@ -201,6 +204,7 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
     if (AHEAD && r + stride < a.rows) fetch(r + stride);
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
+      if (!used(i)) continue;
       if constexpr (DROP && !ADD) drop_columns<false>(g[i], a.drop, step, r * a.drop.quads + (first + i * GROUP * V) / 4);
       if constexpr (TIGHT) {
 #pragma unroll
@@ -231,6 +235,7 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
       if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
+      if (!used(i)) continue;
       const uint32_t c = first + i * GROUP * V;
       Floats<V> d;
 #pragma unroll

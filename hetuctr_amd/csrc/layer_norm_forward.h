@@ -117,6 +117,9 @@ __global__ __launch_bounds__(block_of<LANES>) void norm_rows(NormForward a) {
     px += (int64_t)stride * a.x_stride;
     if constexpr (ADD) pr += (int64_t)stride * a.residual_stride;
   };
+  // whether the wave has columns in its piece i: if not, nothing is drawn or worked out for it
+  const uint32_t begin = WAVES > 1 ? __builtin_amdgcn_readfirstlane(wave * STRETCH) : 0;
+  const auto used = [&](int i) { return (WAVES == 1 && i == 0) || begin + i * GROUP * V < a.width; };
   const auto fetch_affine = [&] {
     load_affine<V, A, R>(w, a.weight, a.narrow, first, GROUP * V, a.width, 1.f);
     load_affine<V, A, R>(b, a.bias, a.narrow, first, GROUP * V, a.width, 0.f);
@@ -154,7 +157,8 @@ __global__ __launch_bounds__(block_of<LANES>) void norm_rows(NormForward a) {
         f[k][i] = floats<V>(settled<V, R>(x[k][i], c, a.width));
         if constexpr (ADD) {
           const Floats<V> g = floats<V>(settled<V, R>(residual[k][i], c, a.width));
-          if constexpr (DROP) drop_columns(f[k][i], a.drop, step, quad + k * GROUPS * a.drop.quads + c / 4);
+          if constexpr (DROP)
+            if (used(i)) drop_columns(f[k][i], a.drop, step, quad + k * GROUPS * a.drop.quads + c / 4);
 #pragma unroll
           for (int j = 0; j < V; j++) f[k][i].v[j] += g.v[j];
           store_columns<V, R>(ps + k * GROUPS * a.sum_stride, c, width(k, r0), f[k][i]);
@@ -216,6 +220,7 @@ __global__ __launch_bounds__(block_of<LANES>) void norm_rows(NormForward a) {
           b[i].v[4 * q] = y4.x, b[i].v[4 * q + 1] = y4.y, b[i].v[4 * q + 2] = y4.z, b[i].v[4 * q + 3] = y4.w;
         }
       }
+      if (!used(i)) continue;
 #pragma unroll
       for (int k = 0; k < ROWS; k++) {
 #pragma unroll
