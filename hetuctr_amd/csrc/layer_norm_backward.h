@@ -196,10 +196,12 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
     for (int i = 0; i < ITEMS; i++) {
       const uint32_t c = first + i * GROUP * V;
       g[i] = floats<V>(settled<V, R>(dy[i], c, a.width));
-      h[i] = floats<V>(settled<V, R>(s[i], c, a.width));
+      // Columns behind the end have no gradient; for the product of the two to be nothing h has to be finite there, as -mean * scale is not
+      // where rows lie far enough from zero.  Ragged rows hold columns of their own there where a vector was moved; else h is 0.
+      h[i] = floats<V>(settled<V, R, R == Rows::kRagged>(s[i], c, a.width));
       if constexpr (ADD && AHEAD) more[i] = ds[i];
 #pragma unroll
-      for (int j = 0; j < V; j++) h[i].v[j] = (h[i].v[j] - mean) * scale;
+      for (int j = 0; j < V; j++) h[i].v[j] = (h[i].v[j] - ((R == Rows::kTiny ? c + j : c) < a.width ? mean : 0.f)) * scale;
     }
     if (AHEAD && r + stride < a.rows) fetch(r + stride);
 #pragma unroll

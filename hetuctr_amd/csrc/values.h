@@ -41,7 +41,7 @@ template <Rows R, typename T> __device__ __forceinline__ T *at_column(T *row, ui
 // more is the row's last V columns (load_raw), moved down by as many as it would end behind (settled; the same number for
 // every row, so the branches are scalar ones).  Rows of 37 floats, a gradient of 2^27 values: 732 us with the move in the
 // branch of the load, where it waits for each load by itself, 348 in two steps.
-// ONCE: nothing reads them again soon.
+// ONCE: nothing reads them again soon.  KEPT: behind the end of a vector that was moved lie other columns of the row, not zeros.
 template <int V, Rows R, bool ONCE = R == Rows::kEven, typename T>
 __device__ __forceinline__ typename Packed<T, V>::type load_raw(const T *row, uint32_t c, uint32_t width) {
   typename Packed<T, V>::type x = (T)0;
@@ -60,7 +60,7 @@ __device__ __forceinline__ typename Packed<T, V>::type load_raw(const T *row, ui
   }
   return x;
 }
-template <int V, Rows R, typename X> __device__ __forceinline__ X settled(X x, uint32_t c, uint32_t width) {
+template <int V, Rows R, bool KEPT = false, typename X> __device__ __forceinline__ X settled(X x, uint32_t c, uint32_t width) {
   if constexpr (R != Rows::kEven)
     if (c < width && c + V > width && (R == Rows::kRagged || width >= V)) {
       const uint32_t by = V - width % V;
@@ -68,7 +68,7 @@ template <int V, Rows R, typename X> __device__ __forceinline__ X settled(X x, u
       for (int k = 1; k < V; k *= 2)
         if (by & k) {
 #pragma unroll
-          for (int j = 0; j < V; j++) x[j] = j + k < V ? x[(j + k) % V] : 0;
+          for (int j = 0; j < V; j++) x[j] = j + k < V ? x[(j + k) % V] : KEPT ? x[j] : 0;
         }
     }
   return x;
