@@ -5,6 +5,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/torch.h>
 
+#include <forward_list>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -29,9 +30,14 @@ struct Arguments {
   void expect(Py_ssize_t n) const {
     if (count != n) refuse("wrong number of arguments");
   }
+  mutable std::forward_list<Tensor> made; // in place of what was given, until the call is made
+  const Tensor &as_read(const Tensor &t) const {
+    if (!t.is_neg()) return t;
+    return made.emplace_front(t.resolve_neg()); // a view of memory that holds the values with the other sign
+  }
   const Tensor &tensor(int i, const char *what) const {
     if (!THPVariable_Check(given[i])) refuse(std::string(what) + " must be a tensor");
-    return THPVariable_Unpack(given[i]);
+    return as_read(THPVariable_Unpack(given[i]));
   }
   Maybe maybe(int i, const char *what) const {
     if (given[i] == Py_None) return std::nullopt;
@@ -63,8 +69,9 @@ int type_of(at::ScalarType t, const char *what) {
   refuse(std::string(what) + " must be float32, bfloat16 or float16, not " + c10::toString(t));
 }
 
-// a Drop (p, seed, step, step_tensor), or None
-hctr_drop drop_of(PyObject *o, const Tensor &like) {
+// argument i: a Drop (p, seed, step, step_tensor), or None
+hctr_drop drop_of(const Arguments &a, int i, const Tensor &like) {
+  PyObject *o = a.given[i];
   hctr_drop d = {0.0, 0, 0, nullptr};
   if (o == Py_None) return d;
   if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) refuse("drop must be a Drop");
@@ -75,7 +82,7 @@ hctr_drop drop_of(PyObject *o, const Tensor &like) {
   PyObject *extra = PyTuple_GET_ITEM(o, 3);
   if (extra != Py_None) {
     if (!THPVariable_Check(extra)) refuse("the step tensor must be one int64 on the device of the values");
-    const Tensor &t = THPVariable_Unpack(extra);
+    const Tensor &t = a.as_read(THPVariable_Unpack(extra));
     if (t.device() != like.device() || t.scalar_type() != at::kLong || t.numel() != 1)
       refuse("the step tensor must be one int64 on the device of the values");
     d.step_dev = (const uint64_t *)t.data_ptr();
@@ -163,7 +170,7 @@ PyObject *dropout(const Arguments &a) {
   hctr_dropout_args r = {};
   r.rows = m.rows, r.width = m.width;
   r.dtype = type_of(x.scalar_type(), "x");
-  r.drop = drop_of(a.given[1], x);
+  r.drop = drop_of(a, 1, x);
   const Tensor y = result(x.sizes(), x, x.scalar_type());
   r.x = m.at, r.y = whole(y, m.width);
   r.stream = a.stream(2);
@@ -195,7 +202,7 @@ PyObject *forward(const Arguments &a) {
   const Affine affine = affine_of(a.maybe(2, "weight"), a.maybe(3, "bias"), m.width, act, x);
   r.weight = pointer(affine.weight), r.bias = pointer(affine.bias), r.affine_dtype = affine.type;
   r.eps = (float)a.number(4);
-  r.drop = drop_of(a.given[5], x);
+  r.drop = drop_of(a, 5, x);
   const Tensor y = result(x.sizes(), x, act);
   r.y = whole(y, m.width);
   if (residual) {
@@ -237,7 +244,7 @@ PyObject *backward(const Arguments &a) {
   r.weight = pointer(affine.weight), r.affine_dtype = affine.type;
   const Tensor mean = statistic(a.tensor(4, "mean"), m.rows, s, "mean"), rstd = statistic(a.tensor(5, "rstd"), m.rows, s, "rstd");
   r.mean = (const float *)mean.data_ptr(), r.rstd = (const float *)rstd.data_ptr();
-  r.drop = drop_of(a.given[8], s);
+  r.drop = drop_of(a, 8, s);
   Maybe dx, dresidual, dweight, dbias, space;
   bool one = false; // dx and dresidual are one tensor
   if (add) {
