@@ -1,6 +1,7 @@
 // Python module `hetuctr_nn`: the dense operators of the C ABI on torch tensors, for hetuctr_amd/nn.py.  Host-only C++: argument
 // checks, results from torch's allocator, one hctr_* call.  It is here because a call of few rows is the host's time: the same
 // steps in Python took 5 us of a layer_norm call, of which the launch is 2.9.
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/torch.h>
@@ -32,6 +33,8 @@ struct Arguments {
   }
   mutable std::forward_list<Tensor> made; // in place of what was given, until the call is made
   const Tensor &as_read(const Tensor &t) const {
+    if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+      refuse("there are no forward-mode derivatives, and a tensor has a tangent");
     if (!t.is_neg()) return t;
     return made.emplace_front(t.resolve_neg()); // a view of memory that holds the values with the other sign
   }

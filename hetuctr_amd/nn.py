@@ -11,8 +11,8 @@ that lives outside (tests/check.py:44), and takes the gradient of those rows bac
 A tensor's last dimension is a row; the others, if any, count rows.  Rows of float32, bfloat16 or float16 may lie any number of
 elements apart; where the tensor's memory order does not allow that, a call copies it first.  Results are new contiguous
 tensors.  Work goes to torch's current stream, nothing waits, and a call may be captured into a graph.  The functions without
-`_backward` in their name can be differentiated (once); the others are the gradients themselves, for programs that keep
-their own books.
+`_backward` in their name can be differentiated (once, in reverse: a tensor with a tangent is refused); the others are the gradients
+themselves, for programs that keep their own books.
 """
 import importlib
 import sys

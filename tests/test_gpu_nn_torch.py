@@ -1,6 +1,7 @@
 """hetuctr_amd.nn beside what torch does around its own operators."""
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from hetuctr_amd import nn
 
@@ -40,3 +41,29 @@ def test_views_that_carry_a_sign(width):
     want = nn.dropout_add_layer_norm_backward(dy, ds, s, mean, rstd, w, b, drop=drop)
     for a, g in zip(nn.dropout_add_layer_norm_backward(negative(dy), negative(ds), negative(s), mean, rstd, w, b, drop=drop), want):
         assert torch.equal(a, g)
+
+
+# ---- forward-mode derivatives -----------------------------------------------------------------------------------------------
+def calls(x, r, w, b, stat):
+    drop = nn.Drop(0.3, 4, 4)
+    yield "dropout", (x,), lambda x: nn.dropout(x, drop)
+    yield "layer_norm", (x, w, b), lambda x, w, b: nn.layer_norm(x, w, b)
+    yield "dropout_add_layer_norm", (x, r, w, b), lambda x, r, w, b: nn.dropout_add_layer_norm(x, r, w, b, drop=drop)
+    yield "layer_norm_backward", (r, x, stat, stat, w), lambda dy, x, mean, rstd, w: nn.layer_norm_backward(dy, x, mean, rstd, w)
+    yield ("dropout_add_layer_norm_backward", (r, r, x, stat, stat, w),
+           lambda dy, ds, s, mean, rstd, w: nn.dropout_add_layer_norm_backward(dy, ds, s, mean, rstd, w))
+
+
+@gpu
+def test_forward_mode_derivatives_are_refused_not_lost():
+    x, r, w, b, stat = values((4, 8), 1), values((4, 8), 2), values(8, 3), values(8, 4), values(4, 5).abs()
+    for name, args, f in calls(x, r, w, b, stat):
+        for i in range(len(args)):
+            for needs in (False, True):
+                with forward_ad.dual_level():
+                    given = [a.clone().requires_grad_(needs) for a in args]
+                    given[i] = forward_ad.make_dual(given[i], torch.ones_like(args[i]))
+                    with pytest.raises(RuntimeError, match="forward-mode|jvp"):
+                        f(*given)
+        with forward_ad.dual_level(), torch.no_grad(), forward_ad._set_fwd_grad_enabled(False):
+            f(forward_ad.make_dual(args[0], torch.ones_like(args[0])), *args[1:])      # nothing to lose
