@@ -1,7 +1,9 @@
 // Python module `hetuctr_nn`: the dense operators of the C ABI on torch tensors, for hetuctr_amd/nn.py.  Host-only C++: argument
 // checks, results from torch's allocator, one hctr_* call.  It is here because a call of few rows is the host's time: the same
 // steps in Python took 5 us of a layer_norm call, of which the launch is 2.9.
+#include <ATen/TracerMode.h>
 #include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/torch.h>
@@ -275,6 +277,18 @@ PyObject *backward(const Arguments &a) {
   return tuple(dx, dweight, dbias);
 }
 
+// The GPU on which tensor x lies; -1: on none, or something sees, and may record or change, what goes through torch's dispatcher (a
+// dispatch mode, a tracer)
+PyObject *unseen_on(PyObject *, PyObject *x) {
+  if (!THPVariable_Check(x)) {
+    PyErr_SetString(PyExc_TypeError, "hetuctr_amd.nn: a tensor is needed");
+    return nullptr;
+  }
+  const bool seen = c10::impl::dispatch_mode_enabled() || at::tracer::impl::is_dispatch_enabled();
+  const Tensor &t = THPVariable_Unpack(x);
+  return PyLong_FromLong(!seen && t.is_cuda() ? t.get_device() : -1);
+}
+
 // An error that Python has set already travels as an empty domain_error.
 template <PyObject *(*F)(const Arguments &)> PyObject *call(PyObject *, PyObject *const *args, Py_ssize_t count) {
   try {
@@ -292,6 +306,7 @@ template <PyObject *(*F)(const Arguments &)> PyCFunction method() { return (PyCF
 PyMethodDef methods[] = {{"dropout", method<dropout>(), METH_FASTCALL, nullptr},
                          {"forward", method<forward>(), METH_FASTCALL, nullptr},
                          {"backward", method<backward>(), METH_FASTCALL, nullptr},
+                         {"unseen_on", unseen_on, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "hetuctr_nn", "The dense operators on torch tensors; use hetuctr_amd.nn.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

@@ -14,11 +14,13 @@ tensors.  Work goes to torch's current stream, nothing waits, and a call may be 
 `_backward` in their name can be differentiated (once, in reverse: a tensor with a tangent is refused); the others are the gradients
 themselves, for programs that keep their own books.
 """
+import functools
 import importlib
 import sys
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import LIBDIR
@@ -50,10 +52,10 @@ class Drop(NamedTuple):
 
 
 def _run(f, x, *args):
-    """f(*args, torch's current stream), on the device of x"""
-    index = x.get_device()
+    """f(*args, torch's current stream), on the device of x; as one of torch's operators while something watches them"""
+    index = _native.unseen_on(x)
     if index < 0:
-        raise RuntimeError("hetuctr_amd.nn: the tensors must be on the GPU")
+        return _as_operator(f, x, args)
     if index == torch.cuda.current_device():
         return f(*args, _stream_of(index))
     with torch.cuda.device(index):
@@ -64,7 +66,7 @@ def _wants_gradient(*tensors):
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
-                return True
+                return not torch._C._is_tracing()       # a traced operator asks again
     return False
 
 
@@ -169,3 +171,106 @@ def dropout_add_layer_norm_backward(dy, ds, s, mean, rstd, weight=None, bias=Non
     s and the rows' statistics that it returned.  dx has the type of dy, dresidual that of s; without dropout and where these
     are one type, they are one tensor."""
     return _run(_native.backward, s, True, dy, ds, s, mean, rstd, weight, bias, drop, True, True, True)
+
+
+# ---- the same as torch operators ----------------------------------------------------------------------------------------
+# torch.jit.trace, make_fx, fake tensors and dispatch modes see what goes through torch's dispatcher: of a call into the extension only
+# that memory was allocated, which a recorded program would then return unfilled.  While one of them is at work, a call
+# goes to the extension through an operator of torch's (hetuctr_amd::..), which is what they see.  Otherwise it does not: the dispatcher
+# and the operator's arguments cost several times what the extension's call does.
+#
+# The operators take a Drop as four arguments, and return the tensors that there are: what would be None is left out, and what
+# would be one tensor twice is there once.
+_DROP = "float p, int seed, int step, Tensor? step_tensor"
+_SCHEMAS = {
+    "dropout": "(Tensor x, %s) -> Tensor[]",
+    "norm": "(Tensor x, Tensor? residual, Tensor? weight, Tensor? bias, float eps, %s, ScalarType? dtype, bool stats) -> Tensor[]",
+    "norm_backward": "(bool add, Tensor dy, Tensor? ds, Tensor s, Tensor mean, Tensor rstd, Tensor? weight, Tensor? bias, %s, "
+                     "bool need_x, bool need_weight, bool need_bias) -> Tensor[]",
+}
+_EXTENSION = {"dropout": _native.dropout, "norm": _native.forward, "norm_backward": _native.backward}
+_DROP_AT = {"dropout": 1, "norm": 5, "norm_backward": 8}
+_NAME_OF = {f: name for name, f in _EXTENSION.items()}
+_library = torch.library.Library("hetuctr_amd", "DEF")
+
+
+def _as_operator(f, x, args):
+    if x.device.type != "cuda":
+        raise RuntimeError("hetuctr_amd.nn: the tensors must be on the GPU")
+    name = _NAME_OF[f]
+    at = _DROP_AT[name]
+    p, seed, step, step_tensor = args[at] or (0.0, 0, 0, None)
+    signed = lambda v: (v + 2 ** 63) % 2 ** 64 - 2 ** 63       # the same modulo 2^64
+    out = iter(getattr(torch.ops.hetuctr_amd, name)(*args[:at], p, signed(seed), signed(step), step_tensor, *args[at + 1:]))
+    if f is _native.dropout:
+        return next(out)
+    if f is _native.forward:
+        there = [True] * (1 if args[1] is None else 2) + [args[7]] * 2
+    else:
+        there = [True, args[6] is not None and args[10], args[7] is not None and args[11]]
+        if args[0]:                                             # dx may be dresidual
+            one = _one_gradient(args[1], args[3], p)
+            there.insert(0, args[9] and not one)
+    out = tuple(next(out) if t else None for t in there)
+    if f is _native.backward and args[0] and args[9] and one:
+        out = (out[1],) + out[1:]
+    return out
+
+
+def _one_gradient(dy, s, p):
+    return dy.dtype == s.dtype and p == 0
+
+
+def _with_drop(name, args):
+    at = _DROP_AT[name]
+    return args[:at] + (Drop(*args[at:at + 4]),) + args[at + 4:]
+
+
+def _compute(name, *args):
+    args = _with_drop(name, args)
+    with torch.cuda.device(args[1 if name == "norm_backward" else 0].device):
+        out = _EXTENSION[name](*args, torch.cuda.current_stream().cuda_stream)
+    if name == "dropout":
+        return [out]
+    return [t for i, t in enumerate(out) if t is not None and not (i and t is out[i - 1])]
+
+
+def _shapes(name, *args):
+    args = _with_drop(name, args)
+    per_row = lambda t: t.new_empty(t.numel() // t.shape[-1], dtype=torch.float32)
+    if name == "dropout":
+        return [args[0].new_empty(args[0].shape)]
+    if name == "norm":
+        x, residual, _, _, _, _, dtype, stats = args
+        out = [x.new_empty(x.shape, dtype=dtype)] + ([] if residual is None else [residual.new_empty(x.shape)])
+        return out + ([per_row(x), per_row(x)] if stats else [])
+    add, dy, _, s, _, _, weight, bias, drop, need_x, need_weight, need_bias = args
+    out = [s.new_empty(s.shape)]
+    if add and need_x and not _one_gradient(dy, s, drop.p):
+        out.insert(0, dy.new_empty(s.shape))
+    return out + [t.new_empty(t.shape) for t, need in ((weight, need_weight), (bias, need_bias)) if t is not None and need]
+
+
+def _differentiable(name, *args):
+    """A recorded program may be run with tensors that want gradients."""
+    tensors = [t for t in args if isinstance(t, torch.Tensor)]
+    if not _wants_gradient(*tensors) and not any(forward_ad.unpack_dual(t, level=0).tangent is not None for t in tensors):
+        with torch._C._AutoDispatchBelowAutograd():
+            return getattr(torch.ops.hetuctr_amd, name)(*args)
+    args = _with_drop(name, args)
+    if name == "dropout":
+        return [_Dropout.apply(*args, args[1].step_tensor)]
+    x, residual, weight, bias, eps, drop, dtype, stats = args
+    if residual is None:
+        out = _LayerNorm.apply(x, weight, bias, eps, drop, dtype, drop.step_tensor)
+    else:
+        out = _DropoutAddLayerNorm.apply(x, residual, weight, bias, eps, drop, drop.step_tensor)
+    return list(out if stats else out[:-2])
+
+
+for _name, _schema in _SCHEMAS.items():
+    _library.define(_name + _schema % _DROP)
+    _library.impl(_name, functools.partial(_compute, _name), "CUDA")
+    torch.library.register_fake("hetuctr_amd::" + _name, functools.partial(_shapes, _name), lib=_library)
+    if _name != "norm_backward":
+        _library.impl(_name, functools.partial(_differentiable, _name), "Autograd")

@@ -2,6 +2,8 @@
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from hetuctr_amd import nn
 
@@ -67,3 +69,117 @@ def test_forward_mode_derivatives_are_refused_not_lost():
                         f(*given)
         with forward_ad.dual_level(), torch.no_grad(), forward_ad._set_fwd_grad_enabled(False):
             f(forward_ad.make_dual(args[0], torch.ones_like(args[0])), *args[1:])      # nothing to lose
+
+
+# ---- programs that are recorded ---------------------------------------------------------------------------------------------
+def program(x, r, dy, w, b, step):
+    drop = nn.Drop(0.3, -4, 2 ** 63 + 1)
+    h, mean, rstd = nn.layer_norm(x, w, b, drop=drop, stats=True, dtype=torch.bfloat16)
+    grads = nn.layer_norm_backward(dy.bfloat16(), x, mean, rstd, w, b, drop=drop)
+    y, s, mean, rstd = nn.dropout_add_layer_norm(h, r, w, None, drop=drop, stats=True)
+    back = nn.dropout_add_layer_norm_backward(dy.bfloat16(), r, s, mean, rstd, w, drop=drop)
+    t, u = nn.dropout_add_layer_norm(r, x)
+    same = nn.dropout_add_layer_norm_backward(dy, None, u, mean, rstd)
+    assert same[0] is same[1] and back[3] is None
+    return (h, *grads, y, s, *back[:3], t, u, same[0], nn.dropout(nn.layer_norm(x), nn.Drop(0.2, 1, 3, step)), nn.dropout(x, None))
+
+
+def inputs(seed, rows=5):
+    return [values(s, seed + i) for i, s in enumerate(((rows, 16), (rows, 16), (rows, 16), 16, 16))] + [torch.tensor([seed], device="cuda")]
+
+
+def differ(got, want):
+    return [i for i, (a, b) in enumerate(zip(got, want)) if a.dtype != b.dtype or not torch.equal(a, b)]
+
+
+@gpu
+@pytest.mark.parametrize("mode", ["real", "fake", "symbolic"])
+def test_programs_recorded_as_graphs_compute_what_they_say(mode):
+    graph = make_fx(program, tracing_mode=mode)(*inputs(1))
+    for seed in (1, 50):
+        assert differ(graph(*inputs(seed)), program(*inputs(seed))) == []
+    if mode == "symbolic":
+        assert differ(graph(*inputs(7, rows=9)), program(*inputs(7, rows=9))) == []
+
+
+@gpu
+@pytest.mark.parametrize("mode", ["real", "fake"])
+def test_training_steps_recorded_as_graphs(mode):
+    def step(x, r, dy, w, b, more):
+        drop = nn.Drop(0.3, 4, 5, more)
+        leaves = [t.detach().requires_grad_() for t in (x, r, w, b)]
+        x, r, w, b = leaves
+        y, s = nn.dropout_add_layer_norm(nn.dropout(x, drop), r, w, b, drop=drop)
+        return torch.autograd.grad((nn.layer_norm(y, w, b, drop=drop), s), leaves, (dy, dy))
+
+    graph = make_fx(step, tracing_mode=mode)(*inputs(1))
+    for seed in (1, 50):
+        assert differ(graph(*inputs(seed)), step(*inputs(seed))) == []
+
+
+@gpu
+@pytest.mark.parametrize("needs", [False, True])
+def test_traced_programs_compute_what_they_say(needs):
+    graph = torch.jit.trace(program, inputs(1) if not needs else [t.requires_grad_(t.is_floating_point()) for t in inputs(1)])
+    for seed in (1, 50):
+        assert differ(graph(*inputs(seed)), program(*inputs(seed))) == []
+    # run with inputs that want gradients
+    f = lambda x, w: nn.layer_norm(nn.dropout(x, nn.Drop(0.2, 1)), w)
+    x, _, dy, w = inputs(3)[:4]
+    if needs:
+        x, w = x.requires_grad_(), w.requires_grad_()
+    graph = torch.jit.trace(f, (x, w))
+    x, w = (t.detach().clone().requires_grad_() for t in (x, w))
+    assert differ(torch.autograd.grad(graph(x, w), (x, w), dy), torch.autograd.grad(f(x, w), (x, w), dy)) == []
+
+
+class Watcher(TorchDispatchMode):
+    def __init__(self):
+        super().__init__()
+        self.seen = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.seen.append(str(func))
+        return func(*args, **(kwargs or {}))
+
+
+@gpu
+def test_dispatch_modes_see_the_calls():
+    want = program(*inputs(1))
+    given = inputs(1)
+    with Watcher() as outer, Watcher() as inner:
+        got = program(*given)
+    assert differ(got, want) == []
+    for watcher in (outer, inner):
+        own = [name for name in watcher.seen if name.startswith("hetuctr_amd.")]
+        assert len(own) == 9 and not any(name.startswith("aten.empty") for name in watcher.seen)
+    # a checkpointed layer is worked out again in its gradient's pass
+    x, _, dy, w, b = (t.requires_grad_() for t in inputs(5)[:5])
+    f = lambda x, w, b: nn.layer_norm(nn.dropout(x, nn.Drop(0.2, 1)), w, b)
+    want = torch.autograd.grad(f(x, w, b), (x, w, b), dy)
+    context = lambda: torch.utils.checkpoint.create_selective_checkpoint_contexts([torch.ops.aten.mm.default])
+    out = torch.utils.checkpoint.checkpoint(f, x, w, b, use_reentrant=False, context_fn=context)
+    assert differ(torch.autograd.grad(out, (x, w, b), dy), want) == []
+
+
+def test_shapes_without_memory():
+    # no GPU is needed: nothing is computed
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x = torch.empty((3, 5, 16), device="cuda")
+        h = torch.empty((3, 5, 16), device="cuda", dtype=torch.bfloat16)
+        w = torch.empty(16, device="cuda")
+        drop = nn.Drop(0.1, 2 ** 64 - 1, -1)
+        assert nn.dropout(h, drop).shape == (3, 5, 16)
+        y, mean, rstd = nn.layer_norm(x, w, None, drop=drop, dtype=torch.bfloat16, stats=True)
+        assert y.shape == x.shape and y.dtype == torch.bfloat16 and mean.shape == rstd.shape == (15,) and mean.dtype == torch.float32
+        dx, dweight, dbias = nn.layer_norm_backward(h, x, mean, rstd, w)
+        assert dx.shape == x.shape and dx.dtype == x.dtype and dweight.shape == (16,) and dbias is None
+        y, s, mean, rstd = nn.dropout_add_layer_norm(h, x, w, w, drop=drop, stats=True)
+        assert y.dtype == h.dtype and s.dtype == x.dtype and s.shape == x.shape and rstd.shape == (15,)
+        dx, dresidual, dweight, dbias = nn.dropout_add_layer_norm_backward(h, x, s, mean, rstd, w, w, drop=drop)
+        assert dx.dtype == h.dtype and dresidual.dtype == x.dtype and dweight.shape == dbias.shape == (16,)
+        dx, dresidual, dweight, dbias = nn.dropout_add_layer_norm_backward(x, None, s, mean, rstd)
+        assert dx is dresidual and dweight is None and dbias is None
+        with pytest.raises(RuntimeError, match="on the GPU"):
+            nn.dropout(torch.empty((2, 4)), drop)
