@@ -91,6 +91,7 @@ hctr_drop drop_of(const Arguments &a, int i, const Tensor &like) {
     if (t.device() != like.device() || t.scalar_type() != at::kLong || t.numel() != 1)
       refuse("the step tensor must be one int64 on the device of the values");
     d.step_dev = (const uint64_t *)t.data_ptr();
+    if (!d.step_dev) refuse("the step tensor has no memory");
   }
   return d;
 }
@@ -145,7 +146,13 @@ Affine affine_of(Maybe weight, Maybe bias, size_t width, at::ScalarType act, con
   a.bias = std::move(bias);
   return a;
 }
-void *pointer(const Maybe &t) { return t ? t->data_ptr() : nullptr; }
+// null: there is no such tensor.  One whose memory is missing must not be taken for that.
+void *pointer(const Maybe &t, const char *what) {
+  if (!t) return nullptr;
+  void *p = t->data_ptr();
+  if (!p && t->numel()) refuse(std::string(what) + " has no memory");
+  return p;
+}
 
 Tensor result(at::IntArrayRef sizes, const Tensor &like, at::ScalarType dtype) { return at::empty(sizes, like.options().dtype(dtype)); }
 hctr_matrix whole(const Tensor &t, size_t width) { return {t.data_ptr(), (int64_t)width}; }
@@ -205,7 +212,7 @@ PyObject *forward(const Arguments &a) {
   r.stream_dtype = residual ? type_of(residual->scalar_type(), "residual") : type_of(x.scalar_type(), "x");
   r.act_dtype = type_of(act, residual ? "x" : "the result");
   const Affine affine = affine_of(a.maybe(2, "weight"), a.maybe(3, "bias"), m.width, act, x);
-  r.weight = pointer(affine.weight), r.bias = pointer(affine.bias), r.affine_dtype = affine.type;
+  r.weight = pointer(affine.weight, "weight"), r.bias = pointer(affine.bias, "bias"), r.affine_dtype = affine.type;
   r.eps = (float)a.number(4);
   r.drop = drop_of(a, 5, x);
   const Tensor y = result(x.sizes(), x, act);
@@ -242,11 +249,12 @@ PyObject *backward(const Arguments &a) {
     same(*ds, s, s.scalar_type(), "ds");
     more = matrix_of(*ds, "ds");
     r.dsum = more.at;
+    pointer(more.kept, "ds");
   }
   r.stream_dtype = type_of(s.scalar_type(), normed);
   r.act_dtype = type_of(dy.scalar_type(), "dy");
   const Affine affine = affine_of(a.maybe(6, "weight"), a.maybe(7, "bias"), m.width, dy.scalar_type(), s);
-  r.weight = pointer(affine.weight), r.affine_dtype = affine.type;
+  r.weight = pointer(affine.weight, "weight"), r.affine_dtype = affine.type;
   const Tensor mean = statistic(a.tensor(4, "mean"), m.rows, s, "mean"), rstd = statistic(a.tensor(5, "rstd"), m.rows, s, "rstd");
   r.mean = (const float *)mean.data_ptr(), r.rstd = (const float *)rstd.data_ptr();
   r.drop = drop_of(a, 8, s);
@@ -263,7 +271,7 @@ PyObject *backward(const Arguments &a) {
   if (dx) r.dx = whole(*dx, m.width);
   if (affine.weight && a.flag(10)) dweight = result(affine.weight->sizes(), s, affine.weight->scalar_type());
   if (affine.bias && a.flag(11)) dbias = result(affine.bias->sizes(), s, affine.bias->scalar_type());
-  r.dweight = pointer(dweight), r.dbias = pointer(dbias);
+  r.dweight = pointer(dweight, "dweight"), r.dbias = pointer(dbias, "dbias");
   if (dweight || dbias) {
     r.workspace_bytes = hctr_layer_norm_workspace(m.rows, m.width);
     if (r.workspace_bytes) {

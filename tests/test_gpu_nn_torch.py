@@ -183,3 +183,36 @@ def test_shapes_without_memory():
         assert dx is dresidual and dweight is None and dbias is None
         with pytest.raises(RuntimeError, match="on the GPU"):
             nn.dropout(torch.empty((2, 4)), drop)
+
+
+# ---- tensors without memory -------------------------------------------------------------------------------------------------
+class Wrapper(torch.Tensor):
+    """A tensor whose values are elsewhere"""
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(cls, t.size(), strides=t.stride(), dtype=t.dtype, device=t.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError("%s of a Wrapper" % func)
+
+
+@gpu
+def test_tensors_without_memory_are_not_taken_for_missing_ones():
+    x, w, stat = values((4, 8), 1), values(8, 2), values(4, 3)
+    step = torch.zeros(1, dtype=torch.int64, device="cuda")
+    freed, hidden, nothing = w.clone(), Wrapper(w), torch._efficientzerotensor(8, device="cuda")
+    freed.untyped_storage().resize_(0)
+    for f in (lambda t: nn.layer_norm(x, t), lambda t: nn.layer_norm(x, None, t), lambda t: nn.layer_norm_backward(x, x, stat, stat, t),
+              lambda t: nn.dropout_add_layer_norm(x, x, w, t)):
+        for t in (freed, hidden, nothing):
+            with pytest.raises(RuntimeError):
+                f(t)
+    for t in (Wrapper(x), torch._efficientzerotensor((4, 8), device="cuda")):
+        with pytest.raises(RuntimeError):
+            nn.dropout_add_layer_norm_backward(x, t, x, stat, stat)
+    with pytest.raises(RuntimeError):
+        nn.dropout(x, nn.Drop(0.5, 1, 0, Wrapper(step)))
+    # what bias holds is not read by the gradient
+    want = nn.layer_norm_backward(x, x, stat, stat, w, w)
+    assert all(torch.equal(a, g) for a, g in zip(nn.layer_norm_backward(x, x, stat, stat, w, freed), want))
