@@ -5,6 +5,7 @@
 #include <c10/core/AutogradState.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/torch.h>
 
@@ -48,22 +49,26 @@ struct Arguments {
     if (given[i] == Py_None) return std::nullopt;
     return tensor(i, what);
   }
-  bool flag(int i) const { return PyObject_IsTrue(given[i]) == 1; }
+  bool flag(int i) const {
+    const int v = PyObject_IsTrue(given[i]);
+    if (v < 0) throw python_error();
+    return v;
+  }
   double number(int i) const {
     const double v = PyFloat_AsDouble(given[i]);
-    if (v == -1.0 && PyErr_Occurred()) throw std::domain_error("");
+    if (v == -1.0 && PyErr_Occurred()) throw python_error();
     return v;
   }
   void *stream(int i) const {
     void *p = PyLong_AsVoidPtr(given[i]);
-    if (!p && PyErr_Occurred()) throw std::domain_error("");
+    if (!p && PyErr_Occurred()) throw python_error();
     return p;
   }
 };
 
 uint64_t word(PyObject *o) { // modulo 2^64
   const uint64_t v = PyLong_AsUnsignedLongLongMask(o);
-  if (v == (uint64_t)-1 && PyErr_Occurred()) throw std::domain_error("");
+  if (v == (uint64_t)-1 && PyErr_Occurred()) throw python_error();
   return v;
 }
 
@@ -81,7 +86,7 @@ hctr_drop drop_of(const Arguments &a, int i, const Tensor &like) {
   if (o == Py_None) return d;
   if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) refuse("drop must be a Drop");
   d.p = PyFloat_AsDouble(PyTuple_GET_ITEM(o, 0));
-  if (d.p == -1.0 && PyErr_Occurred()) throw std::domain_error("");
+  if (d.p == -1.0 && PyErr_Occurred()) throw python_error();
   d.seed = word(PyTuple_GET_ITEM(o, 1));
   d.step = word(PyTuple_GET_ITEM(o, 2));
   PyObject *extra = PyTuple_GET_ITEM(o, 3);
@@ -297,17 +302,13 @@ PyObject *unseen_on(PyObject *, PyObject *x) {
   return PyLong_FromLong(!seen && t.is_cuda() ? t.get_device() : -1);
 }
 
-// An error that Python has set already travels as an empty domain_error.
+// An error comes out as torch's own operators raise it: memory that runs out as torch.OutOfMemoryError, what Python has set already
+// (python_error) as it is.
 template <PyObject *(*F)(const Arguments &)> PyObject *call(PyObject *, PyObject *const *args, Py_ssize_t count) {
-  try {
-    at::NoGradGuard off;
-    return F({args, count});
-  } catch (const std::domain_error &) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "hetuctr_amd.nn: unknown error");
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-  }
-  return nullptr;
+  HANDLE_TH_ERRORS
+  at::NoGradGuard off;
+  return F({args, count});
+  END_HANDLE_TH_ERRORS
 }
 template <PyObject *(*F)(const Arguments &)> PyCFunction method() { return (PyCFunction)(void (*)())call<F>; }
 

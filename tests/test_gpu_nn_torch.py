@@ -216,3 +216,25 @@ def test_tensors_without_memory_are_not_taken_for_missing_ones():
     # what bias holds is not read by the gradient
     want = nn.layer_norm_backward(x, x, stat, stat, w, w)
     assert all(torch.equal(a, g) for a, g in zip(nn.layer_norm_backward(x, x, stat, stat, w, freed), want))
+
+
+# ---- errors -----------------------------------------------------------------------------------------------------------------
+@gpu
+def test_errors_keep_their_type():
+    x = values((1, 1024), 1).expand(2 ** 33, 1024)             # its result would take 32 TiB
+    for f in (lambda: nn.dropout(x, nn.Drop(0.5, 1)), lambda: nn.layer_norm(x)):
+        with pytest.raises(torch.OutOfMemoryError):
+            f()
+    x = values((2, 8), 1)
+    with pytest.raises(RuntimeError) as e:
+        nn.layer_norm(x, eps=-1.0)
+    assert "eps" in str(e.value) and "frame #" not in str(e.value)
+    with pytest.raises(TypeError):
+        nn.layer_norm(x, eps="small")
+    with pytest.raises(TypeError):
+        nn.dropout(x, nn.Drop(0.5, "seed"))
+    with pytest.raises(RuntimeError, match="Boolean value"):
+        nn.layer_norm(x, stats=torch.ones(2))
+    with pytest.raises(RuntimeError) as e:
+        nn.layer_norm(x.to_sparse())
+    assert "frame #" not in str(e.value)
