@@ -302,6 +302,9 @@ PyObject *unseen_on(PyObject *, PyObject *x) {
   return PyLong_FromLong(!seen && t.is_cuda() ? t.get_device() : -1);
 }
 
+// Whether a tracer records torch's operators
+PyObject *traced(PyObject *, PyObject *) { return PyBool_FromLong(at::tracer::impl::is_dispatch_enabled()); }
+
 // An error comes out as torch's own operators raise it: memory that runs out as torch.OutOfMemoryError, what Python has set already
 // (python_error) as it is.
 template <PyObject *(*F)(const Arguments &)> PyObject *call(PyObject *, PyObject *const *args, Py_ssize_t count) {
@@ -316,6 +319,7 @@ PyMethodDef methods[] = {{"dropout", method<dropout>(), METH_FASTCALL, nullptr},
                          {"forward", method<forward>(), METH_FASTCALL, nullptr},
                          {"backward", method<backward>(), METH_FASTCALL, nullptr},
                          {"unseen_on", unseen_on, METH_O, nullptr},
+                         {"traced", traced, METH_NOARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "hetuctr_nn", "The dense operators on torch tensors; use hetuctr_amd.nn.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

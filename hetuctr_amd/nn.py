@@ -66,7 +66,7 @@ def _wants_gradient(*tensors):
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
-                return not torch._C._is_tracing()       # a traced operator asks again
+                return not _native.traced()              # a traced operator asks again
     return False
 
 
