@@ -18,7 +18,10 @@ SYMBOLS = ["hctr_create", "hctr_destroy", "hctr_preprocess", "hctr_preprocess_no
            "hctr_part_sizes", "hctr_part_refine_data", "hctr_part_refine_embed", "hctr_part_get_communication",
            "hctr_part_get_priority", "hctr_part_get_result", "hctr_part_get_counts", "hctr_part_cache_lists",
            "hctr_dropout", "hctr_layer_norm", "hctr_dropout_add_layer_norm", "hctr_layer_norm_backward",
-           "hctr_dropout_add_layer_norm_backward", "hctr_layer_norm_workspace"]
+           "hctr_dropout_add_layer_norm_backward", "hctr_layer_norm_workspace",
+           "hctr_gated_linear", "hctr_gated_linear_workspace", "hctr_gated_linear_backward", "hctr_gated_linear_backward_workspace",
+           "hctr_linear_cross_entropy", "hctr_linear_cross_entropy_workspace", "hctr_linear_cross_entropy_backward",
+           "hctr_linear_cross_entropy_backward_workspace", "hctr_gradient_norm", "hctr_clip_gradients", "hctr_gradient_workspace"]
 
 # items of hctr_debug_fetch (HCTR_F_*)
 UNIQUE, SORTED_ARG, RUN_START, IDX_MAP, ROOT, OFFSET, SEND_CNT, RECV_CNT = range(8)
@@ -86,6 +89,11 @@ def lib():
         for name in ("hctr_dropout", "hctr_layer_norm", "hctr_dropout_add_layer_norm", "hctr_layer_norm_backward",
                      "hctr_dropout_add_layer_norm_backward"):
             getattr(l, name).argtypes = [C.c_char_p]       # the packed argument record
+        for name in ("gated_linear", "gated_linear_backward", "linear_cross_entropy", "linear_cross_entropy_backward"):
+            getattr(l, "hctr_" + name).argtypes = getattr(l, "hctr_%s_workspace" % name).argtypes = [C.c_char_p]
+            getattr(l, "hctr_%s_workspace" % name).restype = C.c_size_t
+        l.hctr_gradient_norm.argtypes = l.hctr_clip_gradients.argtypes = l.hctr_gradient_workspace.argtypes = [C.c_char_p]
+        l.hctr_gradient_workspace.restype = C.c_size_t
         l.hctr_layer_norm_workspace.argtypes = [C.c_size_t, C.c_size_t]
         l.hctr_layer_norm_workspace.restype = C.c_size_t
         _lib = l
@@ -155,6 +163,56 @@ def dropout_add_layer_norm_backward(rows, width, dy, total, dtotal, dx, dresidua
     _check(lib().hctr_dropout_add_layer_norm_backward(_NORM_GRAD_ARGS.pack(
         rows, width, *dy, *total, *dtotal, *dx, *dresidual, weight, dweight, dbias, mean, rstd, workspace, workspace_bytes, *drop,
         stream, *dtypes)))
+
+
+# Products.  dtypes: of the matrices, of the biases; each call takes a workspace (pointer, bytes) of as many bytes as the same arguments
+# give with space=True, which makes no call.
+SILU, GELU, RELU, SIGMOID = range(4)
+_GATED_ARGS = struct.Struct("@QQQ" "PqPqPqPqPqPq" "PP" "PQP" "3i4x")
+_GATED_GRAD_ARGS = struct.Struct("@QQQ" "PqPqPqPqPqPqPqPqPq" "PP" "PQP" "3i4x")
+_ITEMS_ARGS = struct.Struct("@QQQ" "PqPq" "PPqPP" "PQP" "2i")
+_ITEMS_GRAD_ARGS = struct.Struct("@QQQ" "PqPqPqPq" "PPPqPP" "PQP" "2i")
+_GRADIENT, _CLIP_ARGS = struct.Struct("@PPQi4x"), struct.Struct("@PQPPf4x" "PQP")
+
+
+def _call(name, packed, space):
+    if not space:
+        return _check(getattr(lib(), name)(packed))
+    size = getattr(lib(), "hctr_gradient_workspace" if name.startswith(("hctr_gradient", "hctr_clip")) else name + "_workspace")(packed)
+    _check(size == 2 ** 64 - 1)
+    return size
+
+
+def gated_linear(rows, width, hidden, x, gate_weight, up_weight, h, gate, up, gate_bias, up_bias, workspace, dtypes, activation, stream=0,
+                 space=False):
+    return _call("hctr_gated_linear", _GATED_ARGS.pack(rows, width, hidden, *x, *gate_weight, *up_weight, *h, *gate, *up, gate_bias, up_bias,
+                                                       *workspace, stream, *dtypes, activation), space)
+
+
+def gated_linear_backward(rows, width, hidden, dh, x, gate, up, gate_weight, up_weight, dx, dgate_weight, dup_weight, dgate_bias, dup_bias,
+                          workspace, dtypes, activation, stream=0, space=False):
+    return _call("hctr_gated_linear_backward", _GATED_GRAD_ARGS.pack(
+        rows, width, hidden, *dh, *x, *gate, *up, *gate_weight, *up_weight, *dx, *dgate_weight, *dup_weight, dgate_bias, dup_bias, *workspace,
+        stream, *dtypes, activation), space)
+
+
+def linear_cross_entropy(rows, width, items, x, weight, bias, target, ignore_index, loss, lse, workspace, dtypes, stream=0, space=False):
+    return _call("hctr_linear_cross_entropy", _ITEMS_ARGS.pack(rows, width, items, *x, *weight, bias, target, ignore_index, loss, lse, *workspace,
+                                                               stream, *dtypes), space)
+
+
+def linear_cross_entropy_backward(rows, width, items, x, weight, dx, dweight, bias, dbias, target, ignore_index, dloss, lse, workspace, dtypes,
+                                  stream=0, space=False):
+    return _call("hctr_linear_cross_entropy_backward", _ITEMS_GRAD_ARGS.pack(
+        rows, width, items, *x, *weight, *dx, *dweight, bias, dbias, target, ignore_index, dloss, lse, *workspace, stream, *dtypes), space)
+
+
+def clip_gradients(gradients, max_norm, norm, given, workspace, stream=0, space=False, norm_only=False):
+    """gradients: (pointer, pointer to the result, values, type) of each"""
+    # (the array goes by address: it has to live until the call returns)
+    array = C.create_string_buffer(b"".join(_GRADIENT.pack(*g) for g in gradients), max(1, len(gradients) * _GRADIENT.size))
+    return _call("hctr_gradient_norm" if norm_only else "hctr_clip_gradients",
+                 _CLIP_ARGS.pack(C.addressof(array), len(gradients), norm, given, max_norm, *workspace, stream), space)
 
 
 class Table:

@@ -4,7 +4,10 @@
 #include <cstdio>
 #include <cstring>
 
+#include "clip.h"
 #include "dense.h"
+#include "gated.h"
+#include "items.h"
 #include "partition.h"
 #include "table.h"
 
@@ -399,6 +402,93 @@ int hctr_dropout_add_layer_norm_backward(const hctr_norm_grad_args *a) {
 }
 
 size_t hctr_layer_norm_workspace(size_t rows, size_t width) { return layer_norm_workspace(rows, width); }
+
+int hctr_gated_linear(const hctr_gated_args *a) {
+  return guarded([&] {
+    HCTR_CHECK(a, "null argument");
+    gated_linear(*a);
+  });
+}
+
+size_t hctr_gated_linear_workspace(const hctr_gated_args *a) {
+  size_t bytes = (size_t)-1;
+  guarded([&] {
+    HCTR_CHECK(a, "null argument");
+    bytes = gated_linear_workspace(*a);
+  });
+  return bytes;
+}
+
+int hctr_gated_linear_backward(const hctr_gated_grad_args *a) {
+  return guarded([&] {
+    HCTR_CHECK(a, "null argument");
+    gated_linear_backward(*a);
+  });
+}
+
+size_t hctr_gated_linear_backward_workspace(const hctr_gated_grad_args *a) {
+  size_t bytes = (size_t)-1;
+  guarded([&] {
+    HCTR_CHECK(a, "null argument");
+    bytes = gated_linear_backward_workspace(*a);
+  });
+  return bytes;
+}
+
+int hctr_linear_cross_entropy(const hctr_items_args *a) {
+  return guarded([&] {
+    HCTR_CHECK(a, "null argument");
+    linear_cross_entropy(*a);
+  });
+}
+
+size_t hctr_linear_cross_entropy_workspace(const hctr_items_args *a) {
+  size_t bytes = (size_t)-1;
+  guarded([&] {
+    HCTR_CHECK(a, "null argument");
+    bytes = linear_cross_entropy_workspace(*a);
+  });
+  return bytes;
+}
+
+int hctr_linear_cross_entropy_backward(const hctr_items_grad_args *a) {
+  return guarded([&] {
+    HCTR_CHECK(a, "null argument");
+    linear_cross_entropy_backward(*a);
+  });
+}
+
+size_t hctr_linear_cross_entropy_backward_workspace(const hctr_items_grad_args *a) {
+  size_t bytes = (size_t)-1;
+  guarded([&] {
+    HCTR_CHECK(a, "null argument");
+    bytes = linear_cross_entropy_backward_workspace(*a);
+  });
+  return bytes;
+}
+
+int hctr_gradient_norm(const hctr_clip_args *a) {
+  return guarded([&] {
+    HCTR_CHECK(a, "null argument");
+    gradient_norm(*a, false);
+  });
+}
+
+int hctr_clip_gradients(const hctr_clip_args *a) {
+  return guarded([&] {
+    HCTR_CHECK(a, "null argument");
+    gradient_norm(*a, true);
+  });
+}
+
+size_t hctr_gradient_workspace(const hctr_clip_args *a) {
+  size_t bytes = (size_t)-1;
+  guarded([&] {
+    HCTR_CHECK(a, "null argument");
+    bytes = gradient_workspace(*a);
+  });
+  return bytes;
+}
 
 #pragma GCC visibility pop
 } // extern "C"

@@ -1,0 +1,7 @@
+#include "gated_kernels.h"
+
+namespace hctr {
+template void launch_gated<f16_t>(GatedForward &, int, hipStream_t);
+template void launch_gated_few<f16_t>(const GatedForward &, hipStream_t);
+template void launch_slopes<f16_t>(const GatedSlopes &, hipStream_t);
+} // namespace hctr

@@ -1,0 +1,185 @@
+// The kernels of gated.h for one type; gated_*.hip build them side by side.
+#pragma once
+#include "few_rows.h"
+#include "gated.h"
+
+namespace hctr {
+
+// sigmoid(v) and 1 - sigmoid(v), neither by cancellation
+struct Sigmoid {
+  float s, rest;
+};
+__device__ __forceinline__ Sigmoid sigmoid(float v) {
+  const float e = expf(-fabsf(v)), large = 1.f / (1.f + e), small = e * large;
+  return v >= 0.f || v != v ? Sigmoid{large, small} : Sigmoid{small, large};
+}
+// the normal distribution's integral
+__device__ __forceinline__ float normal_integral(float v) { return 0.5f * erfcf(v * -0.70710678118654752f); }
+
+__device__ __forceinline__ float activated(int f, float v) {
+  if (f == HCTR_SILU) return v * sigmoid(v).s;
+  if (f == HCTR_GELU) return v * normal_integral(v);
+  if (f == HCTR_RELU) return v > 0.f || v != v ? v : 0.f;
+  return sigmoid(v).s;
+}
+// f(v) and f'(v)
+struct Slope {
+  float value, slope;
+};
+__device__ __forceinline__ Slope slope_of(int f, float v) {
+  if (f == HCTR_GELU) {
+    const float whole = normal_integral(v);
+    return {v * whole, whole + v * 0.39894228040143268f * expf(-0.5f * v * v)};
+  }
+  if (f == HCTR_RELU) return {v > 0.f || v != v ? v : 0.f, v > 0.f ? 1.f : 0.f};
+  const Sigmoid g = sigmoid(v);
+  if (f == HCTR_SILU) return {v * g.s, g.s + v * g.s * g.rest};
+  return {g.s, g.s * g.rest};
+}
+
+// four neighbouring columns of the result
+template <typename T> __device__ __forceinline__ void finish_gated(const GatedForward &p, uint32_t row, uint32_t column, f32x4 gate, f32x4 up) {
+  f32x4 h;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    gate[e] += bias_at<T>(p.gate_bias, p.narrow, column + e, p.hidden);
+    up[e] += bias_at<T>(p.up_bias, p.narrow, column + e, p.hidden);
+    h[e] = activated(p.activation, gate[e]) * up[e];
+  }
+  write4<T>((T *)p.h + (int64_t)row * p.h_stride, column, p.hidden, p.vectors, h);
+  if (p.gate) write4<T>((T *)p.gate + (int64_t)row * p.gate_stride, column, p.hidden, p.vectors, gate);
+  if (p.up) write4<T>((T *)p.up + (int64_t)row * p.up_stride, column, p.hidden, p.vectors, up);
+}
+
+// Both products in one: the rows of the two matrices of weights alternate in a tile, 32 by 32, so that a wave holds the same columns of
+// both, and makes h of them.
+template <typename T, int TILE> __global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kPaired, TILE, TILE>::kThreads), 2)
+void gated_product(GatedForward p) {
+  typedef Product<T, Lies::kAlong, Lies::kAlong, Second::kPaired, TILE, TILE> P;
+  __shared__ __attribute__((aligned(1024))) char tiles[P::kLdsBytes];
+  uint32_t row, column;
+  tile_of(blockIdx.x, gridDim.x, p.row_tiles, p.column_tiles, p.band, row, column);
+  const uint32_t steps = (p.width + kStep<T> - 1) / kStep<T>, each = (steps + p.splits - 1) / p.splits;
+  const uint32_t k0 = blockIdx.y * each * kStep<T>, k1 = min(p.width, k0 + each * kStep<T>);
+  typename P::Sums sum;
+  P::run(p.x, p.weights, row * TILE, column * TILE, k0, k1, (uint32_t)(uintptr_t)(lds_char *)tiles, sum);
+  const uint32_t l = lane_id(), half = (p.hidden + 3) / 4 * 4;
+#pragma unroll
+  for (int i = 0; i < P::kRowTiles; i++) {
+    const uint32_t r = row * TILE + P::wave_row() + i * 16 + l % 16;
+    if (r >= p.rows) continue;
+#pragma unroll
+    for (int j = 0; j < P::kColumnTiles / 2; j++) {
+      const uint32_t c = (column * TILE + P::wave_column()) / 2 + j * 16 + l / 16 * 4;
+      if (c >= p.hidden) continue;
+      if (!p.partial) {
+        finish_gated<T>(p, r, c, sum[i][j], sum[i][j + P::kColumnTiles / 2]);
+      } else {
+        float *part = p.partial + ((uint64_t)blockIdx.y * p.rows + r) * (2 * half) + c;
+        *(f32x4 *)part = sum[i][j];
+        *(f32x4 *)(part + half) = sum[i][j + P::kColumnTiles / 2];
+      }
+    }
+  }
+}
+
+template <typename T> __global__ __launch_bounds__(256) void gated_join(GatedForward p) {
+  const uint32_t quads = (p.hidden + 3) / 4;
+  const uint64_t total = (uint64_t)p.rows * quads;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
+    const uint64_t r = total >> 32 ? i / quads : (uint32_t)i / quads;
+    const uint32_t c = (uint32_t)(i - r * quads);
+    const f32x4 *from = (const f32x4 *)p.partial + r * (2 * quads) + c;
+    f32x4 gate = from[0], up = from[quads];
+    for (uint32_t s = 1; s < p.splits; s++) {
+      from += (uint64_t)p.rows * (2 * quads);
+      gate += from[0], up += from[quads];
+    }
+    finish_gated<T>(p, (uint32_t)r, c * 4, gate, up);
+  }
+}
+
+template <typename T, int ROWS> __global__ __launch_bounds__((FewRows<T, ROWS>::kThreads)) void gated_few(GatedForward p) {
+  typedef FewRows<T, ROWS> F;
+  __shared__ typename F::Sums sums[F::kWaves];
+  const uint32_t column0 = blockIdx.x * 16, left = min(16u, p.hidden - column0);
+  F::run((const T *)p.loose_x, p.loose_stride, p.rows, (const T *)p.loose_gate + (int64_t)column0 * p.loose_gate_stride,
+         (const T *)p.loose_up + (int64_t)column0 * p.loose_up_stride, left, left, p.loose_gate_stride, p.loose_up_stride, p.width, sums);
+  for (uint32_t t = threadIdx.x; t < p.rows * 4; t += F::kThreads) {
+    const uint32_t r = t / 4, c = t % 4 * 4;
+    if (c < left) finish_gated<T>(p, r, column0 + c, F::joined(sums, r, c), F::joined(sums, r, c + 16));
+  }
+}
+
+// dgate and dup of columns c .. c + V - 1 of a block's rows, and the sums over them.  Eight threads share out the rows of 32 pieces.
+template <typename T, bool SUMS> __global__ __launch_bounds__(256) void gated_slopes(GatedSlopes p) {
+  constexpr int V = kVec<T>, LANES = 32, GROUPS = 8;
+  __shared__ float joined[SUMS ? GROUPS : 1][2][LANES * V];
+  const uint32_t x = threadIdx.x % LANES, y = threadIdx.x / LANES, c = (blockIdx.x * LANES + x) * V;
+  const uint32_t first = blockIdx.y * p.rows_each, last = min(p.rows, first + p.rows_each);
+  Floats<V> sums[2] = {};
+  if (c < p.padded)
+    for (uint32_t r = first + y; r < last; r += GROUPS) {
+      const Floats<V> dh = load_columns<V, Rows::kLong, true>((const T *)p.dh + (int64_t)r * p.dh_stride, c, p.hidden);
+      const Floats<V> gate = load_columns<V, Rows::kLong, true>((const T *)p.gate + (int64_t)r * p.gate_stride, c, p.hidden);
+      const Floats<V> up = load_columns<V, Rows::kLong, true>((const T *)p.up + (int64_t)r * p.up_stride, c, p.hidden);
+      Floats<V> d[2];
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        const Slope s = slope_of(p.activation, gate.v[e]);
+        d[0].v[e] = c + e < p.hidden ? dh.v[e] * up.v[e] * s.slope : 0.f;
+        d[1].v[e] = c + e < p.hidden ? dh.v[e] * s.value : 0.f;
+      }
+      T *to = (T *)p.slopes + (uint64_t)r * (2 * p.padded) + c;
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        *(typename Packed<T, V>::type *)(to + i * p.padded) = rounded<T>(d[i]);
+        if (SUMS)
+#pragma unroll
+          for (int e = 0; e < V; e++) sums[i].v[e] += d[i].v[e];
+      }
+    }
+  if constexpr (SUMS) {
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int e = 0; e < V; e++) joined[y][i][e * LANES + x] = sums[i].v[e];
+    __syncthreads();
+    for (uint32_t t = threadIdx.x; t < 2 * LANES * V; t += 256) {
+      const uint32_t i = t / (LANES * V), at = t % (LANES * V), column = blockIdx.x * LANES * V + at;
+      float sum = 0.f;
+#pragma unroll
+      for (int g = 0; g < GROUPS; g++) sum += joined[g][i][at % V * LANES + at / V];
+      if (column < p.padded) p.sums[(uint64_t)blockIdx.y * (2 * p.padded) + i * p.padded + column] = sum;
+    }
+  }
+}
+
+template <typename T> void launch_gated(GatedForward &p, int tile, hipStream_t s) {
+  p.row_tiles = div_up(p.rows, tile), p.column_tiles = div_up(p.hidden, tile / 2);
+  HCTR_CHECK((uint64_t)p.row_tiles * p.column_tiles * 512 < (1ull << 32), "gated linear: too many tiles");
+  const dim3 blocks(p.row_tiles * p.column_tiles, p.splits);
+  if (tile == 256) hipLaunchKernelGGL((gated_product<T, 256>), blocks, dim3(512), 0, s, p);
+  else hipLaunchKernelGGL((gated_product<T, 128>), blocks, dim3(256), 0, s, p);
+  HCTR_HIP(hipGetLastError());
+  if (p.partial) {
+    const uint64_t quads = (uint64_t)p.rows * ((p.hidden + 3) / 4);
+    hipLaunchKernelGGL((gated_join<T>), dim3((unsigned)min((quads + 255) / 256, (uint64_t)16384)), dim3(256), 0, s, p);
+    HCTR_HIP(hipGetLastError());
+  }
+}
+template <typename T> void launch_gated_few(const GatedForward &p, hipStream_t s) {
+  const dim3 blocks(div_up(p.hidden, 16));
+  if (p.rows <= 16) hipLaunchKernelGGL((gated_few<T, 16>), blocks, dim3(FewRows<T, 16>::kThreads), 0, s, p);
+  else if (p.rows <= 32) hipLaunchKernelGGL((gated_few<T, 32>), blocks, dim3(FewRows<T, 32>::kThreads), 0, s, p);
+  else hipLaunchKernelGGL((gated_few<T, 64>), blocks, dim3(FewRows<T, 64>::kThreads), 0, s, p);
+  HCTR_HIP(hipGetLastError());
+}
+template <typename T> void launch_slopes(const GatedSlopes &p, hipStream_t s) {
+  const dim3 blocks(div_up(p.padded, 32 * kVec<T>), div_up(p.rows, p.rows_each));
+  if (p.sums) hipLaunchKernelGGL((gated_slopes<T, true>), blocks, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((gated_slopes<T, false>), blocks, dim3(256), 0, s, p);
+  HCTR_HIP(hipGetLastError());
+}
+
+} // namespace hctr

@@ -1,0 +1,260 @@
+// The kernels of items.h for one type; items_*.hip build them side by side.
+#pragma once
+#include "few_rows.h"
+#include "items.h"
+#include "items_tail.h"
+
+namespace hctr {
+
+// logits of N neighbouring items, those behind the last one left out
+template <int N> __device__ __forceinline__ Tail tail_of(const f32x4 (&v)[N]) {
+  float most = -kInfinity;
+#pragma unroll
+  for (int j = 0; j < N; j++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) most = fmaxf(most, v[j][e]);
+  Tail t = {most, 0.f};
+  // (a NaN is not the largest, but makes the sum one; with no finite largest value every term is one or zero)
+  const float less = most == -kInfinity ? 0.f : most;
+#pragma unroll
+  for (int j = 0; j < N; j++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) t.sum += exp_less(v[j][e], less);
+  if (t.sum != t.sum) t.most = t.sum;
+  return t;
+}
+
+template <typename T> __device__ __forceinline__ f32x4 bias4(const ItemsProduct &p, uint32_t c) {
+  f32x4 b;
+#pragma unroll
+  for (int e = 0; e < 4; e++) b[e] = c + e < p.items ? bias_at<T>(p.bias, p.narrow, c + e, p.items) : -kInfinity;
+  return b;
+}
+
+// d of four items of a row
+__device__ __forceinline__ f32x4 slope4(f32x4 logit, float lse, float scale, uint32_t hit) {
+  f32x4 d;
+#pragma unroll
+  for (int e = 0; e < 4; e++) d[e] = (exp_less(logit[e], lse) - (hit == (uint32_t)e ? 1.f : 0.f)) * scale;
+  return d;
+}
+
+template <typename T, int TILE, bool GRADIENT>
+__global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kNone, TILE, TILE>::kThreads), 2) void items_product(ItemsProduct p) {
+  typedef Product<T, Lies::kAlong, Lies::kAlong, Second::kNone, TILE, TILE> P;
+  __shared__ __attribute__((aligned(1024))) char tiles[P::kLdsBytes];
+  uint32_t row, column;
+  tile_of(blockIdx.x, gridDim.x, p.row_tiles, p.column_tiles, p.band, row, column);
+  const uint32_t rows = *p.taken.count, row0 = row * TILE, column0 = column * TILE;
+  if (row0 >= rows) return;
+  typename P::Sums sum;
+  P::run(p.x, p.weight, row0, column0, 0, p.width, (uint32_t)(uintptr_t)(lds_char *)tiles, sum);
+  const uint32_t l = lane_id(), wave_column = P::wave_column();
+  f32x4 bias[P::kColumnTiles];
+#pragma unroll
+  for (int j = 0; j < P::kColumnTiles; j++) bias[j] = bias4<T>(p, column0 + wave_column + j * 16 + l / 16 * 4);
+  __syncthreads(); // the tiles are read
+  if constexpr (!GRADIENT) {
+    constexpr int ACROSS = TILE / 64;
+    Tail *tails = (Tail *)tiles; // [ACROSS][TILE]
+#pragma unroll
+    for (int i = 0; i < P::kRowTiles; i++) {
+      const uint32_t in = P::wave_row() + i * 16 + l % 16, r = row0 + in;
+#pragma unroll
+      for (int j = 0; j < P::kColumnTiles; j++) sum[i][j] += bias[j];
+      const uint32_t target = r < rows ? p.taken.target[r] : kNoItem;
+#pragma unroll
+      for (int j = 0; j < P::kColumnTiles; j++) {
+        const uint32_t e = target - (column0 + wave_column + j * 16 + l / 16 * 4);
+        if (e < 4) p.hit[r] = e < 2 ? (e ? sum[i][j][1] : sum[i][j][0]) : (e == 2 ? sum[i][j][2] : sum[i][j][3]);
+      }
+      Tail t = tail_of(sum[i]);
+      t = join_lanes(t, 16);
+      t = join_lanes(t, 32);
+      if (l < 16) tails[wave_column / 64 * TILE + in] = t;
+    }
+    __syncthreads();
+    const uint32_t r = threadIdx.x;
+    if (r < TILE && row0 + r < rows) {
+      Tail t = tails[r];
+#pragma unroll
+      for (int w = 1; w < ACROSS; w++) t = join(t, tails[w * TILE + r]);
+      p.parts[(uint64_t)column * p.rows + row0 + r] = make_float2(t.most, t.sum);
+    }
+  } else {
+    const float scale = p.taken.scale[0];
+    f32x4 down[P::kColumnTiles] = {};
+#pragma unroll
+    for (int i = 0; i < P::kRowTiles; i++) {
+      const uint32_t r = row0 + P::wave_row() + i * 16 + l % 16;
+      if (r >= rows) continue;
+      const float lse = p.taken.lse[r], dloss = p.taken.dloss[r] * scale;
+      const uint32_t target = p.taken.target[r] - p.first;
+#pragma unroll
+      for (int j = 0; j < P::kColumnTiles; j++) {
+        const uint32_t c = column0 + wave_column + j * 16 + l / 16 * 4;
+        const f32x4 d = slope4(sum[i][j] + bias[j], lse, dloss, target - c);
+        down[j] += d;
+        if (c < p.d_stride) write4<T>((T *)p.d + (uint64_t)r * p.d_stride, c, p.d_stride, true, d);
+      }
+    }
+    if (p.sums) {
+      f32x4 *joined = (f32x4 *)tiles; // [2][TILE / 4]
+#pragma unroll
+      for (int j = 0; j < P::kColumnTiles; j++) {
+#pragma unroll
+        for (int mask = 1; mask < 16; mask *= 2)
+#pragma unroll
+          for (int e = 0; e < 4; e++) down[j][e] += __shfl_xor(down[j][e], mask);
+        if (l % 16 == 0) joined[(P::wave_row() ? TILE / 4 : 0) + (wave_column + j * 16) / 4 + l / 16] = down[j];
+      }
+      __syncthreads();
+      const uint32_t c = threadIdx.x * 4;
+      if (c < TILE && column0 + c < p.d_stride) *(f32x4 *)(p.sums + (uint64_t)row * p.d_stride + column0 + c) = joined[c / 4] + joined[TILE / 4 + c / 4];
+    }
+  }
+}
+
+template <typename T, int ROWS, bool GRADIENT> __global__ __launch_bounds__((FewRows<T, ROWS>::kThreads)) void items_few(ItemsProduct p) {
+  typedef FewRows<T, ROWS> F;
+  static_assert(ROWS * 8 <= F::kThreads, "a thread takes four items of a row");
+  __shared__ typename F::Sums sums[F::kWaves];
+  const uint32_t rows = *p.taken.count, column0 = blockIdx.x * kFewItems, left = p.items - column0;
+  if (!rows) return;
+  const T *weight = (const T *)p.loose_weight + (int64_t)column0 * p.loose_stride;
+  const bool second = left > 16;
+  // (the second sixteen are the first ones again if there are no more)
+  F::run((const T *)p.few_x, p.few_stride, rows, weight, weight + (second ? 16 * p.loose_stride : 0), min(left, 16u), second ? min(left - 16, 16u) : min(left, 16u),
+         p.loose_stride, p.loose_stride, p.width, sums);
+  const uint32_t t = threadIdx.x, r = t / 8, c = t % 8 * 4;
+  f32x4 d = {};
+  if (r < rows && r < ROWS) {
+    const f32x4 logit[1] = {F::joined(sums, r, c) + bias4<T>(p, column0 + c)};
+    if constexpr (!GRADIENT) {
+      const uint32_t e = p.taken.target[r] - (column0 + c);
+      if (e < 4) p.hit[r] = e < 2 ? (e ? logit[0][1] : logit[0][0]) : (e == 2 ? logit[0][2] : logit[0][3]);
+      Tail tail = tail_of(logit);
+      for (int mask = 1; mask < 8; mask *= 2) tail = join_lanes(tail, mask);
+      if (c == 0) p.parts[(uint64_t)blockIdx.x * p.rows + r] = make_float2(tail.most, tail.sum);
+    } else {
+      d = slope4(logit[0], p.taken.lse[r], p.taken.dloss[r] * p.taken.scale[0], p.taken.target[r] - p.first - (column0 + c));
+      if (column0 + c < p.d_stride) write4<T>((T *)p.d + (uint64_t)r * p.d_stride, column0 + c, p.d_stride, true, d);
+    }
+  }
+  if (GRADIENT && p.sums) {
+    __syncthreads(); // the sums are read
+    if (r < ROWS) *(f32x4 *)&sums[0][r][c] = d;
+    __syncthreads();
+    if (t < 8 && column0 + t * 4 < p.d_stride) {
+      f32x4 all = {};
+      for (uint32_t i = 0; i < min(rows, (uint32_t)ROWS); i++) all += *(const f32x4 *)&sums[0][i][t * 4];
+      *(f32x4 *)(p.sums + column0 + t * 4) = all;
+    }
+  }
+}
+
+template <typename T, bool GRADIENT> void launch_items(ItemsProduct &p, int tile, hipStream_t s) {
+  if (!tile) {
+    p.column_tiles = div_up(p.items, kFewItems);
+    const dim3 blocks(p.column_tiles), threads(FewRows<T, 16>::kThreads);
+    if (p.rows <= 16) hipLaunchKernelGGL((items_few<T, 16, GRADIENT>), blocks, threads, 0, s, p);
+    else if (p.rows <= 32) hipLaunchKernelGGL((items_few<T, 32, GRADIENT>), blocks, threads, 0, s, p);
+    else hipLaunchKernelGGL((items_few<T, 64, GRADIENT>), blocks, threads, 0, s, p);
+  } else {
+    p.row_tiles = div_up(p.rows, tile), p.column_tiles = div_up(p.items, tile);
+    HCTR_CHECK((uint64_t)p.row_tiles * p.column_tiles * 512 < (1ull << 32), "linear cross entropy: too many tiles");
+    const dim3 blocks(p.row_tiles * p.column_tiles);
+    if (tile == 256) hipLaunchKernelGGL((items_product<T, 256, GRADIENT>), blocks, dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((items_product<T, 128, GRADIENT>), blocks, dim3(256), 0, s, p);
+  }
+  HCTR_HIP(hipGetLastError());
+}
+template <typename T> void launch_items_forward(ItemsProduct &p, int tile, hipStream_t s) { launch_items<T, false>(p, tile, s); }
+template <typename T> void launch_items_gradient(ItemsProduct &p, int tile, hipStream_t s) { launch_items<T, true>(p, tile, s); }
+
+// The power of two that brings the largest |dloss| to 2^13 .. 2^14, where a value of half precision is rounded to 11 bits down to 2^-27 of it
+__device__ __forceinline__ float scale_for(uint32_t most) {
+  if (!most) return 1.f;
+  const int exponent = max(-100, (int)(most >> 23) - 126); // most < 2^exponent
+  return ldexpf(1.f, 14 - exponent);
+}
+
+// Eight rows a block (a wave copies one at a time): it finds how many of those before them take part from the chunks' counts and its own
+// chunk's targets.
+constexpr uint32_t kTakeRows = 8;
+template <typename T> __global__ __launch_bounds__(256) void take_rows(TakeRows p) {
+  constexpr int V = kVec<T>;
+  __shared__ uint32_t words[5];
+  __shared__ uint32_t place[kTakeRows];
+  const uint32_t first = blockIdx.x * kTakeRows, chunk = first / kChunk, t = threadIdx.x;
+  const uint32_t in = first % kChunk, chunk_rows = min(kChunk, p.rows - chunk * kChunk);
+  // the rows of the chunk before this block's, and of the chunks before it; block 0 looks at all of them
+  uint32_t before = 0, all = 0, most = 0;
+  const bool head = blockIdx.x == 0;
+  for (uint32_t i = t; i < (head ? chunk_rows : in); i += 256) {
+    const uint32_t r = chunk * kChunk + i;
+    const bool taken = p.target[r] != p.ignored;
+    before += taken && i < in;
+    all += taken;
+    if (head && taken && p.scaled) most = max(most, size_bits(p.dloss[r]));
+  }
+  if (p.chunks) {
+    const uint32_t chunks = (p.rows + kChunk - 1) / kChunk;
+    if (head) all = most = 0;
+    for (uint32_t i = t; i < (head ? chunks : chunk); i += 256) {
+      const uint2 c = p.chunks[i];
+      if (head) all += c.x, most = max(most, c.y);
+      else before += c.x;
+    }
+  }
+  if (head) before = 0;
+  uint32_t total;
+  block_exclusive_scan<256>(head ? all : before, words, total);
+  if (head) {
+    __shared__ uint32_t largest[4];
+#pragma unroll
+    for (int mask = 32; mask; mask /= 2) most = max(most, (uint32_t)__shfl_xor((int)most, mask));
+    if (lane_id() == 0) largest[t / kWave] = most;
+    __syncthreads();
+    if (t == 0) {
+      *p.taken.count = total;
+      const float scale = p.scaled ? scale_for(max(max(largest[0], largest[1]), max(largest[2], largest[3]))) : 1.f;
+      p.taken.scale[0] = scale, p.taken.scale[1] = 1.f / scale;
+    }
+  }
+  if (t < kTakeRows) {
+    const uint32_t r = first + t;
+    const int64_t target = r < p.rows ? p.target[r] : p.ignored;
+    const bool taken = target != p.ignored;
+    const uint32_t mask = (uint32_t)__ballot(taken) & ((1u << kTakeRows) - 1);
+    const uint32_t to = (head ? 0 : total) + __popc(mask & ((1u << t) - 1));
+    place[t] = taken ? to : kNoItem;
+    if (taken) {
+      p.taken.row_of[to] = r;
+      p.taken.target[to] = target >= 0 && target < (int64_t)p.items ? (uint32_t)target : kNoItem;
+      if (p.dloss) p.taken.dloss[to] = p.dloss[r], p.taken.lse[to] = p.lse_in[r];
+    } else if (r < p.rows) {
+      if (p.loss) p.loss[r] = 0.f;
+      if (p.lse) p.lse[r] = 0.f;
+    }
+  }
+  __syncthreads();
+  for (uint32_t i = t / kWave; i < kTakeRows; i += 256 / kWave) {
+    const uint32_t r = first + i, to = place[i];
+    if (r >= p.rows) break;
+    if (to != kNoItem) {
+      const T *from = (const T *)p.x + (int64_t)r * p.x_stride;
+      for (uint32_t c = lane_id() * V; c < p.to_stride; c += kWave * V)
+        *(typename Packed<T, V>::type *)((T *)p.to + (uint64_t)to * p.to_stride + c) = settled<V, Rows::kLong>(load_raw<V, Rows::kLong>(from, c, p.width), c, p.width);
+    } else if (p.dx) {
+      T *dx = (T *)p.dx + (int64_t)r * p.dx_stride;
+      for (uint32_t c = lane_id() * V; c < p.width; c += kWave * V) store_columns<V, Rows::kLong>(dx, c, p.width, Floats<V>{});
+    }
+  }
+}
+template <typename T> void launch_take_rows(const TakeRows &p, hipStream_t s) {
+  hipLaunchKernelGGL((take_rows<T>), dim3(div_up(p.rows, kTakeRows)), dim3(256), 0, s, p);
+  HCTR_HIP(hipGetLastError());
+}
+
+} // namespace hctr

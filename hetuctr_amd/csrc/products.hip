@@ -1,0 +1,84 @@
+// The choice of tiles for a product, matrices laid out for tiles, sums over rows.
+#include <algorithm>
+
+#include "products.h"
+
+namespace hctr {
+
+// The tile and the number of parts along k that a product should take least time with, in us.  A tile of 256 x 256 has a CU for itself and takes
+// `large` us for a step of 128 bytes of k; of those of 128 x 128 two share a CU: `two` us a step, or `one` while it is alone.  Parts are
+// written and read again as floats.
+Shape shape_of(size_t rows, size_t columns, size_t k, int size, bool paired, bool may_split) {
+  const double large = size == 2 ? 1.8 : 7.7, two = size == 2 ? 1.05 : 3.9, one = size == 2 ? 0.8 : 2.0;
+  const size_t cus = 256, steps = (k * size + kStepBytes - 1) / kStepBytes, wide = paired ? 2 * columns : columns;
+  Shape best = {128, 1};
+  double least = 1e30;
+  for (int tile : {256, 128}) {
+    const size_t tiles = ((rows + tile - 1) / tile) * ((wide + tile - 1) / tile);
+    for (uint32_t splits = 1; splits <= (may_split ? 64u : 1u) && (splits == 1 || steps / splits >= 4); splits *= 2) {
+      const size_t blocks = tiles * splits, each = (steps + splits - 1) / splits;
+      double t;
+      if (tile == 256) t = (double)((blocks + cus - 1) / cus) * (each * large + 4.0);
+      else if (blocks <= cus) t = each * one + 4.0;
+      else t = (double)((blocks + 2 * cus - 1) / (2 * cus)) * (each * two + 4.0);
+      if (splits > 1) t += 4.0 + 2e-6 * parts_bytes(rows, wide, splits) / 4.0;
+      if (t < least) least = t, best = {tile, splits};
+    }
+  }
+  return best;
+}
+
+Layout laid_out(const hctr_matrix &m, size_t rows, size_t width, int dtype, char *&space, hipStream_t s) {
+  const size_t size = size_of(dtype);
+  if (!rows || fits(m, rows, width, size)) return {(const char *)m.data, rows > 1 ? m.stride * (int64_t)size : (int64_t)(width * size)};
+  const size_t stride = up(width * size, 16);
+  const Layout l = {space, (int64_t)stride};
+  if (dtype == HCTR_F32) launch_copy_rows<float>(m, rows, width, space, stride, s);
+  else if (dtype == HCTR_BF16) launch_copy_rows<bf16_t>(m, rows, width, space, stride, s);
+  else launch_copy_rows<f16_t>(m, rows, width, space, stride, s);
+  space += laid_out_bytes(m, rows, width, size);
+  return l;
+}
+
+namespace {
+
+// 16 neighbouring columns per block, whose threads share out the rows, eight loads under way, and join their sums through LDS, in
+// an order that depends on the sizes alone.
+constexpr int kSumThreads = 512, kSumColumns = 16;
+template <typename W> __global__ __launch_bounds__(kSumThreads) void column_sums(ColumnSums p) {
+  constexpr uint32_t ROWS = kSumThreads / kSumColumns, LOADS = 8;
+  __shared__ float sums[ROWS][kSumColumns + 1];
+  const uint32_t x = threadIdx.x % kSumColumns, y = threadIdx.x / kSumColumns, c = blockIdx.x * kSumColumns + x;
+  const uint32_t rows = p.rows_there ? min(p.rows, (*p.rows_there + p.per - 1) / p.per) : p.rows;
+  float sum = 0.f;
+  for (uint32_t i = y; i < rows; i += ROWS * LOADS) {
+    float v[LOADS];
+#pragma unroll
+    for (uint32_t k = 0; k < LOADS; k++) v[k] = c < p.columns && i + k * ROWS < rows ? p.partial[(uint64_t)(i + k * ROWS) * p.columns + c] : 0.f;
+#pragma unroll
+    for (uint32_t k = 0; k < LOADS; k++) sum += v[k];
+  }
+  sums[y][x] = sum;
+  __syncthreads();
+  if (y || c >= p.columns) return;
+  sum = 0.f;
+#pragma unroll
+  for (uint32_t i = 0; i < ROWS; i++) sum += sums[i][x];
+  if (p.scale) sum *= *p.scale;
+  const bool second = c >= p.second_from;
+  const uint32_t at = c - (second ? p.second_from : 0);
+  W *to = (W *)(second ? p.out[1] : p.out[0]);
+  if (to && at < p.count) to[at] = (W)sum;
+}
+
+} // namespace
+
+void launch_column_sums(const ColumnSums &c, int dtype, hipStream_t s) {
+  const dim3 blocks(div_up(c.columns, kSumColumns)), threads(kSumThreads);
+  if (dtype == HCTR_F32) hipLaunchKernelGGL((column_sums<float>), blocks, threads, 0, s, c);
+  else if (dtype == HCTR_BF16) hipLaunchKernelGGL((column_sums<bf16_t>), blocks, threads, 0, s, c);
+  else hipLaunchKernelGGL((column_sums<f16_t>), blocks, threads, 0, s, c);
+  HCTR_HIP(hipGetLastError());
+}
+
+} // namespace hctr

@@ -1,12 +1,16 @@
-"""Operators between the table's rows and a dense model, on torch tensors: dropout from a counter-based generator, layer
-normalisation, and both in one pass, with their gradients.  The reference has none of them: its table hands float rows to a model
-that lives outside (tests/check.py:44), and takes the gradient of those rows back.
+"""Operators between the table's rows and a dense model, and of the model's training step, on torch tensors: dropout from a
+counter-based generator, layer normalisation, and both in one pass; a gated linear layer; softmax cross entropy over many items (the rows of a
+table, say); with their gradients; the norm of all gradients and clipping by it.  The reference has none of them: its table hands
+float rows to a model that lives outside (tests/check.py:44), and takes the gradient of those rows back.
 
     table.preprocess(ids.data_ptr(), n); table.push_pull(grad_ptr, rows.data_ptr())
     rows.requires_grad_()
     h = nn.layer_norm(rows, weight, bias, drop=nn.Drop(0.1, seed=1, step=t), dtype=torch.bfloat16)
     ...                                                     # the dense model
+    h = nn.gated_linear(h, gate_weight, up_weight)
+    loss = nn.linear_cross_entropy(h, item_vectors, target).mean()
     loss.backward()                                         # rows.grad: float32, what the next push_pull takes
+    nn.clip_gradients([p.grad for p in parameters] + [rows.grad], 1.0)
 
 A tensor's last dimension is a row; the others, if any, count rows.  Rows of float32, bfloat16 or float16 may lie any number of
 elements apart; where the tensor's memory order does not allow that, a call copies it first.  Results are new contiguous
@@ -53,6 +57,8 @@ class Drop(NamedTuple):
 
 def _run(f, x, *args):
     """f(*args, torch's current stream), on the device of x; as one of torch's operators while something watches them"""
+    if x is None:
+        raise RuntimeError("hetuctr_amd.nn: there are no gradients")
     index = _native.unseen_on(x)
     if index < 0:
         return _as_operator(f, x, args)
@@ -173,6 +179,102 @@ def dropout_add_layer_norm_backward(dy, ds, s, mean, rstd, weight=None, bias=Non
     return _run(_native.backward, s, True, dy, ds, s, mean, rstd, weight, bias, drop, True, True, True)
 
 
+# ---- a gated linear layer ---------------------------------------------------------------------------------------------
+_ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate_weight, up_weight, gate_bias, up_bias, activation):
+        h, gate, up = _run(_native.gated, x, x, gate_weight, up_weight, gate_bias, up_bias, activation, True)
+        ctx.activation = activation
+        ctx.save_for_backward(x, gate, up, gate_weight, up_weight, gate_bias, up_bias)
+        ctx.mark_non_differentiable(gate, up)
+        return h, gate, up
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh, _gate, _up):
+        return (*_run(_native.gated_backward, dh, dh, *ctx.saved_tensors, ctx.activation, *ctx.needs_input_grad[:5]), None)
+
+
+def gated_linear(x, gate_weight, up_weight, gate_bias=None, up_bias=None, activation="silu", *, saved=False):
+    """f(x @ gate_weight.T + gate_bias) * (x @ up_weight.T + up_bias): both products, the activation f ("silu", "gelu", "relu" or
+    "sigmoid") and their product in one pass.  The weights are [hidden, width], of the type of x; the biases are float32 or of
+    that type.  With `saved` returns (result, gate product, up product), each rounded once, as the gradient needs them."""
+    activation = _ACTIVATIONS.get(activation, -1)
+    if _wants_gradient(x, gate_weight, up_weight, gate_bias, up_bias):
+        out = _GatedLinear.apply(x, gate_weight, up_weight, gate_bias, up_bias, activation)
+    else:
+        out = _run(_native.gated, x, x, gate_weight, up_weight, gate_bias, up_bias, activation, saved)
+    return out if saved else out[0]
+
+
+def gated_linear_backward(dh, x, gate, up, gate_weight, up_weight, gate_bias=None, up_bias=None, activation="silu"):
+    """(dx, dgate_weight, dup_weight, dgate_bias, dup_bias) of gated_linear, given the gradient of its result, what it was called with,
+    and the products that it returned.  Each has the type of what it is the gradient of (None where that is); what the biases
+    hold is not read."""
+    return _run(_native.gated_backward, dh, dh, x, gate, up, gate_weight, up_weight, gate_bias, up_bias, _ACTIVATIONS.get(activation, -1),
+                True, True, True, True, True)
+
+
+# ---- cross entropy over many items ------------------------------------------------------------------------------------
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, target, bias, ignore_index):
+        loss, lse = _run(_native.items, x, x, weight, target, bias, ignore_index, True)
+        ctx.ignore_index = ignore_index
+        ctx.save_for_backward(x, weight, target, lse, bias)
+        ctx.mark_non_differentiable(lse)
+        return loss, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss, _lse):
+        x, weight, target, lse, bias = ctx.saved_tensors
+        dx, dweight, dbias = _run(_native.items_backward, dloss, dloss, x, weight, target, lse, bias, ctx.ignore_index,
+                                  *(ctx.needs_input_grad[i] for i in (0, 1, 3)))
+        return dx, dweight, None, dbias, None
+
+
+def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index=-100, stats=False):
+    """The softmax cross entropy of x @ weight.T + bias with the items that `target` names, float32, one for each row, without a matrix of
+    logits in memory.  weight is [items, width], of the type of x; bias is float32 or of that type; target is int64, of
+    the shape of the result.  Rows whose target is `ignore_index` take no part, whatever x holds there: their loss is 0.  A
+    target that is neither that nor an item gives NaN.  With `stats` returns (loss, log of the sum of exponentials)."""
+    if _wants_gradient(x, weight, bias):
+        out = _LinearCrossEntropy.apply(x, weight, target, bias, ignore_index)
+    else:
+        out = _run(_native.items, x, x, weight, target, bias, ignore_index, stats)
+    return out if stats else out[0]
+
+
+def linear_cross_entropy_backward(dloss, x, weight, target, lse, bias=None, *, ignore_index=-100):
+    """(dx, dweight, dbias) of linear_cross_entropy, given the gradient of its result (float32, one for each row), what it was called
+    with, and the log of the sum of exponentials that it returned.  Each has the type of what it is the gradient of."""
+    return _run(_native.items_backward, dloss, dloss, x, weight, target, lse, bias, ignore_index, True, True, True)
+
+
+# ---- many gradients ---------------------------------------------------------------------------------------------------
+def gradient_norm(gradients):
+    """The 2-norm of all the gradients together: a float32 on the GPU.  Squares and their sums are held in 64 bits.  Not differentiable."""
+    gradients = list(gradients)
+    if _wants_gradient(*gradients):
+        raise RuntimeError("hetuctr_amd.nn: the norm of gradients is not differentiable: call this under torch.no_grad()")
+    return _run(_native.gradient_norm, gradients[0] if gradients else None, gradients)
+
+
+def clip_gradients(gradients, max_norm, *, norm=None, into=None):
+    """Multiplies every gradient by min(1, max_norm / norm), in place or `into` tensors of the same types and shapes, and returns the norm: that
+    of gradient_norm, or the one that is given (a float32 on the GPU: where several GPUs hold a part of the gradients
+    each).  No result may lie where another gradient or result does; each holds its values one behind the other.  Where the norm is
+    not finite, what is multiplied is not either, or zero."""
+    gradients = list(gradients)
+    into = gradients if into is None else list(into)
+    out = _run(_native.clip_gradients, gradients[0] if gradients else None, gradients, into, max_norm, norm, torch.is_grad_enabled())
+    return out if norm is None else norm
+
+
 # ---- the same as torch operators ----------------------------------------------------------------------------------------
 # torch.jit.trace, make_fx, fake tensors and dispatch modes see what goes through torch's dispatcher: of a call into the extension only
 # that memory was allocated, which a recorded program would then return unfilled.  While one of them is at work, a call
@@ -197,6 +299,8 @@ _library = torch.library.Library("hetuctr_amd", "DEF")
 def _as_operator(f, x, args):
     if x.device.type != "cuda":
         raise RuntimeError("hetuctr_amd.nn: the tensors must be on the GPU")
+    if f in _PLAIN_NAME_OF:
+        return _as_plain_operator(f, args)
     name = _NAME_OF[f]
     at = _DROP_AT[name]
     p, seed, step, step_tensor = args[at] or (0.0, 0, 0, None)
@@ -274,3 +378,81 @@ for _name, _schema in _SCHEMAS.items():
     torch.library.register_fake("hetuctr_amd::" + _name, functools.partial(_shapes, _name), lib=_library)
     if _name != "norm_backward":
         _library.impl(_name, functools.partial(_differentiable, _name), "Autograd")
+
+
+# Those without a Drop take the extension's arguments as they are, and return what there is of its results; `_there` says which of them
+# that is.
+_PLAIN_SCHEMAS = {
+    "gated_linear": "(Tensor x, Tensor gate_weight, Tensor up_weight, Tensor? gate_bias, Tensor? up_bias, int activation, bool saved) "
+                    "-> Tensor[]",
+    "gated_linear_backward": "(Tensor dh, Tensor x, Tensor gate, Tensor up, Tensor gate_weight, Tensor up_weight, Tensor? gate_bias, "
+                             "Tensor? up_bias, int activation, bool need_x, bool need_gate_weight, bool need_up_weight, "
+                             "bool need_gate_bias, bool need_up_bias) -> Tensor[]",
+    "linear_cross_entropy": "(Tensor x, Tensor weight, Tensor target, Tensor? bias, int ignore_index, bool stats) -> Tensor[]",
+    "linear_cross_entropy_backward": "(Tensor dloss, Tensor x, Tensor weight, Tensor target, Tensor lse, Tensor? bias, int ignore_index, "
+                                     "bool need_x, bool need_weight, bool need_bias) -> Tensor[]",
+    "gradient_norm": "(Tensor[] gradients) -> Tensor",
+    "clip_gradients": "(Tensor[] gradients, Tensor(a!)[] into, float max_norm, Tensor? norm, bool leaves) -> Tensor",
+}
+_PLAIN = {"gated_linear": _native.gated, "gated_linear_backward": _native.gated_backward, "linear_cross_entropy": _native.items,
+          "linear_cross_entropy_backward": _native.items_backward, "gradient_norm": _native.gradient_norm,
+          "clip_gradients": _native.clip_gradients}
+_PLAIN_NAME_OF = {f: name for name, f in _PLAIN.items()}
+_LISTS = ("gradient_norm", "clip_gradients")
+
+
+def _there(name, args):
+    if name == "gated_linear":
+        return [True, args[6], args[6]]
+    if name == "gated_linear_backward":
+        return [*args[9:12], args[6] is not None and args[12], args[7] is not None and args[13]]
+    if name == "linear_cross_entropy":
+        return [True, args[5]]
+    return [args[7], args[8], args[5] is not None and args[9]]
+
+
+def _as_plain_operator(f, args):
+    name = _PLAIN_NAME_OF[f]
+    out = getattr(torch.ops.hetuctr_amd, name)(*args)
+    if name in _LISTS:
+        return out
+    out = iter(out)
+    return tuple(next(out) if there else None for there in _there(name, args))
+
+
+def _plain_compute(name, *args):
+    first = args[0][0] if name in _LISTS else args[0]
+    with torch.cuda.device(first.device):
+        out = _PLAIN[name](*args, torch.cuda.current_stream().cuda_stream)
+    if name in _LISTS:
+        return out if name == "gradient_norm" or args[3] is None else out.clone()      # an operator's result is a tensor of its own
+    return [t for t in out if t is not None]
+
+
+def _plain_shapes(name, *args):
+    if name in _LISTS:
+        return args[0][0].new_empty((), dtype=torch.float32)
+    if name == "gated_linear":
+        x, gate_weight = args[:2]
+        return [x.new_empty((*x.shape[:-1], gate_weight.shape[0])) for there in _there(name, args) if there]
+    if name == "linear_cross_entropy":
+        return [args[0].new_empty(args[0].shape[:-1], dtype=torch.float32) for there in _there(name, args) if there]
+    of = (args[1], *args[4:8]) if name == "gated_linear_backward" else (args[1], args[2], args[5])
+    return [t.new_empty(t.shape) for t, there in zip(of, _there(name, args)) if there]
+
+
+def _plain_differentiable(name, *args):
+    tensors = [t for t in args if isinstance(t, torch.Tensor)]
+    if not _wants_gradient(*tensors) and not any(forward_ad.unpack_dual(t, level=0).tangent is not None for t in tensors):
+        with torch._C._AutoDispatchBelowAutograd():
+            return getattr(torch.ops.hetuctr_amd, name)(*args)
+    out = (_GatedLinear if name == "gated_linear" else _LinearCrossEntropy).apply(*args[:-1])
+    return list(out if args[-1] else out[:1])
+
+
+for _name, _schema in _PLAIN_SCHEMAS.items():
+    _library.define(_name + _schema)
+    _library.impl(_name, functools.partial(_plain_compute, _name), "CUDA")
+    torch.library.register_fake("hetuctr_amd::" + _name, functools.partial(_plain_shapes, _name), lib=_library)
+    if _name in ("gated_linear", "linear_cross_entropy"):
+        _library.impl(_name, functools.partial(_plain_differentiable, _name), "Autograd")

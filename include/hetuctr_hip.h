@@ -312,6 +312,113 @@ int hctr_layer_norm_backward(const hctr_norm_grad_args *a);
 int hctr_dropout_add_layer_norm_backward(const hctr_norm_grad_args *a);
 size_t hctr_layer_norm_workspace(size_t rows, size_t width);
 
+/* ---- the heavy operators of a training step around the table ---------------------------------------------------------------
+ * As above: work goes to `stream`, nothing is allocated, waited for or kept, results are the same bits every time; workspaces
+ * are device memory, 16-byte aligned, in use until the work is done, and of as many bytes as the function beside each
+ * call says for the same arguments (whose stream and workspace it does not read; pointers it looks at, but does not follow;
+ * (size_t)-1 where the call would refuse them for their sizes or types).
+ * Products run on the matrix cores: 16-bit values are multiplied exactly, float values as floats; sums are held in 32 bits.
+ * Matrices of weights are [columns of the result] x [columns of x], as rows.  rows and items < 2^31 - 65536; width, hidden <= 2^20.
+ *
+ * hctr_gated_linear:  gate = x gate_weight^T + gate_bias,  up = x up_weight^T + up_bias,  h = f(gate) * up
+ * rows x width times width x hidden, twice; all matrices are of type `dtype`, the biases (`hidden` elements each, NULL: none)
+ * of bias_dtype: HCTR_F32 or dtype.  f: v * sigmoid(v), v * Phi(v) (Phi: the normal distribution's integral), max(v, 0), sigmoid(v).
+ * h comes from the products before they are rounded.  gate and up (rows x hidden; data NULL: not wanted) are for the gradient. */
+enum { HCTR_SILU = 0, HCTR_GELU = 1, HCTR_RELU = 2, HCTR_SIGMOID = 3 };
+typedef struct hctr_gated_args {
+  size_t rows, width, hidden;
+  hctr_matrix x, gate_weight, up_weight, h, gate, up;
+  const void *gate_bias, *up_bias;
+  void *workspace;
+  size_t workspace_bytes;
+  void *stream;
+  int dtype, bias_dtype, activation;
+} hctr_gated_args;
+int hctr_gated_linear(const hctr_gated_args *a);
+size_t hctr_gated_linear_workspace(const hctr_gated_args *a);
+
+/* Its gradient, given that of h and the products gate and up that the forward pass left:
+ *     dgate = dh * up * f'(gate),  dup = dh * f(gate)
+ *     dx = dgate gate_weight + dup up_weight,  dgate_weight = dgate^T x,  dup_weight = dup^T x,  dgate_bias, dup_bias: their sums over the rows
+ * dgate and dup are rounded to dtype before the products, not for the biases.  f' of max(v, 0) is 0 at 0.  Any result may be missing (data
+ * NULL); gate_weight and up_weight are read for dx alone, x for the weights' gradients alone. */
+typedef struct hctr_gated_grad_args {
+  size_t rows, width, hidden;
+  hctr_matrix dh, x, gate, up, gate_weight, up_weight, dx, dgate_weight, dup_weight;
+  void *dgate_bias, *dup_bias;
+  void *workspace;
+  size_t workspace_bytes;
+  void *stream;
+  int dtype, bias_dtype, activation;
+} hctr_gated_grad_args;
+int hctr_gated_linear_backward(const hctr_gated_grad_args *a);
+size_t hctr_gated_linear_backward_workspace(const hctr_gated_grad_args *a);
+
+/* Softmax cross entropy over `items`: with l = x weight^T + bias, rows x items, which is never stored,
+ *     lse[r] = log(sum over the items of exp(l[r])),   loss[r] = lse[r] - l[r][target[r]]
+ * A row whose target is ignore_index takes no part, whatever x holds there: its loss and lse are 0.  One whose target is neither that nor
+ * an item gets NaN for both.  x and weight are of `dtype`, bias (`items` elements, NULL: none) is HCTR_F32 or dtype.  An
+ * item whose bias is -infinity does not count; if none is left, lse is -infinity and loss NaN.  lse may be NULL. */
+typedef struct hctr_items_args {
+  size_t rows, width, items;
+  hctr_matrix x, weight;
+  const void *bias;
+  const int64_t *target;
+  int64_t ignore_index;
+  float *loss, *lse;
+  void *workspace;
+  size_t workspace_bytes;
+  void *stream;
+  int dtype, bias_dtype;
+} hctr_items_args;
+int hctr_linear_cross_entropy(const hctr_items_args *a);
+size_t hctr_linear_cross_entropy_workspace(const hctr_items_args *a);
+
+/* Its gradient, given that of loss and the lse that the forward pass left:
+ *     d = (exp(l - lse) - [item is the target]) * dloss,   dx = d weight,  dweight = d^T x,  dbias: the sums of d over the rows
+ * in pieces of the items, of which d is held, rounded to dtype (for HCTR_F16 after a power of two that the largest dloss gives, which the
+ * results are divided by).  Ignored rows have zeros in dx and no part in the others.  Any result may be missing (data NULL). */
+typedef struct hctr_items_grad_args {
+  size_t rows, width, items;
+  hctr_matrix x, weight, dx, dweight;
+  const void *bias;
+  void *dbias;
+  const int64_t *target;
+  int64_t ignore_index;
+  const float *dloss, *lse;
+  void *workspace;
+  size_t workspace_bytes;
+  void *stream;
+  int dtype, bias_dtype;
+} hctr_items_grad_args;
+int hctr_linear_cross_entropy_backward(const hctr_items_grad_args *a);
+size_t hctr_linear_cross_entropy_backward_workspace(const hctr_items_grad_args *a);
+
+/* norm = the 2-norm of all `count` gradients together (squares and their sums in 64 bits), a float in device memory.
+ * hctr_clip_gradients also writes each gradient times min(1, max_norm / norm) to its `into`, which may be the gradient's own place (where
+ * nothing is written if nothing changes) but may not overlap any other; if `given` is not NULL, the norm is taken from there (device memory; as
+ * when several GPUs hold a part each), and norm may be NULL.  A norm that is not finite makes every result so or zero, as the product says.
+ * values: elements, one behind the other; into: of the same type.  The array of hctr_gradient is host memory, read before the call returns. */
+typedef struct hctr_gradient {
+  const void *values;
+  void *into;
+  size_t count;
+  int dtype;
+} hctr_gradient;
+typedef struct hctr_clip_args {
+  const hctr_gradient *gradients;
+  size_t count;
+  float *norm;
+  const float *given;
+  float max_norm;
+  void *workspace;
+  size_t workspace_bytes;
+  void *stream;
+} hctr_clip_args;
+int hctr_gradient_norm(const hctr_clip_args *a);
+int hctr_clip_gradients(const hctr_clip_args *a);
+size_t hctr_gradient_workspace(const hctr_clip_args *a);
+
 /* Version string of the library. */
 const char *hctr_version(void);
 
