@@ -15,7 +15,6 @@ struct GatedForward {
   int activation;
   void *h, *gate, *up; // gate, up: may be null
   int64_t h_stride, gate_stride, up_stride;
-  bool vectors;
 };
 template <typename T> void launch_gated(GatedForward &p, int tile, hipStream_t s);
 template <typename T> void launch_gated_few(const GatedForward &p, hipStream_t s);

@@ -11,10 +11,6 @@ namespace {
 
 Operand operand(const Layout &l, size_t rows) { return {{l.at, nullptr}, l.stride, (uint32_t)rows, 0, 0}; }
 
-bool vectors(const hctr_matrix &m, size_t rows, size_t columns, size_t size) {
-  return !m.data || ((uintptr_t)m.data % (4 * size) == 0 && columns % 4 == 0 && (rows <= 1 || m.stride % 4 == 0));
-}
-
 struct ForwardPlan {
   bool few;
   Shape shape;
@@ -55,7 +51,6 @@ template <typename T> void forward(const hctr_gated_args &a) {
   p.activation = a.activation;
   p.h = a.h.data, p.gate = a.gate.data, p.up = a.up.data;
   p.h_stride = a.h.stride, p.gate_stride = a.gate.stride, p.up_stride = a.up.stride;
-  p.vectors = vectors(a.h, a.rows, a.hidden, size) && vectors(a.gate, a.rows, a.hidden, size) && vectors(a.up, a.rows, a.hidden, size);
   if (plan.few) {
     p.loose_x = a.x.data, p.loose_gate = a.gate_weight.data, p.loose_up = a.up_weight.data;
     p.loose_stride = a.x.stride, p.loose_gate_stride = a.gate_weight.stride, p.loose_up_stride = a.up_weight.stride;
@@ -156,7 +151,7 @@ template <typename T> void backward(const hctr_gated_grad_args &a) {
     q.rows = (uint32_t)a.rows, q.columns = (uint32_t)a.width, q.k = (uint32_t)(2 * padded);
     q.splits = plan.dx.splits, q.band = 8;
     q.partial = q.splits > 1 ? (float *)parts : nullptr;
-    q.result = {{a.dx.data, nullptr}, {a.dx.stride, 0}, q.rows, q.columns, ~0u, vectors(a.dx, a.rows, a.width, size), nullptr, nullptr};
+    q.result = {{a.dx.data, nullptr}, {a.dx.stride, 0}, q.rows, q.columns, ~0u, nullptr, nullptr};
     launch_forward_product<T>(q, plan.dx.tile, s);
     if (q.partial) launch_join<T>(q, s);
   }
@@ -171,8 +166,8 @@ template <typename T> void backward(const hctr_gated_grad_args &a) {
     q.splits = plan.dweight.splits, q.band = 8;
     q.partial = q.splits > 1 ? (float *)parts : nullptr;
     const hctr_matrix &first = gate ? a.dgate_weight : a.dup_weight, &second = a.dup_weight;
-    q.result = {{first.data, both ? second.data : nullptr}, {first.stride, second.stride}, (uint32_t)a.hidden, q.columns, (uint32_t)padded,
-                vectors(first, a.hidden, a.width, size) && vectors(second, a.hidden, a.width, size), nullptr, nullptr};
+    q.result = {{first.data, both ? second.data : nullptr}, {first.stride, second.stride}, (uint32_t)a.hidden, q.columns, (uint32_t)padded, nullptr,
+                nullptr};
     launch_across_product<T>(q, plan.dweight.tile, s);
     if (q.partial) launch_join<T>(q, s);
   }

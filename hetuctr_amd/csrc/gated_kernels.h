@@ -37,8 +37,8 @@ __device__ __forceinline__ Slope slope_of(int f, float v) {
   return {g.s, g.s * g.rest};
 }
 
-// four neighbouring columns of the result
-template <typename T> __device__ __forceinline__ void finish_gated(const GatedForward &p, uint32_t row, uint32_t column, f32x4 gate, f32x4 up) {
+// four neighbouring columns of both products, which get their biases, and of the result
+template <typename T> __device__ __forceinline__ f32x4 gated4(const GatedForward &p, uint32_t column, f32x4 &gate, f32x4 &up) {
   f32x4 h;
 #pragma unroll
   for (int e = 0; e < 4; e++) {
@@ -46,9 +46,13 @@ template <typename T> __device__ __forceinline__ void finish_gated(const GatedFo
     up[e] += bias_at<T>(p.up_bias, p.narrow, column + e, p.hidden);
     h[e] = activated(p.activation, gate[e]) * up[e];
   }
-  write4<T>((T *)p.h + (int64_t)row * p.h_stride, column, p.hidden, p.vectors, h);
-  if (p.gate) write4<T>((T *)p.gate + (int64_t)row * p.gate_stride, column, p.hidden, p.vectors, gate);
-  if (p.up) write4<T>((T *)p.up + (int64_t)row * p.up_stride, column, p.hidden, p.vectors, up);
+  return h;
+}
+template <typename T> __device__ __forceinline__ void finish_gated(const GatedForward &p, uint32_t row, uint32_t column, f32x4 gate, f32x4 up) {
+  const f32x4 h = gated4<T>(p, column, gate, up);
+  write4<T>((T *)p.h + (int64_t)row * p.h_stride, column, p.hidden, h);
+  if (p.gate) write4<T>((T *)p.gate + (int64_t)row * p.gate_stride, column, p.hidden, gate);
+  if (p.up) write4<T>((T *)p.up + (int64_t)row * p.up_stride, column, p.hidden, up);
 }
 
 // Both products in one: the rows of the two matrices of weights alternate in a tile, 32 by 32, so that a wave holds the same columns of
@@ -64,6 +68,40 @@ void gated_product(GatedForward p) {
   typename P::Sums sum;
   P::run(p.x, p.weights, row * TILE, column * TILE, k0, k1, (uint32_t)(uintptr_t)(lds_char *)tiles, sum);
   const uint32_t l = lane_id(), half = (p.hidden + 3) / 4 * 4;
+  if constexpr (sizeof(T) == 2) {
+    if (!p.partial) {
+      typedef Staged<T, TILE, TILE / 2> S;
+      const uint32_t lds = (uint32_t)(uintptr_t)(lds_char *)tiles;
+      const auto out = [&](uint32_t from, void *to, int64_t stride) {
+        S::template each<P::kThreads>(from, [&](uint32_t r, uint32_t c, auto x) {
+          r += row * TILE, c += column * (TILE / 2);
+          if (r < p.rows && c < p.hidden) write<8>((T *)to + (int64_t)r * stride, c, p.hidden, x);
+        });
+      };
+      __syncthreads(); // the tiles are read
+#pragma unroll
+      for (int i = 0; i < P::kRowTiles; i++)
+#pragma unroll
+        for (int j = 0; j < P::kColumnTiles / 2; j++) {
+          const uint32_t r = P::wave_row() + i * 16 + l % 16, c = P::wave_column() / 2 + j * 16 + l / 16 * 4;
+          S::put(lds, r, c, gated4<T>(p, column * (TILE / 2) + c, sum[i][j], sum[i][j + P::kColumnTiles / 2]));
+          if (p.gate) S::put(lds + S::kBytes, r, c, sum[i][j]);
+        }
+      __syncthreads();
+      out(lds, p.h, p.h_stride);
+      if (p.gate) out(lds + S::kBytes, p.gate, p.gate_stride);
+      if (!p.up) return;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < P::kRowTiles; i++)
+#pragma unroll
+        for (int j = 0; j < P::kColumnTiles / 2; j++)
+          S::put(lds, P::wave_row() + i * 16 + l % 16, P::wave_column() / 2 + j * 16 + l / 16 * 4, sum[i][j + P::kColumnTiles / 2]);
+      __syncthreads();
+      out(lds, p.up, p.up_stride);
+      return;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < P::kRowTiles; i++) {
     const uint32_t r = row * TILE + P::wave_row() + i * 16 + l % 16;

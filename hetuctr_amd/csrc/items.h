@@ -7,7 +7,7 @@ namespace hctr {
 // What is known of the rows that take part, which are numbered anew, in their order; all in device memory
 struct Taken {
   uint32_t *count;
-  float *scale;      // [2]: what d is multiplied by before it is rounded, and 1 / that
+  float *scale;      // [2]: what d is multiplied by before it is rounded to 16 bits, and 1 / that
   uint32_t *row_of;  // [rows] where each one lies among all rows
   uint32_t *target;  // its item; kNoItem: that is none
   float *dloss, *lse; // of the gradient

@@ -58,10 +58,6 @@ __global__ __launch_bounds__(kJoinRows *kJoinGroups) void join_tails(const float
   if (lse) lse[to] = item ? log_sum + t.most : nan;
 }
 
-bool aligned(const hctr_matrix &m, size_t rows, size_t columns, size_t size) {
-  return (uintptr_t)m.data % (4 * size) == 0 && columns % 4 == 0 && (rows <= 1 || m.stride % 4 == 0);
-}
-
 struct RowsSpace { // of the rows that take part, in the workspace
   size_t taken, chunks, x, bytes;
 };
@@ -187,7 +183,7 @@ template <typename T> void backward(const hctr_items_grad_args &a) {
     t = take<T>(a.x, a.target, a.ignore_index, a.rows, a.width, a.items, a.dloss, space, s);
     t.dloss = a.dloss, t.lse_in = a.lse;
     t.dx = a.dx.data, t.dx_stride = a.dx.stride;
-    t.scaled = std::is_same_v<T, f16_t>;
+    t.scaled = !std::is_same_v<T, float>;
     launch_take_rows<T>(t, s);
   }
   char *d = space, *acc = d + plan.d, *parts = acc + plan.acc, *sums = parts + plan.parts, *rest = sums + plan.sums;
@@ -231,7 +227,7 @@ template <typename T> void backward(const hctr_items_grad_args &a) {
       q.splits = plan.dx.splits, q.band = 8;
       q.partial = plan.acc ? (float *)acc : nullptr;
       q.add = i > 0;
-      q.result = {{a.dx.data, nullptr}, {a.dx.stride, 0}, q.rows, q.columns, ~0u, aligned(a.dx, a.rows, a.width, size), back, t.taken.row_of};
+      q.result = {{a.dx.data, nullptr}, {a.dx.stride, 0}, q.rows, q.columns, ~0u, back, t.taken.row_of};
       launch_forward_product<T>(q, plan.dx.tile, s);
     }
     if (a.dweight.data) {
@@ -243,7 +239,7 @@ template <typename T> void backward(const hctr_items_grad_args &a) {
       v.k_there = count;
       v.splits = plan.dweight.splits, v.band = 8;
       v.partial = plan.parts ? (float *)parts : nullptr;
-      v.result = {{dweight.data, nullptr}, {dweight.stride, 0}, v.rows, v.columns, ~0u, aligned(dweight, some, a.width, size), back, nullptr};
+      v.result = {{dweight.data, nullptr}, {dweight.stride, 0}, v.rows, v.columns, ~0u, back, nullptr};
       launch_across_product<T>(v, plan.dweight.tile, s);
       if (v.partial) launch_join<T>(v, s);
     }

@@ -84,19 +84,30 @@ __global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kNo
   } else {
     const float scale = p.taken.scale[0];
     f32x4 down[P::kColumnTiles] = {};
+    typedef std::conditional_t<sizeof(T) == 2, T, bf16_t> Narrow; // (floats are not staged)
+    typedef Staged<Narrow, TILE, TILE> S;
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_char *)tiles;
 #pragma unroll
     for (int i = 0; i < P::kRowTiles; i++) {
-      const uint32_t r = row0 + P::wave_row() + i * 16 + l % 16;
-      if (r >= rows) continue;
-      const float lse = p.taken.lse[r], dloss = p.taken.dloss[r] * scale;
-      const uint32_t target = p.taken.target[r] - p.first;
+      const uint32_t in = P::wave_row() + i * 16 + l % 16, r = row0 + in;
+      const bool there = r < rows;
+      const float lse = there ? p.taken.lse[r] : 0.f, dloss = there ? p.taken.dloss[r] * scale : 0.f;
+      const uint32_t target = there ? p.taken.target[r] - p.first : kNoItem;
 #pragma unroll
       for (int j = 0; j < P::kColumnTiles; j++) {
-        const uint32_t c = column0 + wave_column + j * 16 + l / 16 * 4;
-        const f32x4 d = slope4(sum[i][j] + bias[j], lse, dloss, target - c);
-        down[j] += d;
-        if (c < p.d_stride) write4<T>((T *)p.d + (uint64_t)r * p.d_stride, c, p.d_stride, true, d);
+        const uint32_t c = wave_column + j * 16 + l / 16 * 4;
+        const f32x4 d = slope4(sum[i][j] + bias[j], lse, dloss, target - (column0 + c));
+        if (there) down[j] += d;
+        if constexpr (sizeof(T) == 2) S::put(lds, in, c, d);
+        else if (there && column0 + c < p.d_stride) write4<T>((T *)p.d + (uint64_t)r * p.d_stride, column0 + c, p.d_stride, d);
       }
+    }
+    if constexpr (sizeof(T) == 2) {
+      __syncthreads();
+      S::template each<P::kThreads>(lds, [&](uint32_t r, uint32_t c, auto x) {
+        if (row0 + r < rows && column0 + c < p.d_stride) *(typename Packed<T, 8>::type *)((T *)p.d + (uint64_t)(row0 + r) * p.d_stride + column0 + c) = x;
+      });
+      if (p.sums) __syncthreads(); // the staged tile is read
     }
     if (p.sums) {
       f32x4 *joined = (f32x4 *)tiles; // [2][TILE / 4]
@@ -138,7 +149,7 @@ template <typename T, int ROWS, bool GRADIENT> __global__ __launch_bounds__((Few
       if (c == 0) p.parts[(uint64_t)blockIdx.x * p.rows + r] = make_float2(tail.most, tail.sum);
     } else {
       d = slope4(logit[0], p.taken.lse[r], p.taken.dloss[r] * p.taken.scale[0], p.taken.target[r] - p.first - (column0 + c));
-      if (column0 + c < p.d_stride) write4<T>((T *)p.d + (uint64_t)r * p.d_stride, column0 + c, p.d_stride, true, d);
+      if (column0 + c < p.d_stride) write4<T>((T *)p.d + (uint64_t)r * p.d_stride, column0 + c, p.d_stride, d);
     }
   }
   if (GRADIENT && p.sums) {
@@ -172,12 +183,12 @@ template <typename T, bool GRADIENT> void launch_items(ItemsProduct &p, int tile
 template <typename T> void launch_items_forward(ItemsProduct &p, int tile, hipStream_t s) { launch_items<T, false>(p, tile, s); }
 template <typename T> void launch_items_gradient(ItemsProduct &p, int tile, hipStream_t s) { launch_items<T, true>(p, tile, s); }
 
-// The power of two that brings the largest |dloss| to 2^13 .. 2^14, where a value of half precision is rounded to 11 bits down to 2^-27 of it
-__device__ __forceinline__ float scale_for(uint32_t most) {
-  if (!most) return 1.f;
-  const int exponent = max(-100, (int)(most >> 23) - 126); // most < 2^exponent
-  return ldexpf(1.f, 14 - exponent);
-}
+// What brings the largest |dloss| to 2^13, where values of half precision are rounded to 11 bits down to 2^-27 of it.  That largest one
+// becomes a power of two: where all rows have the same, as those of a mean do, the target's slope, p - 1 times it, is rounded with a
+// p that is small and not with dloss, whose rounding would be the same in every row and add up (8192 rows of 1/6144 in bfloat16: dx and
+// dweight are 0.0033 of their size off instead of 0.0017, of which 0.0017 are their own rounding).
+constexpr float kScaled = 8192.f;
+__device__ __forceinline__ float largest_of(uint32_t bits) { return bits ? fmaxf(__builtin_bit_cast(float, bits), 0x1p-100f) : kScaled; }
 
 // Eight rows a block (a wave copies one at a time): it finds how many of those before them take part from the chunks' counts and its own
 // chunk's targets.
@@ -218,8 +229,8 @@ template <typename T> __global__ __launch_bounds__(256) void take_rows(TakeRows 
     __syncthreads();
     if (t == 0) {
       *p.taken.count = total;
-      const float scale = p.scaled ? scale_for(max(max(largest[0], largest[1]), max(largest[2], largest[3]))) : 1.f;
-      p.taken.scale[0] = scale, p.taken.scale[1] = 1.f / scale;
+      const float one = p.scaled ? largest_of(max(max(largest[0], largest[1]), max(largest[2], largest[3]))) : kScaled;
+      p.taken.scale[0] = kScaled / one, p.taken.scale[1] = one / kScaled;
     }
   }
   if (t < kTakeRows) {

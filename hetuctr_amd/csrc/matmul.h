@@ -227,6 +227,29 @@ template <typename T, Lies LA, Lies LB, Second SB, int BM, int BN> struct Produc
   }
 };
 
+// A tile of results of 16 bits on its way out: the waves put four columns at a time into LDS, where they take 32 bytes of 16 rows each, in
+// different banks, and the block writes whole rows of it.  Straight from the registers a store is 16 pieces of 32 bytes, one a row, which
+// all go to one memory channel where rows lie a power of two apart (8192 x 32768 x 4096 in bfloat16: 2276 us, rows 128 bytes
+// further apart 1898).
+template <typename T, int ROWS, int COLUMNS> struct Staged {
+  static_assert(sizeof(T) == 2, "pieces of eight columns");
+  static constexpr uint32_t kBytes = ROWS * COLUMNS * 2, kPieces = COLUMNS / 8, kMask = COLUMNS / 16 < 16 ? COLUMNS / 16 - 1 : 15;
+  static __device__ __forceinline__ void put(uint32_t lds, uint32_t row, uint32_t column, f32x4 v) {
+    const Floats<4> f = {{v[0], v[1], v[2], v[3]}};
+    const uint32_t at = lds + row * (COLUMNS * 2) + ((column / 16 ^ (row & kMask)) * 32 | column % 16 * 2);
+    *(__attribute__((address_space(3))) typename Packed<T, 4>::type *)(uintptr_t)at = rounded<T>(f);
+  }
+  // f(row, column, its eight values) for every piece, by all threads of the block
+  template <int THREADS, typename F> static __device__ __forceinline__ void each(uint32_t lds, F &&f) {
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < ROWS * kPieces; i += THREADS) {
+      const uint32_t row = i / kPieces, piece = i % kPieces;
+      const uint32_t at = lds + row * (COLUMNS * 2) + ((piece / 2 ^ (row & kMask)) * 32 | piece % 2 * 16);
+      f(row, piece * 8, *(const __attribute__((address_space(3))) typename Packed<T, 8>::type *)(uintptr_t)at);
+    }
+  }
+};
+
 // The tile that a block works on.  Neighbouring blocks go to different XCDs: each XCD gets a stretch of neighbouring tiles, and takes them
 // in bands of `band` tiles of rows, so that those at work share lines in its L2.
 __device__ __forceinline__ void tile_of(uint32_t block, uint32_t blocks, uint32_t row_tiles, uint32_t column_tiles, uint32_t band, uint32_t &row, uint32_t &column) {

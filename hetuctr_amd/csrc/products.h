@@ -10,31 +10,31 @@ struct Result {
   void *to[2];
   int64_t stride[2]; // elements
   uint32_t rows, columns, second_from;
-  bool vectors;            // four columns can be written at once
   const float *scale;      // what every value is multiplied by, or null
   const uint32_t *row_of;  // where a row goes, or null: its own place
 };
 
-template <typename T> __device__ __forceinline__ void write4(T *to, uint32_t column, uint32_t columns, bool vectors, f32x4 v) {
-  const Floats<4> f = {{v[0], v[1], v[2], v[3]}};
-  const typename Packed<T, 4>::type x = rounded<T>(f);
-  if (vectors) {
-    *(typename Packed<T, 4>::type *)(to + column) = x;
+// columns `column` .. `column` + V - 1 of a row, or as many of them as there are
+template <int V, typename T> __device__ __forceinline__ void write(T *row, uint32_t column, uint32_t columns, typename Packed<T, V>::type x) {
+  if (column + V <= columns) {
+    *(typename Packed<T, V>::memory *)(row + column) = x;
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (column + e < columns) to[column + e] = x[e];
+    for (int e = 0; e < V - 1; e++)
+      if (column + e < columns) row[column + e] = x[e];
   }
 }
-// columns `column` .. `column` + 3 (a multiple of four, below `columns`) of a row
-template <typename T> __device__ __forceinline__ void write4(const Result &r, uint32_t row, uint32_t column, f32x4 v) {
+template <typename T> __device__ __forceinline__ void write4(T *row, uint32_t column, uint32_t columns, f32x4 v) {
+  const Floats<4> f = {{v[0], v[1], v[2], v[3]}};
+  write<4>(row, column, columns, rounded<T>(f));
+}
+// a row of a result; null: it is not wanted
+template <typename T> __device__ __forceinline__ T *row_of(const Result &r, uint32_t row) {
   if (r.row_of) row = r.row_of[row];
   const bool second = row >= r.second_from;
   row -= second ? r.second_from : 0;
   T *to = (T *)(second ? r.to[1] : r.to[0]);
-  if (!to || row >= r.rows) return;
-  if (r.scale) v *= *r.scale;
-  write4<T>(to + (int64_t)row * (second ? r.stride[1] : r.stride[0]), column, r.columns, r.vectors, v);
+  return to && row < r.rows ? to + (int64_t)row * (second ? r.stride[1] : r.stride[0]) : nullptr;
 }
 
 // A product, cut along k into `splits` parts where its tiles alone would leave the card idle: each part's sums go to `partial` as floats

@@ -18,6 +18,24 @@ __global__ __launch_bounds__((Product<T, LA, LB, SB, TILE, TILE>::kThreads), 2) 
   typename P::Sums sum;
   P::run(p.a, p.b, row0, column0, k0, k1, (uint32_t)(uintptr_t)(lds_char *)tiles, sum);
   const uint32_t l = lane_id(), columns = (p.columns + 3) / 4 * 4;
+  const float scale = !p.partial && p.result.scale ? *p.result.scale : 1.f;
+  if constexpr (sizeof(T) == 2) {
+    if (!p.partial) {
+      typedef Staged<T, TILE, TILE> S;
+      const uint32_t lds = (uint32_t)(uintptr_t)(lds_char *)tiles;
+      __syncthreads(); // the tiles are read
+#pragma unroll
+      for (int i = 0; i < P::kRowTiles; i++)
+#pragma unroll
+        for (int j = 0; j < P::kColumnTiles; j++) S::put(lds, P::wave_row() + i * 16 + l % 16, P::wave_column() + j * 16 + l / 16 * 4, sum[i][j] * scale);
+      __syncthreads();
+      S::template each<P::kThreads>(lds, [&](uint32_t r, uint32_t c, auto x) {
+        if (row0 + r >= rows || column0 + c >= p.columns) return;
+        if (T *to = row_of<T>(p.result, row0 + r)) write<8>(to, column0 + c, p.columns, x);
+      });
+      return;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < P::kRowTiles; i++) {
     const uint32_t r = row0 + P::wave_row() + i * 16 + l % 16;
@@ -28,7 +46,7 @@ __global__ __launch_bounds__((Product<T, LA, LB, SB, TILE, TILE>::kThreads), 2) 
       const uint32_t c = column0 + P::wave_column() + j * 16 + l / 16 * 4;
       if (c >= p.columns) continue;
       if (!p.partial) {
-        write4<T>(p.result, r, c, sum[i][j]);
+        if (T *to = row_of<T>(p.result, r)) write4<T>(to, c, p.columns, sum[i][j] * scale);
       } else {
         f32x4 *to = (f32x4 *)(part + c);
         *to = p.add ? *to + sum[i][j] : sum[i][j];
@@ -39,13 +57,14 @@ __global__ __launch_bounds__((Product<T, LA, LB, SB, TILE, TILE>::kThreads), 2) 
 
 template <typename T> __global__ __launch_bounds__(256) void join_parts(const float *partial, uint32_t splits, uint32_t rows, uint32_t columns, const uint32_t *rows_there, Result result) {
   const uint32_t quads = (columns + 3) / 4, there = rows_there ? min(rows, *rows_there) : rows;
+  const float scale = result.scale ? *result.scale : 1.f;
   const uint64_t total = (uint64_t)there * quads, apart = (uint64_t)rows * quads;
   for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
     const f32x4 *from = (const f32x4 *)partial + i;
     f32x4 sum = from[0];
     for (uint32_t s = 1; s < splits; s++) sum += from[s * apart];
     const uint64_t r = total >> 32 ? i / quads : (uint32_t)i / quads;
-    write4<T>(result, (uint32_t)r, (uint32_t)(i - r * quads) * 4, sum);
+    if (T *to = row_of<T>(result, (uint32_t)r)) write4<T>(to, (uint32_t)(i - r * quads) * 4, columns, sum * scale);
   }
 }
 

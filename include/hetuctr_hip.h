@@ -376,8 +376,8 @@ size_t hctr_linear_cross_entropy_workspace(const hctr_items_args *a);
 
 /* Its gradient, given that of loss and the lse that the forward pass left:
  *     d = (exp(l - lse) - [item is the target]) * dloss,   dx = d weight,  dweight = d^T x,  dbias: the sums of d over the rows
- * in pieces of the items, of which d is held, rounded to dtype (for HCTR_F16 after a power of two that the largest dloss gives, which the
- * results are divided by).  Ignored rows have zeros in dx and no part in the others.  Any result may be missing (data NULL). */
+ * in pieces of the items, of which d is held, rounded to dtype (to 16 bits after a factor that brings the largest dloss to 2^13, by which the
+ * results are divided).  Ignored rows have zeros in dx and no part in the others.  Any result may be missing (data NULL). */
 typedef struct hctr_items_grad_args {
   size_t rows, width, items;
   hctr_matrix x, weight, dx, dweight;
