@@ -17,9 +17,9 @@ OBJ = os.path.join(CSRC, "build")
 LIBDIR = os.path.join(HERE, "lib")
 HIP_SOURCES = ["radix_sort.hip", "tile_sort.hip", "preprocess.hip", "push.hip", "pull.hip", "init.hip", "table.hip", "checkpoint.hip", "loader.hip", "partition.hip", "host_copy.hip", "dropout.hip", "layer_norm_f32.hip", "layer_norm_f32_bf16.hip", "layer_norm_f32_f16.hip", "layer_norm_bf16.hip", "layer_norm_f16.hip", "layer_norm.hip",
                "products.hip", "products_f32.hip", "products_bf16.hip", "products_f16.hip", "gated.hip", "gated_f32.hip", "gated_bf16.hip", "gated_f16.hip",
-               "items.hip", "items_f32.hip", "items_bf16.hip", "items_f16.hip", "clip.hip", "c_api.hip"]
+               "items.hip", "items_f32.hip", "items_bf16.hip", "items_f16.hip", "items_narrow_bf16.hip", "items_narrow_f16.hip", "clip.hip", "c_api.hip"]
 HEADERS = ["common.h", "host_copy.h", "kernels.h", "radix_sort.h", "tile_sort.h", "run_lists.h", "row_slices.h", "launch_cut.h", "unique_tile.h", "table.h", "partition.h", "dense.h", "layer_norm.h", "layer_norm_forward.h", "layer_norm_backward.h", "philox.h", "values.h",
-           "matmul.h", "few_rows.h", "products.h", "products_kernels.h", "gated.h", "gated_kernels.h", "items.h", "items_kernels.h", "items_tail.h", "clip.h",
+           "matmul.h", "few_rows.h", "products.h", "products_kernels.h", "gated.h", "gated_kernels.h", "items.h", "items_kernels.h", "items_tail.h", "items_narrow.h", "clip.h",
            os.path.join("..", "..", "include", "hetuctr_hip.h")]
 # packed-fp32 instruction selection is switched off for all device code; no fused multiply-add contraction, so
 # that "sum * -lr" then "row + that" rounds twice like the CPU restatement it is checked against (fused

@@ -29,64 +29,40 @@ __global__ __launch_bounds__(256) void count_rows(const int64_t *target, int64_t
   if (threadIdx.x == 0) chunks[blockIdx.x] = make_uint2(counts[0] + counts[1] + counts[2] + counts[3], max(max(sizes[0], sizes[1]), max(sizes[2], sizes[3])));
 }
 
-// The tiles' parts of 8 rows joined by 128 groups of threads, each of which takes every 128th tile; then the groups', in pairs.
-constexpr uint32_t kJoinRows = 8, kJoinGroups = 128;
-__global__ __launch_bounds__(kJoinRows *kJoinGroups) void join_tails(const float2 *parts, uint32_t tiles, uint32_t rows, const float *hit, Taken taken, float *loss, float *lse) {
-  constexpr uint32_t LOADS = 4;
-  __shared__ Tail tails[kJoinGroups][kJoinRows];
-  const uint32_t there = *taken.count, x = threadIdx.x % kJoinRows, y = threadIdx.x / kJoinRows, r = blockIdx.x * kJoinRows + x;
-  if (blockIdx.x * kJoinRows >= there) return;
-  Tail t = {-kInfinity, 0.f};
-  for (uint32_t i = y; i < tiles; i += kJoinGroups * LOADS) {
-    float2 v[LOADS];
-#pragma unroll
-    for (uint32_t k = 0; k < LOADS; k++) v[k] = r < there && i + k * kJoinGroups < tiles ? parts[(uint64_t)(i + k * kJoinGroups) * rows + r] : make_float2(-kInfinity, 0.f);
-#pragma unroll
-    for (uint32_t k = 0; k < LOADS; k++) t = join(t, Tail{v[k].x, v[k].y});
-  }
-  tails[y][x] = t;
-  for (uint32_t n = kJoinGroups / 2; n; n /= 2) {
-    __syncthreads();
-    if (y < n) tails[y][x] = join(tails[y][x], tails[y + n][x]);
-  }
-  if (y || r >= there) return;
-  t = tails[0][x];
-  const float log_sum = logf(t.sum), nan = __builtin_nanf("");
-  const bool item = taken.target[r] != kNoItem;
-  const uint32_t to = taken.row_of[r];
-  loss[to] = item ? log_sum + (t.most - hit[r]) : nan;
-  if (lse) lse[to] = item ? log_sum + t.most : nan;
-}
-
-struct RowsSpace { // of the rows that take part, in the workspace
-  size_t taken, chunks, x, bytes;
+// of the workspace
+struct RowsSpace {
+  size_t each, taken, chunks, x, bias, bytes; // each: of a number for every row
 };
-RowsSpace rows_space(size_t rows, size_t width, size_t size) {
+RowsSpace rows_space(size_t rows, size_t width, size_t items, size_t size) {
   RowsSpace r;
-  r.taken = 256 + 4 * up(rows * 4, 256);
+  r.each = up(rows, kFilled) * 4;
+  r.taken = 256 + 4 * r.each;
   r.chunks = rows > kChunk ? up(div_up(rows, kChunk) * sizeof(uint2), 256) : 0;
   r.x = up(rows * up(width * size, 16), 256);
-  r.bytes = r.taken + r.chunks + r.x;
+  r.bias = up(items, kFilled) * sizeof(float);
+  r.bytes = r.taken + r.chunks + r.x + r.bias;
   return r;
 }
 
 // Rows that take part, at the workspace's beginning, which moves on
-template <typename T> TakeRows take(const hctr_matrix &x, const int64_t *target, int64_t ignored, size_t rows, size_t width, size_t items, const float *dloss, char *&space,
-                                    hipStream_t s) {
-  const RowsSpace need = rows_space(rows, width, sizeof(T));
-  const size_t each = up(rows * 4, 256);
+template <typename T, typename A> TakeRows take(const A &a, const float *dloss, char *&space, hipStream_t s) {
+  const size_t rows = a.rows, width = a.width, items = a.items;
+  const RowsSpace need = rows_space(rows, width, items, sizeof(T));
+  const size_t each = need.each;
   TakeRows t = {};
-  t.x = x.data, t.x_stride = x.stride;
-  t.target = target, t.ignored = ignored;
+  t.x = a.x.data, t.x_stride = a.x.stride;
+  t.target = a.target, t.ignored = a.ignore_index;
+  t.bias = a.bias, t.narrow = a.bias_dtype != HCTR_F32;
   t.rows = (uint32_t)rows, t.width = (uint32_t)width, t.items = (uint32_t)items;
   char *at = space + 256;
-  t.taken = {(uint32_t *)space, (float *)space + 4, (uint32_t *)at, (uint32_t *)(at + each), (float *)(at + 2 * each), (float *)(at + 3 * each)};
+  t.taken = {(uint32_t *)space, (float *)space + 4, (uint32_t *)at, (uint32_t *)(at + each), (float *)(at + 2 * each), (float *)(at + 3 * each),
+             (float *)(space + need.taken + need.chunks + need.x)};
   t.to = space + need.taken + need.chunks;
   t.to_stride = (uint32_t)(up(width * sizeof(T), 16) / sizeof(T));
   if (need.chunks) {
     uint2 *chunks = (uint2 *)(space + need.taken);
     t.chunks = chunks;
-    hipLaunchKernelGGL(count_rows, dim3(div_up(rows, kChunk)), dim3(256), 0, s, target, ignored, dloss, (uint32_t)rows, chunks);
+    hipLaunchKernelGGL(count_rows, dim3(div_up(rows, kChunk)), dim3(256), 0, s, a.target, a.ignore_index, dloss, (uint32_t)rows, chunks);
     HCTR_HIP(hipGetLastError());
   }
   space += need.bytes;
@@ -94,46 +70,71 @@ template <typename T> TakeRows take(const hctr_matrix &x, const int64_t *target,
 }
 Operand taken_rows(const TakeRows &t, size_t size) { return {{(const char *)t.to, nullptr}, (int64_t)(t.to_stride * size), t.rows, 0, 0}; }
 
+// Few rows take the weights past the LDS, narrow ones hold their rows in registers, others go by tiles.
+enum class Way { kFew, kNarrow, kTiles };
+Way way_of(size_t rows, size_t width, size_t size, bool gradient) {
+  if (!gradient && rows <= kFewRows) return Way::kFew;
+  if (size == 2 && width <= kNarrow) return Way::kNarrow;
+  return rows <= kFewRows ? Way::kFew : Way::kTiles;
+}
+
 struct ForwardPlan {
+  Way way;
   int tile;
-  size_t hit, parts, weight, bytes;
+  size_t tiles, parts, weight, bytes; // tiles: along the items
 };
 ForwardPlan plan_of(const hctr_items_args &a) {
   ForwardPlan p = {};
   if (!a.rows) return p;
   const size_t size = size_of(a.dtype);
-  p.tile = a.rows <= kFewRows ? 0 : shape_of(a.rows, a.items, a.width, (int)size, false, false).tile;
-  p.hit = up(a.rows * 4, 256);
-  p.parts = up(div_up(a.items, p.tile ? p.tile : kFewItems) * a.rows * sizeof(float2), 256);
-  p.weight = p.tile ? laid_out_bytes(a.weight, a.items, a.width, size) : 0;
-  p.bytes = rows_space(a.rows, a.width, size).bytes + p.hit + p.parts + p.weight;
+  p.way = way_of(a.rows, a.width, size, false);
+  if (p.way == Way::kTiles) p.tile = shape_of(a.rows, a.items, a.width, (int)size, false, false).tile;
+  p.tiles = p.way == Way::kNarrow ? narrow_ranges(a.rows, a.items, a.width, false) : div_up(a.items, p.tile ? p.tile : kFewItems);
+  p.parts = up(p.tiles * a.rows * sizeof(float2), 256);
+  p.weight = p.way == Way::kFew ? 0 : laid_out_bytes(a.weight, a.items, a.width, size);
+  p.bytes = rows_space(a.rows, a.width, a.items, size).bytes + p.parts + p.weight;
   return p;
+}
+
+ItemsNarrow narrow_of(const TakeRows &t, const Layout &weight) {
+  ItemsNarrow n = {};
+  n.x = (const char *)t.to, n.x_stride = t.to_stride * 2;
+  n.weight = weight.at, n.weight_stride = weight.stride;
+  n.rows = t.rows, n.width = t.width, n.items = t.items;
+  n.taken = t.taken;
+  return n;
 }
 
 template <typename T> void forward(const hctr_items_args &a) {
   const ForwardPlan plan = plan_of(a);
   const hipStream_t s = (hipStream_t)a.stream;
   char *space = (char *)a.workspace;
-  TakeRows t = take<T>(a.x, a.target, a.ignore_index, a.rows, a.width, a.items, nullptr, space, s);
+  TakeRows t = take<T>(a, nullptr, space, s);
   t.loss = a.loss, t.lse = a.lse;
   launch_take_rows<T>(t, s);
-  ItemsProduct p = {};
-  p.hit = (float *)space, space += plan.hit;
-  p.parts = (float2 *)space, space += plan.parts;
-  p.rows = t.rows, p.width = t.width, p.items = t.items, p.band = 8;
-  p.bias = a.bias, p.narrow = a.bias_dtype != HCTR_F32;
-  p.taken = t.taken;
-  p.x = taken_rows(t, sizeof(T));
-  p.few_x = t.to, p.few_stride = t.to_stride;
-  p.loose_weight = a.weight.data, p.loose_stride = a.weight.stride;
-  if (plan.tile) {
-    const Layout w = laid_out(a.weight, a.items, a.width, a.dtype, space, s);
+  float2 *parts = (float2 *)space;
+  space += plan.parts;
+  Layout w = {};
+  if (plan.way != Way::kFew) w = laid_out(a.weight, a.items, a.width, a.dtype, space, s);
+  if (plan.way == Way::kNarrow) {
+    if constexpr (sizeof(T) == 2) {
+      ItemsNarrow n = narrow_of(t, w);
+      n.ranges = (uint32_t)plan.tiles;
+      n.parts = parts;
+      launch_narrow_forward<T>(n, s);
+    }
+  } else {
+    ItemsProduct p = {};
+    p.parts = parts;
+    p.rows = t.rows, p.width = t.width, p.items = t.items, p.band = 8;
+    p.taken = t.taken;
+    p.x = taken_rows(t, sizeof(T));
+    p.few_x = t.to, p.few_stride = t.to_stride;
+    p.loose_weight = a.weight.data, p.loose_stride = a.weight.stride;
     p.weight = {{w.at, nullptr}, w.stride, p.items, 0, 0};
+    launch_items_forward<T>(p, plan.tile, s);
   }
-  launch_items_forward<T>(p, plan.tile, s);
-  hipLaunchKernelGGL(join_tails, dim3(div_up(a.rows, kJoinRows)), dim3(kJoinRows * kJoinGroups), 0, s, (const float2 *)p.parts, p.column_tiles, p.rows, (const float *)p.hit,
-                     p.taken, a.loss, a.lse);
-  HCTR_HIP(hipGetLastError());
+  launch_join_tails<T>({parts, (uint32_t)plan.tiles, t.rows, t.width, t.to, a.weight.data, t.to_stride, a.weight.stride, t.taken, a.loss, a.lse}, s);
 }
 
 // What is held of d at a time: large enough for every product to fill the card, and to make the sums that dx is joined from a small part
@@ -141,6 +142,8 @@ template <typename T> void forward(const hctr_items_args &a) {
 constexpr size_t kPieceBytes = (size_t)512 << 20;
 
 struct BackwardPlan {
+  Way way;
+  size_t dx_ranges, dweight_ranges; // of the narrow way
   size_t piece, pieces, d_stride;
   int tile;
   Shape dx, dweight;
@@ -149,13 +152,25 @@ struct BackwardPlan {
 BackwardPlan plan_of(const hctr_items_grad_args &a) {
   BackwardPlan p = {};
   const size_t size = size_of(a.dtype), rows = std::max<size_t>(a.rows, 1);
+  p.way = way_of(a.rows, a.width, size, true);
+  if (a.rows && p.way == Way::kNarrow) {
+    p.rows = rows_space(a.rows, a.width, a.items, size).bytes;
+    p.weight = laid_out_bytes(a.weight, a.items, a.width, size);
+    p.dx_ranges = narrow_ranges(a.rows, a.items, a.width, true);
+    p.dweight_ranges = narrow_ranges(a.items, a.rows, a.width, true);
+    if (a.dx.data) p.acc = up(parts_bytes(a.rows, a.width, (uint32_t)p.dx_ranges), 256);
+    if (a.dweight.data && p.dweight_ranges > 1) p.parts = up(parts_bytes(a.items, a.width, (uint32_t)p.dweight_ranges), 256);
+    if (a.dbias) p.sums = up(p.dweight_ranges * a.items * sizeof(float), 256);
+    p.bytes = p.rows + p.acc + p.parts + p.sums + p.weight;
+    return p;
+  }
   p.piece = std::min(up(a.items, 64), std::min<size_t>(kMaxStride / size, std::max<size_t>(2048, kPieceBytes / (rows * size) / 256 * 256)));
   p.pieces = (a.items + p.piece - 1) / p.piece;
   p.d_stride = p.piece;
   const size_t some = std::min(a.items, p.piece);
-  p.tile = a.rows <= kFewRows ? 0 : shape_of(a.rows, some, a.width, (int)size, false, false).tile;
+  p.tile = p.way == Way::kFew ? 0 : shape_of(a.rows, some, a.width, (int)size, false, false).tile;
   if (a.rows) {
-    p.rows = rows_space(a.rows, a.width, size).bytes;
+    p.rows = rows_space(a.rows, a.width, a.items, size).bytes;
     p.d = up(a.rows * p.d_stride * size, 256);
   }
   if (a.dx.data && a.rows) {
@@ -173,6 +188,36 @@ BackwardPlan plan_of(const hctr_items_grad_args &a) {
   return p;
 }
 
+// Narrow rows: nothing is held of d; the items' sums are made beside the weight's gradient.
+template <typename T> void backward_narrow(const hctr_items_grad_args &a, const BackwardPlan &plan, const TakeRows &t, char *space) {
+  if constexpr (sizeof(T) == 2) {
+    const hipStream_t s = (hipStream_t)a.stream;
+    char *acc = space, *parts = acc + plan.acc, *sums = parts + plan.parts, *rest = sums + plan.sums;
+    ItemsNarrow n = narrow_of(t, laid_out(a.weight, a.items, a.width, a.dtype, rest, s));
+    const auto join = [&](const ItemsNarrow &n, uint32_t rows, const uint32_t *there) {
+      ProductArgs q = {};
+      q.rows = rows, q.columns = n.width, q.splits = n.ranges, q.partial = n.partial, q.rows_there = there, q.result = n.result;
+      launch_join<T>(q, s);
+    };
+    if (a.dx.data) {
+      n.ranges = (uint32_t)plan.dx_ranges;
+      n.partial = (float *)acc;
+      n.result = {{a.dx.data, nullptr}, {a.dx.stride, 0}, t.rows, t.width, ~0u, t.taken.scale + 1, t.taken.row_of};
+      launch_narrow_dx<T>(n, s);
+      join(n, t.rows, t.taken.count);
+    }
+    if (a.dweight.data || a.dbias) {
+      n.ranges = (uint32_t)plan.dweight_ranges;
+      n.partial = plan.parts ? (float *)parts : nullptr;
+      n.sums = a.dbias ? (float *)sums : nullptr;
+      n.result = {{a.dweight.data, nullptr}, {a.dweight.stride, 0}, t.items, t.width, ~0u, t.taken.scale + 1, nullptr};
+      launch_narrow_dweight<T>(n, s);
+      if (n.partial) join(n, t.items, nullptr);
+      if (n.sums) launch_column_sums({n.sums, n.ranges, t.items, ~0u, t.items, nullptr, 1, t.taken.scale + 1, {a.dbias, nullptr}}, a.bias_dtype, s);
+    }
+  }
+}
+
 template <typename T> void backward(const hctr_items_grad_args &a) {
   const BackwardPlan plan = plan_of(a);
   const hipStream_t s = (hipStream_t)a.stream;
@@ -180,11 +225,12 @@ template <typename T> void backward(const hctr_items_grad_args &a) {
   char *space = (char *)a.workspace;
   TakeRows t = {};
   if (a.rows) {
-    t = take<T>(a.x, a.target, a.ignore_index, a.rows, a.width, a.items, a.dloss, space, s);
+    t = take<T>(a, a.dloss, space, s);
     t.dloss = a.dloss, t.lse_in = a.lse;
     t.dx = a.dx.data, t.dx_stride = a.dx.stride;
     t.scaled = !std::is_same_v<T, float>;
     launch_take_rows<T>(t, s);
+    if (plan.way == Way::kNarrow) return backward_narrow<T>(a, plan, t, space);
   }
   char *d = space, *acc = d + plan.d, *parts = acc + plan.acc, *sums = parts + plan.parts, *rest = sums + plan.sums;
   const uint32_t *count = t.taken.count;
@@ -203,8 +249,6 @@ template <typename T> void backward(const hctr_items_grad_args &a) {
         p.weight = {{w.at, nullptr}, w.stride, (uint32_t)some, 0, 0};
       }
       p.rows = t.rows, p.width = t.width, p.items = (uint32_t)some, p.first = (uint32_t)first, p.band = 8;
-      p.narrow = a.bias_dtype != HCTR_F32;
-      p.bias = a.bias ? (const char *)a.bias + first * (p.narrow ? size : 4) : nullptr;
       p.taken = t.taken;
       p.x = taken_rows(t, size);
       p.few_x = t.to, p.few_stride = t.to_stride;
@@ -253,6 +297,12 @@ template <typename A> void check(const A &a) {
 }
 
 } // namespace
+
+// As many blocks as the card holds at a time, two a CU, of eight tiles of 64 rows at least.
+uint32_t narrow_ranges(size_t owned, size_t through, size_t width, bool gradient) {
+  const size_t owners = (owned + 255) / (gradient && width > 64 ? 192 : 256), tiles = (through + 63) / 64;
+  return (uint32_t)std::max<size_t>(1, std::min(512 / std::max<size_t>(1, owners), tiles / 8));
+}
 
 size_t linear_cross_entropy_workspace(const hctr_items_args &a) {
   check(a);

@@ -6,36 +6,34 @@
 
 namespace hctr {
 
-// logits of N neighbouring items, those behind the last one left out
+// logits of N times four items
 template <int N> __device__ __forceinline__ Tail tail_of(const f32x4 (&v)[N]) {
-  float most = -kInfinity;
+  float most = kLowest;
 #pragma unroll
   for (int j = 0; j < N; j++)
 #pragma unroll
-    for (int e = 0; e < 4; e++) most = fmaxf(most, v[j][e]);
+    for (int e = 0; e < 4; e += 2) most = fmaxf(fmaxf(most, v[j][e]), v[j][e + 1]);
   Tail t = {most, 0.f};
-  // (a NaN is not the largest, but makes the sum one; with no finite largest value every term is one or zero)
-  const float less = most == -kInfinity ? 0.f : most;
 #pragma unroll
   for (int j = 0; j < N; j++)
 #pragma unroll
-    for (int e = 0; e < 4; e++) t.sum += exp_less(v[j][e], less);
-  if (t.sum != t.sum) t.most = t.sum;
-  return t;
+    for (int e = 0; e < 4; e++) t.sum += __builtin_amdgcn_exp2f(v[j][e] - most);
+  return t; // (a NaN is not the largest, but makes the sum one)
 }
 
-template <typename T> __device__ __forceinline__ f32x4 bias4(const ItemsProduct &p, uint32_t c) {
-  f32x4 b;
+__device__ __forceinline__ f32x4 bias4(const ItemsProduct &p, uint32_t c) { return *(const f32x4 *)(p.taken.bias + p.first + c); }
+__device__ __forceinline__ f32x4 logit4(f32x4 sum, f32x4 bias) {
 #pragma unroll
-  for (int e = 0; e < 4; e++) b[e] = c + e < p.items ? bias_at<T>(p.bias, p.narrow, c + e, p.items) : -kInfinity;
-  return b;
+  for (int e = 0; e < 4; e++) sum[e] = __builtin_fmaf(sum[e], kLog2E, bias[e]);
+  return sum;
 }
 
-// d of four items of a row
-__device__ __forceinline__ f32x4 slope4(f32x4 logit, float lse, float scale, uint32_t hit) {
+// d of a row's item, before the target's part; the sum over k less lse is rounded once, whatever the two are
+__device__ __forceinline__ float chance(float sum, float lse, float bias) { return __builtin_amdgcn_exp2f(__builtin_fmaf(sum - lse, kLog2E, bias)); }
+__device__ __forceinline__ f32x4 slope4(f32x4 sum, f32x4 bias, float lse, float scale, uint32_t hit) {
   f32x4 d;
 #pragma unroll
-  for (int e = 0; e < 4; e++) d[e] = (exp_less(logit[e], lse) - (hit == (uint32_t)e ? 1.f : 0.f)) * scale;
+  for (int e = 0; e < 4; e++) d[e] = (chance(sum[e], lse, bias[e]) - (hit == (uint32_t)e ? 1.f : 0.f)) * scale;
   return d;
 }
 
@@ -52,22 +50,16 @@ __global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kNo
   const uint32_t l = lane_id(), wave_column = P::wave_column();
   f32x4 bias[P::kColumnTiles];
 #pragma unroll
-  for (int j = 0; j < P::kColumnTiles; j++) bias[j] = bias4<T>(p, column0 + wave_column + j * 16 + l / 16 * 4);
+  for (int j = 0; j < P::kColumnTiles; j++) bias[j] = bias4(p, column0 + wave_column + j * 16 + l / 16 * 4);
   __syncthreads(); // the tiles are read
   if constexpr (!GRADIENT) {
     constexpr int ACROSS = TILE / 64;
     Tail *tails = (Tail *)tiles; // [ACROSS][TILE]
 #pragma unroll
     for (int i = 0; i < P::kRowTiles; i++) {
-      const uint32_t in = P::wave_row() + i * 16 + l % 16, r = row0 + in;
+      const uint32_t in = P::wave_row() + i * 16 + l % 16;
 #pragma unroll
-      for (int j = 0; j < P::kColumnTiles; j++) sum[i][j] += bias[j];
-      const uint32_t target = r < rows ? p.taken.target[r] : kNoItem;
-#pragma unroll
-      for (int j = 0; j < P::kColumnTiles; j++) {
-        const uint32_t e = target - (column0 + wave_column + j * 16 + l / 16 * 4);
-        if (e < 4) p.hit[r] = e < 2 ? (e ? sum[i][j][1] : sum[i][j][0]) : (e == 2 ? sum[i][j][2] : sum[i][j][3]);
-      }
+      for (int j = 0; j < P::kColumnTiles; j++) sum[i][j] = logit4(sum[i][j], bias[j]);
       Tail t = tail_of(sum[i]);
       t = join_lanes(t, 16);
       t = join_lanes(t, 32);
@@ -96,7 +88,7 @@ __global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kNo
 #pragma unroll
       for (int j = 0; j < P::kColumnTiles; j++) {
         const uint32_t c = wave_column + j * 16 + l / 16 * 4;
-        const f32x4 d = slope4(sum[i][j] + bias[j], lse, dloss, target - (column0 + c));
+        const f32x4 d = slope4(sum[i][j], bias[j], lse, dloss, target - (column0 + c));
         if (there) down[j] += d;
         if constexpr (sizeof(T) == 2) S::put(lds, in, c, d);
         else if (there && column0 + c < p.d_stride) write4<T>((T *)p.d + (uint64_t)r * p.d_stride, column0 + c, p.d_stride, d);
@@ -140,15 +132,14 @@ template <typename T, int ROWS, bool GRADIENT> __global__ __launch_bounds__((Few
   const uint32_t t = threadIdx.x, r = t / 8, c = t % 8 * 4;
   f32x4 d = {};
   if (r < rows && r < ROWS) {
-    const f32x4 logit[1] = {F::joined(sums, r, c) + bias4<T>(p, column0 + c)};
+    const f32x4 sum = F::joined(sums, r, c), bias = bias4(p, column0 + c);
     if constexpr (!GRADIENT) {
-      const uint32_t e = p.taken.target[r] - (column0 + c);
-      if (e < 4) p.hit[r] = e < 2 ? (e ? logit[0][1] : logit[0][0]) : (e == 2 ? logit[0][2] : logit[0][3]);
+      const f32x4 logit[1] = {logit4(sum, bias)};
       Tail tail = tail_of(logit);
       for (int mask = 1; mask < 8; mask *= 2) tail = join_lanes(tail, mask);
       if (c == 0) p.parts[(uint64_t)blockIdx.x * p.rows + r] = make_float2(tail.most, tail.sum);
     } else {
-      d = slope4(logit[0], p.taken.lse[r], p.taken.dloss[r] * p.taken.scale[0], p.taken.target[r] - p.first - (column0 + c));
+      d = slope4(sum, bias, p.taken.lse[r], p.taken.dloss[r] * p.taken.scale[0], p.taken.target[r] - p.first - (column0 + c));
       if (column0 + c < p.d_stride) write4<T>((T *)p.d + (uint64_t)r * p.d_stride, column0 + c, p.d_stride, d);
     }
   }
@@ -197,7 +188,15 @@ template <typename T> __global__ __launch_bounds__(256) void take_rows(TakeRows 
   constexpr int V = kVec<T>;
   __shared__ uint32_t words[5];
   __shared__ uint32_t place[kTakeRows];
-  const uint32_t first = blockIdx.x * kTakeRows, chunk = first / kChunk, t = threadIdx.x;
+  const uint32_t t = threadIdx.x, row_blocks = (p.rows + kTakeRows - 1) / kTakeRows;
+  if (blockIdx.x >= row_blocks) {
+    // a bias below -1e30 is as good as -infinity: a difference from it would say nothing about the rest of the logit
+    const uint32_t c = (blockIdx.x - row_blocks) * kFilled + t;
+    const float b = bias_at<T>(p.bias, p.narrow, c, p.items);
+    p.taken.bias[c] = c >= p.items || b < -1e30f ? -kInfinity : b * kLog2E;
+    return;
+  }
+  const uint32_t first = blockIdx.x * kTakeRows, chunk = first / kChunk;
   const uint32_t in = first % kChunk, chunk_rows = min(kChunk, p.rows - chunk * kChunk);
   // the rows of the chunk before this block's, and of the chunks before it; block 0 looks at all of them
   uint32_t before = 0, all = 0, most = 0;
@@ -232,6 +231,8 @@ template <typename T> __global__ __launch_bounds__(256) void take_rows(TakeRows 
       const float one = p.scaled ? largest_of(max(max(largest[0], largest[1]), max(largest[2], largest[3]))) : kScaled;
       p.taken.scale[0] = kScaled / one, p.taken.scale[1] = one / kScaled;
     }
+    if (p.dloss && total + t < (total + kFilled - 1) / kFilled * kFilled)
+      p.taken.target[total + t] = kNoItem, p.taken.dloss[total + t] = 0.f, p.taken.lse[total + t] = kInfinity;
   }
   if (t < kTakeRows) {
     const uint32_t r = first + t;
@@ -264,7 +265,59 @@ template <typename T> __global__ __launch_bounds__(256) void take_rows(TakeRows 
   }
 }
 template <typename T> void launch_take_rows(const TakeRows &p, hipStream_t s) {
-  hipLaunchKernelGGL((take_rows<T>), dim3(div_up(p.rows, kTakeRows)), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((take_rows<T>), dim3(div_up(p.rows, kTakeRows) + div_up(p.items, kFilled)), dim3(256), 0, s, p);
+  HCTR_HIP(hipGetLastError());
+}
+
+// The tiles' parts of 8 rows joined by 32 groups of threads, each of which takes every 32nd tile; then the groups', in pairs.  The same threads
+// multiply each row with its target's weights, for the logit that the loss is less by.
+constexpr uint32_t kJoinRows = 8, kJoinGroups = 32;
+template <typename T> __global__ __launch_bounds__(kJoinRows *kJoinGroups) void join_tails(JoinTails p) {
+  constexpr uint32_t LOADS = 8;
+  __shared__ Tail tails[kJoinGroups][kJoinRows];
+  __shared__ float hits[kJoinRows];
+  const uint32_t there = *p.taken.count, x = threadIdx.x % kJoinRows, y = threadIdx.x / kJoinRows, row0 = blockIdx.x * kJoinRows, r = row0 + x;
+  if (row0 >= there) return;
+  // a wave takes two of the rows
+  for (uint32_t i = threadIdx.x / kWave; i < kJoinRows && row0 + i < there; i += kJoinRows * kJoinGroups / kWave) {
+    const uint32_t item = p.taken.target[row0 + i];
+    float sum = 0.f;
+    if (item != kNoItem) {
+      constexpr int V = kVec<T>;
+      const T *a = (const T *)p.x + (uint64_t)(row0 + i) * p.x_stride, *b = (const T *)p.weight + (int64_t)item * p.weight_stride;
+      for (uint32_t c = lane_id() * V; c < p.width; c += kWave * V) {
+        const Floats<V> u = floats<V>(*(const typename Packed<T, V>::type *)(a + c)), w = load_columns<V, Rows::kLong, false>(b, c, p.width);
+#pragma unroll
+        for (int e = 0; e < V; e++) sum = __builtin_fmaf(u.v[e], w.v[e], sum);
+      }
+    }
+#pragma unroll
+    for (int mask = 32; mask; mask /= 2) sum += __shfl_xor(sum, mask);
+    if (lane_id() == 0) hits[i] = item == kNoItem ? __builtin_nanf("") : __builtin_fmaf(sum, kLog2E, p.taken.bias[item]);
+  }
+  Tail t = {kLowest, 0.f};
+  for (uint32_t i = y; i < p.tiles; i += kJoinGroups * LOADS) {
+    float2 v[LOADS];
+#pragma unroll
+    for (uint32_t k = 0; k < LOADS; k++)
+      v[k] = r < there && i + k * kJoinGroups < p.tiles ? p.parts[(uint64_t)(i + k * kJoinGroups) * p.rows + r] : make_float2(kLowest, 0.f);
+#pragma unroll
+    for (uint32_t k = 0; k < LOADS; k++) t = join(t, Tail{v[k].x, v[k].y});
+  }
+  tails[y][x] = t;
+  for (uint32_t n = kJoinGroups / 2; n; n /= 2) {
+    __syncthreads();
+    if (y < n) tails[y][x] = join(tails[y][x], tails[y + n][x]);
+  }
+  if (y || r >= there) return;
+  t = tails[0][x];
+  const float log_sum = log2f(t.sum), hit = hits[x];
+  const uint32_t to = p.taken.row_of[r];
+  p.loss[to] = (log_sum + (t.most - hit)) * kLog2;
+  if (p.lse) p.lse[to] = hit != hit ? hit : (log_sum + t.most) * kLog2;
+}
+template <typename T> void launch_join_tails(const JoinTails &p, hipStream_t s) {
+  hipLaunchKernelGGL((join_tails<T>), dim3(div_up(p.rows, kJoinRows)), dim3(kJoinRows * kJoinGroups), 0, s, p);
   HCTR_HIP(hipGetLastError());
 }
 
