@@ -139,13 +139,23 @@ template <typename T> __global__ __launch_bounds__(256) void gated_join(GatedFor
 
 template <typename T, int ROWS> __global__ __launch_bounds__((FewRows<T, ROWS>::kThreads)) void gated_few(GatedForward p) {
   typedef FewRows<T, ROWS> F;
-  __shared__ typename F::Sums sums[F::kWaves];
-  const uint32_t column0 = blockIdx.x * 16, left = min(16u, p.hidden - column0);
-  F::run((const T *)p.loose_x, p.loose_stride, p.rows, (const T *)p.loose_gate + (int64_t)column0 * p.loose_gate_stride,
-         (const T *)p.loose_up + (int64_t)column0 * p.loose_up_stride, left, left, p.loose_gate_stride, p.loose_up_stride, p.width, sums);
-  for (uint32_t t = threadIdx.x; t < p.rows * 4; t += F::kThreads) {
-    const uint32_t r = t / 4, c = t % 4 * 4;
-    if (c < left) finish_gated<T>(p, r, column0 + c, F::joined(sums, r, c), F::joined(sums, r, c + 16));
+  constexpr uint32_t HALF = F::kGroups / 2, COLUMNS = HALF * 16;
+  __shared__ typename F::Sums sums[F::kSums];
+  const uint32_t column0 = blockIdx.x * COLUMNS;
+  const T *groups[F::kGroups];
+  uint32_t left[F::kGroups];
+  int64_t stride[F::kGroups];
+#pragma unroll
+  for (uint32_t j = 0; j < HALF; j++) {
+    const uint32_t c = min(column0 + j * 16, p.hidden - 1); // (behind the last column: that one again)
+    groups[j] = (const T *)p.loose_gate + (int64_t)c * p.loose_gate_stride, groups[j + HALF] = (const T *)p.loose_up + (int64_t)c * p.loose_up_stride;
+    stride[j] = p.loose_gate_stride, stride[j + HALF] = p.loose_up_stride;
+    left[j] = left[j + HALF] = p.hidden - c;
+  }
+  F::run((const T *)p.loose_x, p.loose_stride, p.rows, groups, left, stride, p.width, sums);
+  for (uint32_t t = threadIdx.x; t < p.rows * (COLUMNS / 4); t += F::kThreads) {
+    const uint32_t r = t / (COLUMNS / 4), c = t % (COLUMNS / 4) * 4;
+    if (column0 + c < p.hidden) finish_gated<T>(p, r, column0 + c, *(const f32x4 *)&sums[0][r][c], *(const f32x4 *)&sums[0][r][c + COLUMNS]);
   }
 }
 
@@ -207,10 +217,13 @@ template <typename T> void launch_gated(GatedForward &p, int tile, hipStream_t s
   }
 }
 template <typename T> void launch_gated_few(const GatedForward &p, hipStream_t s) {
-  const dim3 blocks(div_up(p.hidden, 16));
-  if (p.rows <= 16) hipLaunchKernelGGL((gated_few<T, 16>), blocks, dim3(FewRows<T, 16>::kThreads), 0, s, p);
-  else if (p.rows <= 32) hipLaunchKernelGGL((gated_few<T, 32>), blocks, dim3(FewRows<T, 32>::kThreads), 0, s, p);
-  else hipLaunchKernelGGL((gated_few<T, 64>), blocks, dim3(FewRows<T, 64>::kThreads), 0, s, p);
+  const auto launch = [&](auto kernel, auto f) {
+    typedef decltype(f) F;
+    hipLaunchKernelGGL(kernel, dim3(div_up(p.hidden, F::kWeights / 2)), dim3(F::kThreads), 0, s, p);
+  };
+  if (p.rows <= 16) launch(gated_few<T, 16>, FewRows<T, 16>());
+  else if (p.rows <= 32) launch(gated_few<T, 32>, FewRows<T, 32>());
+  else launch(gated_few<T, 64>, FewRows<T, 64>());
   HCTR_HIP(hipGetLastError());
 }
 template <typename T> void launch_slopes(const GatedSlopes &p, hipStream_t s) {

@@ -120,45 +120,56 @@ __global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kNo
 
 template <typename T, int ROWS, bool GRADIENT> __global__ __launch_bounds__((FewRows<T, ROWS>::kThreads)) void items_few(ItemsProduct p) {
   typedef FewRows<T, ROWS> F;
-  static_assert(ROWS * 8 <= F::kThreads, "a thread takes four items of a row");
-  __shared__ typename F::Sums sums[F::kWaves];
-  const uint32_t rows = *p.taken.count, column0 = blockIdx.x * kFewItems, left = p.items - column0;
+  constexpr uint32_t QUADS = F::kWeights / 4; // of a row
+  __shared__ typename F::Sums sums[F::kSums];
+  const uint32_t rows = *p.taken.count, column0 = blockIdx.x * F::kWeights;
   if (!rows) return;
-  const T *weight = (const T *)p.loose_weight + (int64_t)column0 * p.loose_stride;
-  const bool second = left > 16;
-  // (the second sixteen are the first ones again if there are no more)
-  F::run((const T *)p.few_x, p.few_stride, rows, weight, weight + (second ? 16 * p.loose_stride : 0), min(left, 16u), second ? min(left - 16, 16u) : min(left, 16u),
-         p.loose_stride, p.loose_stride, p.width, sums);
-  const uint32_t t = threadIdx.x, r = t / 8, c = t % 8 * 4;
-  f32x4 d = {};
-  if (r < rows && r < ROWS) {
-    const f32x4 sum = F::joined(sums, r, c), bias = bias4(p, column0 + c);
+  const T *groups[F::kGroups];
+  uint32_t left[F::kGroups];
+  int64_t stride[F::kGroups];
+#pragma unroll
+  for (uint32_t j = 0; j < F::kGroups; j++) {
+    const uint32_t c = min(column0 + j * 16, p.items - 1); // (behind the last item: that one again)
+    groups[j] = (const T *)p.loose_weight + (int64_t)c * p.loose_stride;
+    stride[j] = p.loose_stride;
+    left[j] = p.items - c;
+  }
+  F::run((const T *)p.few_x, p.few_stride, rows, groups, left, stride, p.width, sums);
+  // four items of a row a thread; the threads of a row are neighbours
+  for (uint32_t t = threadIdx.x; t < ROWS * QUADS; t += F::kThreads) {
+    const uint32_t r = t / QUADS, c = t % QUADS * 4;
+    const f32x4 sum = *(const f32x4 *)&sums[0][r][c], bias = column0 + c < p.items ? bias4(p, column0 + c) : f32x4{-kInfinity, -kInfinity, -kInfinity, -kInfinity};
     if constexpr (!GRADIENT) {
       const f32x4 logit[1] = {logit4(sum, bias)};
       Tail tail = tail_of(logit);
-      for (int mask = 1; mask < 8; mask *= 2) tail = join_lanes(tail, mask);
-      if (c == 0) p.parts[(uint64_t)blockIdx.x * p.rows + r] = make_float2(tail.most, tail.sum);
+#pragma unroll
+      for (uint32_t mask = 1; mask < QUADS; mask *= 2) tail = join_lanes(tail, mask);
+      if (c == 0 && r < rows) p.parts[(uint64_t)blockIdx.x * p.rows + r] = make_float2(tail.most, tail.sum);
     } else {
-      d = slope4(sum, bias, p.taken.lse[r], p.taken.dloss[r] * p.taken.scale[0], p.taken.target[r] - p.first - (column0 + c));
-      if (column0 + c < p.d_stride) write4<T>((T *)p.d + (uint64_t)r * p.d_stride, column0 + c, p.d_stride, d);
+      f32x4 d = {};
+      if (r < rows) {
+        d = slope4(sum, bias, p.taken.lse[r], p.taken.dloss[r] * p.taken.scale[0], p.taken.target[r] - p.first - (column0 + c));
+        if (column0 + c < p.d_stride) write4<T>((T *)p.d + (uint64_t)r * p.d_stride, column0 + c, p.d_stride, d);
+      }
+      *(f32x4 *)&sums[0][r][c] = d;
     }
   }
   if (GRADIENT && p.sums) {
-    __syncthreads(); // the sums are read
-    if (r < ROWS) *(f32x4 *)&sums[0][r][c] = d;
     __syncthreads();
-    if (t < 8 && column0 + t * 4 < p.d_stride) {
+    const uint32_t c = threadIdx.x * 4;
+    if (c < F::kWeights && column0 + c < p.d_stride) {
       f32x4 all = {};
-      for (uint32_t i = 0; i < min(rows, (uint32_t)ROWS); i++) all += *(const f32x4 *)&sums[0][i][t * 4];
-      *(f32x4 *)(p.sums + column0 + t * 4) = all;
+      for (uint32_t i = 0; i < min(rows, (uint32_t)ROWS); i++) all += *(const f32x4 *)&sums[0][i][c];
+      *(f32x4 *)(p.sums + column0 + c) = all;
     }
   }
 }
 
 template <typename T, bool GRADIENT> void launch_items(ItemsProduct &p, int tile, hipStream_t s) {
   if (!tile) {
-    p.column_tiles = div_up(p.items, kFewItems);
+    p.column_tiles = div_up(p.items, few_items(p.rows));
     const dim3 blocks(p.column_tiles), threads(FewRows<T, 16>::kThreads);
+    static_assert(FewRows<T, 16>::kWeights == few_items(16) && FewRows<T, 32>::kWeights == few_items(32) && FewRows<T, 64>::kWeights == few_items(64));
     if (p.rows <= 16) hipLaunchKernelGGL((items_few<T, 16, GRADIENT>), blocks, threads, 0, s, p);
     else if (p.rows <= 32) hipLaunchKernelGGL((items_few<T, 32, GRADIENT>), blocks, threads, 0, s, p);
     else hipLaunchKernelGGL((items_few<T, 64, GRADIENT>), blocks, threads, 0, s, p);
