@@ -37,7 +37,7 @@ template <typename F> __device__ __forceinline__ void with_entry(const Entries &
 }
 
 // f(piece, place, how many of its values are there) for the kLoads pieces of 16 bytes that a thread has of a chunk, all loaded first
-template <typename T, typename F> __device__ __forceinline__ void pieces_of(const T *values, uint64_t count, uint32_t chunk, F &&f) {
+template <bool ONCE, typename T, typename F> __device__ __forceinline__ void pieces_of(const T *values, uint64_t count, uint32_t chunk, F &&f) {
   constexpr int V = kVec<T>;
   typedef typename Packed<T, V>::memory Loose;
   const uint64_t base = (uint64_t)chunk * (kChunkBytes / sizeof(T)) + threadIdx.x * V;
@@ -47,7 +47,7 @@ template <typename T, typename F> __device__ __forceinline__ void pieces_of(cons
     const uint64_t at = base + (uint64_t)i * (kBlock * V);
     v[i] = (T)0;
     if (at + V <= count) {
-      v[i] = *(const Loose *)(values + at);
+      v[i] = ONCE ? __builtin_nontemporal_load((const Loose *)(values + at)) : *(const Loose *)(values + at);
     } else if (at < count) {
 #pragma unroll
       for (int j = 0; j < V; j++)
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(kBlock) void sum_squares(Entries e, double *sums) {
   double sum = 0.0;
   for (uint32_t chunk = blockIdx.x; chunk < e.chunks; chunk += gridDim.x)
     with_entry(e, chunk, [&](const auto *values, auto *, uint64_t count, uint32_t in) {
-      pieces_of(values, count, in, [&](const auto &v, uint64_t, uint32_t) {
+      pieces_of<false>(values, count, in, [&](const auto &v, uint64_t, uint32_t) {
 #pragma unroll
         for (int j = 0; j < (int)(sizeof(v) / sizeof(*values)); j++) {
           const double d = (double)(float)v[j];
@@ -96,21 +96,25 @@ __device__ __forceinline__ double total_norm(const double *sums, uint32_t count)
   return sqrt(block_total(sum));
 }
 
-__global__ __launch_bounds__(kBlock) void finish_norm(const double *sums, uint32_t count, const float *given, float *norm) {
+// the norm, as a float and for scale_gradients; either may be null
+__global__ __launch_bounds__(kBlock) void finish_norm(const double *sums, uint32_t count, const float *given, float *norm, double *whole) {
   const double n = given ? (double)*given : total_norm(sums, count);
-  if (threadIdx.x == 0) *norm = (float)n;
+  if (threadIdx.x) return;
+  if (norm) *norm = (float)n;
+  if (whole) *whole = n;
 }
 
-// The chunks are taken in the other direction than by sum_squares: what was read last is still in the last cache.
-__global__ __launch_bounds__(kBlock) void scale_gradients(Entries e, const double *sums, uint32_t count, const float *given, float max_norm, float *norm) {
-  const double n = given ? (double)*given : total_norm(sums, count);
+// The chunks are taken in the other direction than by sum_squares: what was read last is still in the last cache.  The norm is `given`, or
+// `whole`, or made of the sums by every block.
+__global__ __launch_bounds__(kBlock) void scale_gradients(Entries e, const double *sums, uint32_t count, const float *given, const double *whole, float max_norm, float *norm) {
+  const double n = given ? (double)*given : whole ? *whole : total_norm(sums, count);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
   const bool same = n <= (double)max_norm;
   const float factor = same ? 1.f : (float)((double)max_norm / n);
   for (uint32_t i = blockIdx.x; i < e.chunks; i += gridDim.x)
     with_entry(e, e.chunks - 1 - i, [&](const auto *values, auto *into, uint64_t total, uint32_t in) {
       if (same && values == into) return;
-      pieces_of(values, total, in, [&](const auto &v, uint64_t at, uint32_t there) {
+      pieces_of<true>(values, total, in, [&](const auto &v, uint64_t at, uint32_t there) {
         typedef std::remove_const_t<std::remove_pointer_t<decltype(into)>> T;
         constexpr int V = kVec<T>;
         Floats<V> f = floats<V>(v);
@@ -202,7 +206,7 @@ void check_places(const hctr_clip_args &a) {
 
 size_t gradient_workspace(const hctr_clip_args &a) {
   check(a);
-  return launches_of(a) * most_blocks(launches_of(a)) * sizeof(double);
+  return (launches_of(a) * most_blocks(launches_of(a)) + 1) * sizeof(double); // the sums, and the norm
 }
 
 void gradient_norm(const hctr_clip_args &a, bool clip) {
@@ -227,13 +231,21 @@ void gradient_norm(const hctr_clip_args &a, bool clip) {
       count += blocks;
     });
   float *norm = a.norm == a.given ? nullptr : a.norm;
-  if (norm && (!clip || !launches)) {
-    hipLaunchKernelGGL(finish_norm, dim3(1), dim3(kBlock), 0, s, (const double *)sums, count, clip ? a.given : nullptr, norm);
+  uint64_t chunks = 0;
+  for (size_t i = 0; i < a.count; i++) chunks += chunks_of(a.gradients[i]);
+  // Few chunks: the blocks that scale make the norm themselves, a launch less (28.8 MB in 17 gradients: FEW us, with three launches MANY).  Many:
+  // a block for each, without that work, moves more at a time than blocks that stay (4.1 GB: 1787 us, ONE EACH).
+  const bool many = chunks > 4 * kMostBlocks;
+  double *whole = clip && many && !a.given ? sums + launches * most : nullptr;
+  if (!clip || !launches || whole) {
+    if (norm || whole) hipLaunchKernelGGL(finish_norm, dim3(1), dim3(kBlock), 0, s, (const double *)sums, count, clip ? a.given : nullptr, norm, whole);
     HCTR_HIP(hipGetLastError());
+    if (whole) norm = nullptr;
   }
   if (!clip) return;
   in_launches(a, [&](const Entries &e) {
-    hipLaunchKernelGGL(scale_gradients, dim3(std::min(e.chunks, kMostBlocks)), dim3(kBlock), 0, s, e, (const double *)sums, count, a.given, a.max_norm, norm);
+    const uint32_t blocks = many ? std::min(e.chunks, 1u << 23) : std::min(e.chunks, kMostBlocks);
+    hipLaunchKernelGGL(scale_gradients, dim3(blocks), dim3(kBlock), 0, s, e, (const double *)sums, count, a.given, (const double *)whole, a.max_norm, norm);
     HCTR_HIP(hipGetLastError());
     norm = nullptr;
   });

@@ -70,10 +70,9 @@ template <typename T, typename A> TakeRows take(const A &a, const float *dloss, 
 }
 Operand taken_rows(const TakeRows &t, size_t size) { return {{(const char *)t.to, nullptr}, (int64_t)(t.to_stride * size), t.rows, 0, 0}; }
 
-// Few rows take the weights past the LDS, narrow ones hold their rows in registers, others go by tiles.
+// Narrow matrices of 16 bits hold their rows in registers; few rows take the weights past the LDS; others go by tiles.
 enum class Way { kFew, kNarrow, kTiles };
-Way way_of(size_t rows, size_t width, size_t size, bool gradient) {
-  if (!gradient && rows <= kFewRows) return Way::kFew;
+Way way_of(size_t rows, size_t width, size_t size) {
   if (size == 2 && width <= kNarrow) return Way::kNarrow;
   return rows <= kFewRows ? Way::kFew : Way::kTiles;
 }
@@ -87,7 +86,7 @@ ForwardPlan plan_of(const hctr_items_args &a) {
   ForwardPlan p = {};
   if (!a.rows) return p;
   const size_t size = size_of(a.dtype);
-  p.way = way_of(a.rows, a.width, size, false);
+  p.way = way_of(a.rows, a.width, size);
   if (p.way == Way::kTiles) p.tile = shape_of(a.rows, a.items, a.width, (int)size, false, false).tile;
   p.tiles = p.way == Way::kNarrow ? narrow_ranges(a.rows, a.items, a.width, false) : div_up(a.items, p.tile ? p.tile : few_items(a.rows));
   p.parts = up(p.tiles * a.rows * sizeof(float2), 256);
@@ -152,7 +151,7 @@ struct BackwardPlan {
 BackwardPlan plan_of(const hctr_items_grad_args &a) {
   BackwardPlan p = {};
   const size_t size = size_of(a.dtype), rows = std::max<size_t>(a.rows, 1);
-  p.way = way_of(a.rows, a.width, size, true);
+  p.way = way_of(a.rows, a.width, size);
   if (a.rows && p.way == Way::kNarrow) {
     p.rows = rows_space(a.rows, a.width, a.items, size).bytes;
     p.weight = laid_out_bytes(a.weight, a.items, a.width, size);

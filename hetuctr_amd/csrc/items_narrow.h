@@ -85,6 +85,9 @@ template <typename T, int KS, Narrow MODE> __global__ __launch_bounds__(256, 2) 
   const char *own = WEIGHT ? p.weight : p.x, *other = WEIGHT ? p.x : p.weight;
   const int64_t own_stride = WEIGHT ? p.weight_stride : p.x_stride, stride = WEIGHT ? p.x_stride : p.weight_stride;
 
+  // Of the two waves that share a SIMD one goes first, so that they do not do the same at the same time: by the number that the hardware gave it
+  // (us, weights' gradient: 4096 rows and a million items 2236 -> 2136, 65536 and 20000 956 -> 865; the others the same or 1 % slower).
+  if (WEIGHT && __builtin_amdgcn_s_getreg(3 << 11 | 4) & 1) __builtin_amdgcn_s_setprio(1);
   Fragment<T> mine[OI][KS];
   float own_bias[OI], lse[OI], dloss[OI];
   uint32_t target[OI];

@@ -199,31 +199,65 @@ template <typename T, Lies LA, Lies LB, Second SB, int BM, int BN> struct Produc
 #pragma unroll
       for (int j = 0; j < kColumnTiles; j++) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (k0 >= k1) return;
-    ta.load(k0, k1 - k0, lds);
-    tb.load(k0, k1 - k0, lds + BM * kStepBytes);
-    uint32_t stage = 0;
-    for (uint32_t k = k0; k < k1; k += step) {
+    const auto load = [&](uint32_t k, uint32_t stage) {
+      ta.load(k, k1 - k, lds + stage * kStageBytes);
+      tb.load(k, k1 - k, lds + stage * kStageBytes + BM * kStepBytes);
+    };
+    // Half a step's fragments are read from LDS while the other half's are multiplied, a few instructions between each of them.  The barrier
+    // stands in the middle: there the second half of this step is in registers, and nobody needs its tiles any more; the next step's
+    // tiles are there, which have been under way for a whole step; and there is work at hand for both sides of it.  (8192 x 8192 x 8192 in
+    // bfloat16, operands of zeros, which the clock does not suffer from: 852 us with a step's reads in front of its products, 741 so; random ones
+    // 1083 and 988.)
+    Fragment<T> fa[2][kRowTiles], fb[2][kColumnTiles];
+    const auto read = [&](uint32_t from, auto half) {
+      constexpr uint32_t H = decltype(half)::value;
+#pragma unroll
+      for (int j = 0; j < kColumnTiles; j++) fb[H][j] = fragment<T, LB, BN>(from + BM * kStepBytes, wave_column() + j * 16, H);
+#pragma unroll
+      for (int i = 0; i < kRowTiles; i++) fa[H][i] = fragment<T, LA, BM>(from, wave_row() + i * 16, H);
+    };
+    const auto products = [&](auto half) {
+      constexpr uint32_t H = decltype(half)::value;
+#pragma unroll
+      for (int i = 0; i < kRowTiles; i++)
+#pragma unroll
+        for (int j = 0; j < kColumnTiles; j++) sum[i][j] = multiply<T>(fb[H][j], fa[H][i], sum[i][j]);
+    };
+    constexpr std::integral_constant<uint32_t, 0> first;
+    constexpr std::integral_constant<uint32_t, 1> second;
+    // reads and products of one region, in turn
+    constexpr int kPerFragment = sizeof(T) == 2 ? 2 : 4, kMultiplies = kRowTiles * kColumnTiles * (sizeof(T) == 2 ? 1 : 4);
+    constexpr int kReads = kRowTiles * (LA == Lies::kAlong ? 1 : kPerFragment) + kColumnTiles * (LB == Lies::kAlong ? 1 : kPerFragment);
+    const auto in_turn = [&] {
+#pragma unroll
+      for (int i = 0; i < kReads; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, kMultiplies / kReads, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x8, kMultiplies - kReads * (kMultiplies / kReads), 0);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    load(k0, 0);
+    tiles_ready();
+    if (k0 + step < k1) load(k0 + step, 1);
+    read(lds, first);
+    uint32_t stage = 0, k = k0;
+    for (; k + step < k1; k += step) {
+      __builtin_amdgcn_sched_barrier(0);
+      read(lds + stage * kStageBytes, second);
+      products(first);
+      in_turn();
       tiles_ready();
-      const uint32_t here = lds + stage * kStageBytes;
+      if (k + 2 * step < k1) load(k + 2 * step, stage);
       stage ^= 1;
-      if (k + step < k1) {
-        const uint32_t next = lds + stage * kStageBytes;
-        ta.load(k + step, k1 - k - step, next);
-        tb.load(k + step, k1 - k - step, next + BM * kStepBytes);
-      }
-#pragma unroll
-      for (uint32_t kk = 0; kk < 2; kk++) {
-        Fragment<T> fa[kRowTiles], fb[kColumnTiles];
-#pragma unroll
-        for (int j = 0; j < kColumnTiles; j++) fb[j] = fragment<T, LB, BN>(here + BM * kStepBytes, wave_column() + j * 16, kk);
-#pragma unroll
-        for (int i = 0; i < kRowTiles; i++) fa[i] = fragment<T, LA, BM>(here, wave_row() + i * 16, kk);
-#pragma unroll
-        for (int i = 0; i < kRowTiles; i++)
-#pragma unroll
-          for (int j = 0; j < kColumnTiles; j++) sum[i][j] = multiply<T>(fb[j], fa[i], sum[i][j]);
-      }
+      __builtin_amdgcn_sched_barrier(0);
+      read(lds + stage * kStageBytes, first);
+      products(second);
+      in_turn();
     }
+    read(lds + stage * kStageBytes, second);
+    products(first);
+    products(second);
   }
 };
 

@@ -6,22 +6,19 @@
 namespace hctr {
 
 // The tile and the number of parts along k that a product should take least time with, in us.  A tile of 256 x 256 has a CU for itself and takes
-// `large` us for a step of 128 bytes of k; of those of 128 x 128 two share a CU: `two` us a step, or `one` while it is alone.  Parts are
-// written and read again as floats.
+// `large` us for a step of 128 bytes of k; of those of 128 x 128 two share a CU, and take `two` us a step together, or `one` alone.  Every
+// tile costs what it takes to begin and to end.  Parts are written and read again as floats, by a launch more.
 Shape shape_of(size_t rows, size_t columns, size_t k, int size, bool paired, bool may_split) {
-  const double large = size == 2 ? 1.8 : 7.7, two = size == 2 ? 1.05 : 3.9, one = size == 2 ? 0.8 : 2.0;
+  const double large = size == 2 ? 1.8 : 7.7, two = size == 2 ? 1.05 : 3.9, one = size == 2 ? 0.8 : 2.0, ends = 4.0;
   const size_t cus = 256, steps = (k * size + kStepBytes - 1) / kStepBytes, wide = paired ? 2 * columns : columns;
   Shape best = {128, 1};
   double least = 1e30;
   for (int tile : {256, 128}) {
     const size_t tiles = ((rows + tile - 1) / tile) * ((wide + tile - 1) / tile);
-    for (uint32_t splits = 1; splits <= (may_split ? 64u : 1u) && (splits == 1 || steps / splits >= 4); splits *= 2) {
-      const size_t blocks = tiles * splits, each = (steps + splits - 1) / splits;
-      double t;
-      if (tile == 256) t = (double)((blocks + cus - 1) / cus) * (each * large + 4.0);
-      else if (blocks <= cus) t = each * one + 4.0;
-      else t = (double)((blocks + 2 * cus - 1) / (2 * cus)) * (each * two + 4.0);
-      if (splits > 1) t += 4.0 + 2e-6 * parts_bytes(rows, wide, splits) / 4.0;
+    for (uint32_t splits = 1; splits <= (may_split ? 32u : 1u) && (splits == 1 || steps / splits >= 4); splits++) {
+      const size_t each = (steps + splits - 1) / splits, turns = (tiles * splits + cus - 1) / cus; // tiles that a CU has to do
+      double t = tile == 256 ? turns * (each * large + ends) : turns / 2 * (each * two + ends) + turns % 2 * (each * one + ends);
+      if (splits > 1) t += 4.0 + 0.5e-6 * parts_bytes(rows, wide, splits);
       if (t < least) least = t, best = {tile, splits};
     }
   }
@@ -71,9 +68,31 @@ template <typename W> __global__ __launch_bounds__(kSumThreads) void column_sums
   if (to && at < p.count) to[at] = (W)sum;
 }
 
+// few rows: a thread per column
+template <typename W> __global__ __launch_bounds__(256) void few_sums(ColumnSums p) {
+  const uint32_t c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= p.columns) return;
+  const uint32_t rows = p.rows_there ? min(p.rows, (*p.rows_there + p.per - 1) / p.per) : p.rows;
+  float sum = 0.f;
+  for (uint32_t i = 0; i < rows; i++) sum += p.partial[(uint64_t)i * p.columns + c];
+  if (p.scale) sum *= *p.scale;
+  const bool second = c >= p.second_from;
+  const uint32_t at = c - (second ? p.second_from : 0);
+  W *to = (W *)(second ? p.out[1] : p.out[0]);
+  if (to && at < p.count) to[at] = (W)sum;
+}
+
 } // namespace
 
 void launch_column_sums(const ColumnSums &c, int dtype, hipStream_t s) {
+  if (c.rows <= 4) {
+    const dim3 blocks(div_up(c.columns, 256)), threads(256);
+    if (dtype == HCTR_F32) hipLaunchKernelGGL((few_sums<float>), blocks, threads, 0, s, c);
+    else if (dtype == HCTR_BF16) hipLaunchKernelGGL((few_sums<bf16_t>), blocks, threads, 0, s, c);
+    else hipLaunchKernelGGL((few_sums<f16_t>), blocks, threads, 0, s, c);
+    HCTR_HIP(hipGetLastError());
+    return;
+  }
   const dim3 blocks(div_up(c.columns, kSumColumns)), threads(kSumThreads);
   if (dtype == HCTR_F32) hipLaunchKernelGGL((column_sums<float>), blocks, threads, 0, s, c);
   else if (dtype == HCTR_BF16) hipLaunchKernelGGL((column_sums<bf16_t>), blocks, threads, 0, s, c);
