@@ -1,19 +1,27 @@
-// Products of a few rows (up to 64) with a matrix of weights, which is all that takes time: it is read once, straight into registers.
+// Products of a few rows (up to 32) with a matrix of weights, which is all that takes time: it is read once, straight into registers.
 #pragma once
 #include "matmul.h"
 
 namespace hctr {
 
-constexpr uint32_t kFewRows = 64;
+constexpr uint32_t kFewRows = 32;
 
-// ROWS (16, 32 or 64) rows of x times kWeights rows of weights, in groups of 16 that the caller says the places of.  A block's waves share out
-// k; every wave has the fragments of kAhead steps under way, which lanes fetch from any address an element can have.  The waves'
-// sums are joined through LDS, in pairs.  With more than 16 rows a wave takes 64 rows of weights at a time instead of 32, so
-// that x, which every block reads, is not most of what goes through the caches (us, half precision, 64 rows, twice 8192 x 8192: 95
-// with 32, LATER with 64).
-template <typename T, int ROWS> struct FewRows {
-  static constexpr int kWaves = 8, kThreads = kWaves * kWave, kTiles = ROWS / 16, kGroups = ROWS == 16 ? 2 : 4, kWeights = kGroups * 16,
-                       kAhead = ROWS == 16 ? 8 : ROWS == 32 ? 4 : 3, kPitch = kWeights + 4;
+// How many groups of 16 rows of weights a wave takes at a time: four, so that x, which every block reads, is not most of what goes through the
+// caches, but two where that leaves CUs idle, and for the fewest rows, whose x is next to nothing, where it leaves few blocks for the last
+// ones.  (us, bfloat16, with two and four: 16384 x 4096 twice, 1 row 46.9, 49.2, 16 rows 60.6, 51.1; 131072 x 4096, 1 row 223, 206,
+// 16 rows 253, 201.)
+inline int few_groups(size_t rows, size_t weights) {
+  const size_t blocks = weights / 64;
+  return blocks < 256 || (rows <= 4 && blocks < 1024) ? 2 : 4;
+}
+
+// ROWS (16 or 32) rows of x times GROUPS * 16 rows of weights, in groups of 16 that the caller says the places of.  A block's waves share out
+// k; every wave has the fragments of kAhead steps under way, which lanes fetch from any address an element can have: as many as leave
+// room for several blocks on a CU, which hide more than further steps of one would (32 rows and 131072 x 4096: 226 us with four steps, 206
+// with two).  The waves' sums are joined through LDS, in pairs.
+template <typename T, int ROWS, int GROUPS> struct FewRows {
+  static constexpr int kWaves = 8, kThreads = kWaves * kWave, kTiles = ROWS / 16, kGroups = GROUPS, kWeights = kGroups * 16, kAhead = kTiles == 1 && GROUPS == 2 ? 8 : kTiles == 1 ? 4 : 2,
+                       kPitch = kWeights + 4;
   typedef float Sums[ROWS][kPitch];
   typedef typename Packed<T, kVec<T>>::memory Loose;
   static constexpr uint32_t kStepK = 64 / sizeof(T);

@@ -137,8 +137,8 @@ template <typename T> __global__ __launch_bounds__(256) void gated_join(GatedFor
   }
 }
 
-template <typename T, int ROWS> __global__ __launch_bounds__((FewRows<T, ROWS>::kThreads)) void gated_few(GatedForward p) {
-  typedef FewRows<T, ROWS> F;
+template <typename T, int ROWS, int GROUPS> __global__ __launch_bounds__((FewRows<T, ROWS, GROUPS>::kThreads)) void gated_few(GatedForward p) {
+  typedef FewRows<T, ROWS, GROUPS> F;
   constexpr uint32_t HALF = F::kGroups / 2, COLUMNS = HALF * 16;
   __shared__ typename F::Sums sums[F::kSums];
   const uint32_t column0 = blockIdx.x * COLUMNS;
@@ -217,13 +217,16 @@ template <typename T> void launch_gated(GatedForward &p, int tile, hipStream_t s
   }
 }
 template <typename T> void launch_gated_few(const GatedForward &p, hipStream_t s) {
-  const auto launch = [&](auto kernel, auto f) {
-    typedef decltype(f) F;
-    hipLaunchKernelGGL(kernel, dim3(div_up(p.hidden, F::kWeights / 2)), dim3(F::kThreads), 0, s, p);
+  const auto launch = [&](auto kernel, int groups) {
+    hipLaunchKernelGGL(kernel, dim3(div_up(p.hidden, 8 * groups)), dim3(FewRows<T, 16, 2>::kThreads), 0, s, p);
   };
-  if (p.rows <= 16) launch(gated_few<T, 16>, FewRows<T, 16>());
-  else if (p.rows <= 32) launch(gated_few<T, 32>, FewRows<T, 32>());
-  else launch(gated_few<T, 64>, FewRows<T, 64>());
+  if (few_groups(p.rows, 2 * (size_t)p.hidden) == 2) {
+    if (p.rows <= 16) launch(gated_few<T, 16, 2>, 2);
+    else launch(gated_few<T, 32, 2>, 2);
+  } else {
+    if (p.rows <= 16) launch(gated_few<T, 16, 4>, 4);
+    else launch(gated_few<T, 32, 4>, 4);
+  }
   HCTR_HIP(hipGetLastError());
 }
 template <typename T> void launch_slopes(const GatedSlopes &p, hipStream_t s) {

@@ -57,8 +57,6 @@ struct ItemsProduct {
 };
 template <typename T> void launch_items_forward(ItemsProduct &p, int tile, hipStream_t s);  // tile 0: few rows
 template <typename T> void launch_items_gradient(ItemsProduct &p, int tile, hipStream_t s);
-constexpr uint32_t few_items(size_t rows) { return rows <= 16 ? 32 : 64; } // a tile's items where rows are few
-
 // The parts of the rows joined: loss and lse
 struct JoinTails {
   const float2 *parts;

@@ -88,7 +88,7 @@ ForwardPlan plan_of(const hctr_items_args &a) {
   const size_t size = size_of(a.dtype);
   p.way = way_of(a.rows, a.width, size);
   if (p.way == Way::kTiles) p.tile = shape_of(a.rows, a.items, a.width, (int)size, false, false).tile;
-  p.tiles = p.way == Way::kNarrow ? narrow_ranges(a.rows, a.items, a.width, false) : div_up(a.items, p.tile ? p.tile : few_items(a.rows));
+  p.tiles = p.way == Way::kNarrow ? narrow_ranges(a.rows, a.items, a.width, false) : div_up(a.items, p.tile ? p.tile : 16 * few_groups(a.rows, a.items));
   p.parts = up(p.tiles * a.rows * sizeof(float2), 256);
   p.weight = p.way == Way::kFew ? 0 : laid_out_bytes(a.weight, a.items, a.width, size);
   p.bytes = rows_space(a.rows, a.width, a.items, size).bytes + p.parts + p.weight;

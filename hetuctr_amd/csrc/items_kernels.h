@@ -118,8 +118,8 @@ __global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kNo
   }
 }
 
-template <typename T, int ROWS, bool GRADIENT> __global__ __launch_bounds__((FewRows<T, ROWS>::kThreads)) void items_few(ItemsProduct p) {
-  typedef FewRows<T, ROWS> F;
+template <typename T, int ROWS, int GROUPS, bool GRADIENT> __global__ __launch_bounds__((FewRows<T, ROWS, GROUPS>::kThreads)) void items_few(ItemsProduct p) {
+  typedef FewRows<T, ROWS, GROUPS> F;
   constexpr uint32_t QUADS = F::kWeights / 4; // of a row
   __shared__ typename F::Sums sums[F::kSums];
   const uint32_t rows = *p.taken.count, column0 = blockIdx.x * F::kWeights;
@@ -167,12 +167,17 @@ template <typename T, int ROWS, bool GRADIENT> __global__ __launch_bounds__((Few
 
 template <typename T, bool GRADIENT> void launch_items(ItemsProduct &p, int tile, hipStream_t s) {
   if (!tile) {
-    p.column_tiles = div_up(p.items, few_items(p.rows));
-    const dim3 blocks(p.column_tiles), threads(FewRows<T, 16>::kThreads);
-    static_assert(FewRows<T, 16>::kWeights == few_items(16) && FewRows<T, 32>::kWeights == few_items(32) && FewRows<T, 64>::kWeights == few_items(64));
-    if (p.rows <= 16) hipLaunchKernelGGL((items_few<T, 16, GRADIENT>), blocks, threads, 0, s, p);
-    else if (p.rows <= 32) hipLaunchKernelGGL((items_few<T, 32, GRADIENT>), blocks, threads, 0, s, p);
-    else hipLaunchKernelGGL((items_few<T, 64, GRADIENT>), blocks, threads, 0, s, p);
+    const auto launch = [&](auto kernel, int groups) {
+      p.column_tiles = div_up(p.items, 16 * groups);
+      hipLaunchKernelGGL(kernel, dim3(p.column_tiles), dim3(FewRows<T, 16, 2>::kThreads), 0, s, p);
+    };
+    if (few_groups(p.rows, p.items) == 2) {
+      if (p.rows <= 16) launch(items_few<T, 16, 2, GRADIENT>, 2);
+      else launch(items_few<T, 32, 2, GRADIENT>, 2);
+    } else {
+      if (p.rows <= 16) launch(items_few<T, 16, 4, GRADIENT>, 4);
+      else launch(items_few<T, 32, 4, GRADIENT>, 4);
+    }
   } else {
     p.row_tiles = div_up(p.rows, tile), p.column_tiles = div_up(p.items, tile);
     HCTR_CHECK((uint64_t)p.row_tiles * p.column_tiles * 512 < (1ull << 32), "linear cross entropy: too many tiles");
@@ -192,10 +197,8 @@ template <typename T> void launch_items_gradient(ItemsProduct &p, int tile, hipS
 constexpr float kScaled = 8192.f;
 __device__ __forceinline__ float largest_of(uint32_t bits) { return bits ? fmaxf(__builtin_bit_cast(float, bits), 0x1p-100f) : kScaled; }
 
-// Eight rows a block (a wave copies one at a time): it finds how many of those before them take part from the chunks' counts and its own
-// chunk's targets.
-constexpr uint32_t kTakeRows = 8;
-template <typename T> __global__ __launch_bounds__(256) void take_rows(TakeRows p) {
+// A few rows a block: it finds how many of those before them take part from the chunks' counts and its own chunk's targets.
+template <typename T, uint32_t kTakeRows> __global__ __launch_bounds__(256) void take_rows(TakeRows p) {
   constexpr int V = kVec<T>;
   __shared__ uint32_t words[5];
   __shared__ uint32_t place[kTakeRows];
@@ -262,41 +265,48 @@ template <typename T> __global__ __launch_bounds__(256) void take_rows(TakeRows 
     }
   }
   __syncthreads();
-  for (uint32_t i = t / kWave; i < kTakeRows; i += 256 / kWave) {
-    const uint32_t r = first + i, to = place[i];
-    if (r >= p.rows) break;
-    if (to != kNoItem) {
-      const T *from = (const T *)p.x + (int64_t)r * p.x_stride;
-      for (uint32_t c = lane_id() * V; c < p.to_stride; c += kWave * V)
-        *(typename Packed<T, V>::type *)((T *)p.to + (uint64_t)to * p.to_stride + c) = settled<V, Rows::kLong>(load_raw<V, Rows::kLong>(from, c, p.width), c, p.width);
-    } else if (p.dx) {
-      T *dx = (T *)p.dx + (int64_t)r * p.dx_stride;
-      for (uint32_t c = lane_id() * V; c < p.width; c += kWave * V) store_columns<V, Rows::kLong>(dx, c, p.width, Floats<V>{});
+  // all rows' pieces in turn, several loads under way
+  const uint32_t pieces = p.to_stride / V;
+  constexpr int LOADS = 4;
+  for (uint32_t from = t; from < kTakeRows * pieces; from += 256 * LOADS) {
+    typename Packed<T, V>::type v[LOADS];
+#pragma unroll
+    for (int k = 0; k < LOADS; k++) {
+      const uint32_t at = from + k * 256, i = at / pieces, c = (at - i * pieces) * V;
+      if (i < kTakeRows && place[i] != kNoItem) v[k] = load_raw<V, Rows::kLong>((const T *)p.x + (int64_t)(first + i) * p.x_stride, c, p.width);
+    }
+#pragma unroll
+    for (int k = 0; k < LOADS; k++) {
+      const uint32_t at = from + k * 256, i = at / pieces, c = (at - i * pieces) * V;
+      if (i >= kTakeRows || first + i >= p.rows) continue;
+      if (place[i] != kNoItem) *(typename Packed<T, V>::type *)((T *)p.to + (uint64_t)place[i] * p.to_stride + c) = settled<V, Rows::kLong>(v[k], c, p.width);
+      else if (p.dx) store_columns<V, Rows::kLong>((T *)p.dx + (int64_t)(first + i) * p.dx_stride, c, p.width, Floats<V>{});
     }
   }
 }
 template <typename T> void launch_take_rows(const TakeRows &p, hipStream_t s) {
-  hipLaunchKernelGGL((take_rows<T>), dim3(div_up(p.rows, kTakeRows) + div_up(p.items, kFilled)), dim3(256), 0, s, p);
+  const auto launch = [&](auto kernel, uint32_t rows) { hipLaunchKernelGGL(kernel, dim3(div_up(p.rows, rows) + div_up(p.items, kFilled)), dim3(256), 0, s, p); };
+  if (p.rows <= kChunk) launch(take_rows<T, 2>, 2);
+  else launch(take_rows<T, 8>, 8);
   HCTR_HIP(hipGetLastError());
 }
 
-// The tiles' parts of 8 rows joined by 32 groups of threads, each of which takes every 32nd tile; then the groups', in pairs.  The same threads
-// multiply each row with its target's weights, for the logit that the loss is less by.
-constexpr uint32_t kJoinRows = 8, kJoinGroups = 32;
-template <typename T> __global__ __launch_bounds__(kJoinRows *kJoinGroups) void join_tails(JoinTails p) {
-  constexpr uint32_t LOADS = 8;
-  __shared__ Tail tails[kJoinGroups][kJoinRows];
-  __shared__ float hits[kJoinRows];
-  const uint32_t there = *p.taken.count, x = threadIdx.x % kJoinRows, y = threadIdx.x / kJoinRows, row0 = blockIdx.x * kJoinRows, r = row0 + x;
+// The tiles' parts of ROWS rows joined by the other threads, each of which takes every so many tiles' parts of a row; then theirs, in pairs.  The
+// block's four waves multiply the rows with their targets' weights, for the logits that the losses are less by.
+template <typename T, uint32_t ROWS> __global__ __launch_bounds__(256) void join_tails(JoinTails p) {
+  constexpr uint32_t GROUPS = 256 / ROWS, LOADS = 8, WAVES = ROWS < 4 ? 4 / ROWS : 1; // waves for a row
+  constexpr int V = kVec<T>;
+  __shared__ Tail tails[GROUPS][ROWS];
+  __shared__ float hits[WAVES][ROWS];
+  const uint32_t there = *p.taken.count, x = threadIdx.x % ROWS, y = threadIdx.x / ROWS, row0 = blockIdx.x * ROWS, r = row0 + x;
   if (row0 >= there) return;
-  // a wave takes two of the rows
-  for (uint32_t i = threadIdx.x / kWave; i < kJoinRows && row0 + i < there; i += kJoinRows * kJoinGroups / kWave) {
-    const uint32_t item = p.taken.target[row0 + i];
+  for (uint32_t w = threadIdx.x / kWave; w < ROWS * WAVES; w += 4) {
+    const uint32_t i = w % ROWS, share = w / ROWS, item = row0 + i < there ? p.taken.target[row0 + i] : kNoItem;
     float sum = 0.f;
     if (item != kNoItem) {
-      constexpr int V = kVec<T>;
       const T *a = (const T *)p.x + (uint64_t)(row0 + i) * p.x_stride, *b = (const T *)p.weight + (int64_t)item * p.weight_stride;
-      for (uint32_t c = lane_id() * V; c < p.width; c += kWave * V) {
+#pragma unroll 4
+      for (uint32_t c = (share * kWave + lane_id()) * V; c < p.width; c += WAVES * kWave * V) {
         const Floats<V> u = floats<V>(*(const typename Packed<T, V>::type *)(a + c)), w = load_columns<V, Rows::kLong, false>(b, c, p.width);
 #pragma unroll
         for (int e = 0; e < V; e++) sum = __builtin_fmaf(u.v[e], w.v[e], sum);
@@ -304,31 +314,35 @@ template <typename T> __global__ __launch_bounds__(kJoinRows *kJoinGroups) void 
     }
 #pragma unroll
     for (int mask = 32; mask; mask /= 2) sum += __shfl_xor(sum, mask);
-    if (lane_id() == 0) hits[i] = item == kNoItem ? __builtin_nanf("") : __builtin_fmaf(sum, kLog2E, p.taken.bias[item]);
+    if (lane_id() == 0) hits[share][i] = item == kNoItem ? __builtin_nanf("") : share ? sum * kLog2E : __builtin_fmaf(sum, kLog2E, p.taken.bias[item]);
   }
   Tail t = {kLowest, 0.f};
-  for (uint32_t i = y; i < p.tiles; i += kJoinGroups * LOADS) {
+  for (uint32_t i = y; i < p.tiles; i += GROUPS * LOADS) {
     float2 v[LOADS];
 #pragma unroll
-    for (uint32_t k = 0; k < LOADS; k++)
-      v[k] = r < there && i + k * kJoinGroups < p.tiles ? p.parts[(uint64_t)(i + k * kJoinGroups) * p.rows + r] : make_float2(kLowest, 0.f);
+    for (uint32_t k = 0; k < LOADS; k++) v[k] = r < there && i + k * GROUPS < p.tiles ? p.parts[(uint64_t)(i + k * GROUPS) * p.rows + r] : make_float2(kLowest, 0.f);
 #pragma unroll
     for (uint32_t k = 0; k < LOADS; k++) t = join(t, Tail{v[k].x, v[k].y});
   }
   tails[y][x] = t;
-  for (uint32_t n = kJoinGroups / 2; n; n /= 2) {
+  for (uint32_t n = GROUPS / 2; n; n /= 2) {
     __syncthreads();
     if (y < n) tails[y][x] = join(tails[y][x], tails[y + n][x]);
   }
   if (y || r >= there) return;
   t = tails[0][x];
-  const float log_sum = log2f(t.sum), hit = hits[x];
+  float hit = hits[0][x];
+#pragma unroll
+  for (uint32_t w = 1; w < WAVES; w++) hit += hits[w][x];
+  const float log_sum = log2f(t.sum);
   const uint32_t to = p.taken.row_of[r];
   p.loss[to] = (log_sum + (t.most - hit)) * kLog2;
   if (p.lse) p.lse[to] = hit != hit ? hit : (log_sum + t.most) * kLog2;
 }
 template <typename T> void launch_join_tails(const JoinTails &p, hipStream_t s) {
-  hipLaunchKernelGGL((join_tails<T>), dim3(div_up(p.rows, kJoinRows)), dim3(kJoinRows * kJoinGroups), 0, s, p);
+  // (few rows: more blocks)
+  if (p.rows <= 1024) hipLaunchKernelGGL((join_tails<T, 2>), dim3(div_up(p.rows, 2)), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((join_tails<T, 8>), dim3(div_up(p.rows, 8)), dim3(256), 0, s, p);
   HCTR_HIP(hipGetLastError());
 }
 
