@@ -36,8 +36,9 @@ template <typename F> __device__ __forceinline__ void with_entry(const Entries &
   else f((const f16_t *)e.values[low], (f16_t *)e.into[low], e.count[low], in);
 }
 
-// f(piece, place, how many of its values are there) for the kLoads pieces of 16 bytes that a thread has of a chunk, all loaded first
-template <bool ONCE, typename T, typename F> __device__ __forceinline__ void pieces_of(const T *values, uint64_t count, uint32_t chunk, F &&f) {
+// f(piece, place, how many of its values are there) for the kLoads pieces of 16 bytes that a thread has of a chunk, all loaded first;
+// meanwhile(): what is done while they are under way
+template <bool ONCE, typename T, typename M, typename F> __device__ __forceinline__ void pieces_of(const T *values, uint64_t count, uint32_t chunk, M &&meanwhile, F &&f) {
   constexpr int V = kVec<T>;
   typedef typename Packed<T, V>::memory Loose;
   const uint64_t base = (uint64_t)chunk * (kChunkBytes / sizeof(T)) + threadIdx.x * V;
@@ -54,6 +55,7 @@ template <bool ONCE, typename T, typename F> __device__ __forceinline__ void pie
         if (at + j < count) v[i][j] = values[at + j];
     }
   }
+  meanwhile();
 #pragma unroll
   for (int i = 0; i < kLoads; i++) {
     const uint64_t at = base + (uint64_t)i * (kBlock * V);
@@ -78,7 +80,7 @@ __global__ __launch_bounds__(kBlock) void sum_squares(Entries e, double *sums) {
   double sum = 0.0;
   for (uint32_t chunk = blockIdx.x; chunk < e.chunks; chunk += gridDim.x)
     with_entry(e, chunk, [&](const auto *values, auto *, uint64_t count, uint32_t in) {
-      pieces_of<false>(values, count, in, [&](const auto &v, uint64_t, uint32_t) {
+      pieces_of<false>(values, count, in, [] {}, [&](const auto &v, uint64_t, uint32_t) {
 #pragma unroll
         for (int j = 0; j < (int)(sizeof(v) / sizeof(*values)); j++) {
           const double d = (double)(float)v[j];
@@ -107,14 +109,22 @@ __global__ __launch_bounds__(kBlock) void finish_norm(const double *sums, uint32
 // The chunks are taken in the other direction than by sum_squares: what was read last is still in the last cache.  The norm is `given`, or
 // `whole`, or made of the sums by every block.
 __global__ __launch_bounds__(kBlock) void scale_gradients(Entries e, const double *sums, uint32_t count, const float *given, const double *whole, float max_norm, float *norm) {
-  const double n = given ? (double)*given : whole ? *whole : total_norm(sums, count);
-  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
-  const bool same = n <= (double)max_norm;
-  const float factor = same ? 1.f : (float)((double)max_norm / n);
+  bool known = false, same = false;
+  float factor = 1.f;
+  // (the block's first values are under way by then)
+  const auto find = [&] {
+    if (known) return;
+    known = true;
+    const double n = given ? (double)*given : whole ? *whole : total_norm(sums, count);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+    same = n <= (double)max_norm;
+    factor = same ? 1.f : (float)((double)max_norm / n);
+  };
   for (uint32_t i = blockIdx.x; i < e.chunks; i += gridDim.x)
     with_entry(e, e.chunks - 1 - i, [&](const auto *values, auto *into, uint64_t total, uint32_t in) {
       if (same && values == into) return;
-      pieces_of<true>(values, total, in, [&](const auto &v, uint64_t at, uint32_t there) {
+      pieces_of<true>(values, total, in, find, [&](const auto &v, uint64_t at, uint32_t there) {
+        if (same && values == into) return;
         typedef std::remove_const_t<std::remove_pointer_t<decltype(into)>> T;
         constexpr int V = kVec<T>;
         Floats<V> f = floats<V>(v);

@@ -57,7 +57,7 @@ template <typename T> __device__ __forceinline__ void finish_gated(const GatedFo
 
 // Both products in one: the rows of the two matrices of weights alternate in a tile, 32 by 32, so that a wave holds the same columns of
 // both, and makes h of them.
-template <typename T, int TILE> __global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kPaired, TILE, TILE>::kThreads), 2)
+template <typename T, int TILE> __global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kPaired, TILE, TILE>::kThreads), (Product<T, Lies::kAlong, Lies::kAlong, Second::kPaired, TILE, TILE>::kWavesEach))
 void gated_product(GatedForward p) {
   typedef Product<T, Lies::kAlong, Lies::kAlong, Second::kPaired, TILE, TILE> P;
   __shared__ __attribute__((aligned(1024))) char tiles[P::kLdsBytes];
@@ -208,7 +208,8 @@ template <typename T> void launch_gated(GatedForward &p, int tile, hipStream_t s
   HCTR_CHECK((uint64_t)p.row_tiles * p.column_tiles * 512 < (1ull << 32), "gated linear: too many tiles");
   const dim3 blocks(p.row_tiles * p.column_tiles, p.splits);
   if (tile == 256) hipLaunchKernelGGL((gated_product<T, 256>), blocks, dim3(512), 0, s, p);
-  else hipLaunchKernelGGL((gated_product<T, 128>), blocks, dim3(256), 0, s, p);
+  else if (tile == 128) hipLaunchKernelGGL((gated_product<T, 128>), blocks, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((gated_product<T, 64>), blocks, dim3(128), 0, s, p);
   HCTR_HIP(hipGetLastError());
   if (p.partial) {
     const uint64_t quads = (uint64_t)p.rows * ((p.hidden + 3) / 4);

@@ -70,11 +70,14 @@ template <typename T, typename A> TakeRows take(const A &a, const float *dloss, 
 }
 Operand taken_rows(const TakeRows &t, size_t size) { return {{(const char *)t.to, nullptr}, (int64_t)(t.to_stride * size), t.rows, 0, 0}; }
 
-// Narrow matrices of 16 bits hold their rows in registers; few rows take the weights past the LDS; others go by tiles.
+// Narrow matrices of 16 bits hold their rows in registers; few rows take the weights past the LDS; others go by tiles, but for those that
+// are few and long: a block for 32 rows shares out k among its waves (us, 35 rows of 8086 columns, 712 items: 67 by tiles, 36 so,
+// float 307 and 72).
 enum class Way { kFew, kNarrow, kTiles };
-Way way_of(size_t rows, size_t width, size_t size) {
+Way way_of(size_t rows, size_t width, size_t items, size_t size) {
   if (size == 2 && width <= kNarrow) return Way::kNarrow;
-  return rows <= kFewRows ? Way::kFew : Way::kTiles;
+  if (rows <= kFewRows) return Way::kFew;
+  return (size_t)div_up(rows, 64) * div_up(items, 64) <= 64 && width * size >= 32 * kStepBytes ? Way::kFew : Way::kTiles;
 }
 
 struct ForwardPlan {
@@ -86,7 +89,7 @@ ForwardPlan plan_of(const hctr_items_args &a) {
   ForwardPlan p = {};
   if (!a.rows) return p;
   const size_t size = size_of(a.dtype);
-  p.way = way_of(a.rows, a.width, size);
+  p.way = way_of(a.rows, a.width, a.items, size);
   if (p.way == Way::kTiles) p.tile = shape_of(a.rows, a.items, a.width, (int)size, false, false).tile;
   p.tiles = p.way == Way::kNarrow ? narrow_ranges(a.rows, a.items, a.width, false) : div_up(a.items, p.tile ? p.tile : 16 * few_groups(a.rows, a.items));
   p.parts = up(p.tiles * a.rows * sizeof(float2), 256);
@@ -151,7 +154,7 @@ struct BackwardPlan {
 BackwardPlan plan_of(const hctr_items_grad_args &a) {
   BackwardPlan p = {};
   const size_t size = size_of(a.dtype), rows = std::max<size_t>(a.rows, 1);
-  p.way = way_of(a.rows, a.width, size);
+  p.way = way_of(a.rows, a.width, a.items, size);
   if (a.rows && p.way == Way::kNarrow) {
     p.rows = rows_space(a.rows, a.width, a.items, size).bytes;
     p.weight = laid_out_bytes(a.weight, a.items, a.width, size);
@@ -176,13 +179,13 @@ BackwardPlan plan_of(const hctr_items_grad_args &a) {
     p.dx = shape_of(a.rows, a.width, some, (int)size, false, true);
     if (p.dx.splits > 1 || p.pieces > 1) p.acc = up(parts_bytes(a.rows, a.width, p.dx.splits), 256);
   }
-  // (the slopes of few rows, too, may come from a matrix that is laid out anew: dx takes it)
+  // (few rows do not need the weights laid out for their slopes, but dx does)
   if (a.rows && (p.tile || a.dx.data)) p.weight = laid_out_bytes(a.weight, some, a.width, size);
   if (a.dweight.data) {
     p.dweight = shape_of(some, a.width, a.rows, (int)size, false, true);
     if (p.dweight.splits > 1) p.parts = up(parts_bytes(some, a.width, p.dweight.splits), 256);
   }
-  if (a.dbias) p.sums = up((p.tile ? div_up(a.rows, p.tile) : 1) * p.d_stride * sizeof(float), 256);
+  if (a.dbias) p.sums = up(div_up(a.rows, p.tile ? p.tile : kFewRows) * p.d_stride * sizeof(float), 256);
   p.bytes = p.rows + p.d + p.acc + p.parts + p.sums + p.weight;
   return p;
 }
@@ -293,6 +296,7 @@ template <typename T> void backward(const hctr_items_grad_args &a) {
 template <typename A> void check(const A &a) {
   check_dtype(a.dtype, "linear cross entropy");
   check_sizes(a.rows, a.width, a.items, ((size_t)1 << 31) - 65536, "linear cross entropy", "there must be 1 to 2^31 - 65536 items");
+  HCTR_CHECK(a.rows <= (1u << 26), "linear cross entropy: too many rows"); // 32 threads each, in a launch
 }
 
 } // namespace

@@ -38,7 +38,7 @@ __device__ __forceinline__ f32x4 slope4(f32x4 sum, f32x4 bias, float lse, float 
 }
 
 template <typename T, int TILE, bool GRADIENT>
-__global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kNone, TILE, TILE>::kThreads), 2) void items_product(ItemsProduct p) {
+__global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kNone, TILE, TILE>::kThreads), (Product<T, Lies::kAlong, Lies::kAlong, Second::kNone, TILE, TILE>::kWavesEach)) void items_product(ItemsProduct p) {
   typedef Product<T, Lies::kAlong, Lies::kAlong, Second::kNone, TILE, TILE> P;
   __shared__ __attribute__((aligned(1024))) char tiles[P::kLdsBytes];
   uint32_t row, column;
@@ -122,8 +122,9 @@ template <typename T, int ROWS, int GROUPS, bool GRADIENT> __global__ __launch_b
   typedef FewRows<T, ROWS, GROUPS> F;
   constexpr uint32_t QUADS = F::kWeights / 4; // of a row
   __shared__ typename F::Sums sums[F::kSums];
-  const uint32_t rows = *p.taken.count, column0 = blockIdx.x * F::kWeights;
-  if (!rows) return;
+  const uint32_t count = *p.taken.count, row0 = blockIdx.y * ROWS, column0 = blockIdx.x * F::kWeights;
+  if (row0 >= count) return;
+  const uint32_t rows = min(count - row0, (uint32_t)ROWS);
   const T *groups[F::kGroups];
   uint32_t left[F::kGroups];
   int64_t stride[F::kGroups];
@@ -134,7 +135,7 @@ template <typename T, int ROWS, int GROUPS, bool GRADIENT> __global__ __launch_b
     stride[j] = p.loose_stride;
     left[j] = p.items - c;
   }
-  F::run((const T *)p.few_x, p.few_stride, rows, groups, left, stride, p.width, sums);
+  F::run((const T *)p.few_x + (uint64_t)row0 * p.few_stride, p.few_stride, rows, groups, left, stride, p.width, sums);
   // four items of a row a thread; the threads of a row are neighbours
   for (uint32_t t = threadIdx.x; t < ROWS * QUADS; t += F::kThreads) {
     const uint32_t r = t / QUADS, c = t % QUADS * 4;
@@ -144,12 +145,12 @@ template <typename T, int ROWS, int GROUPS, bool GRADIENT> __global__ __launch_b
       Tail tail = tail_of(logit);
 #pragma unroll
       for (uint32_t mask = 1; mask < QUADS; mask *= 2) tail = join_lanes(tail, mask);
-      if (c == 0 && r < rows) p.parts[(uint64_t)blockIdx.x * p.rows + r] = make_float2(tail.most, tail.sum);
+      if (c == 0 && r < rows) p.parts[(uint64_t)blockIdx.x * p.rows + row0 + r] = make_float2(tail.most, tail.sum);
     } else {
       f32x4 d = {};
       if (r < rows) {
-        d = slope4(sum, bias, p.taken.lse[r], p.taken.dloss[r] * p.taken.scale[0], p.taken.target[r] - p.first - (column0 + c));
-        if (column0 + c < p.d_stride) write4<T>((T *)p.d + (uint64_t)r * p.d_stride, column0 + c, p.d_stride, d);
+        d = slope4(sum, bias, p.taken.lse[row0 + r], p.taken.dloss[row0 + r] * p.taken.scale[0], p.taken.target[row0 + r] - p.first - (column0 + c));
+        if (column0 + c < p.d_stride) write4<T>((T *)p.d + (uint64_t)(row0 + r) * p.d_stride, column0 + c, p.d_stride, d);
       }
       *(f32x4 *)&sums[0][r][c] = d;
     }
@@ -159,31 +160,32 @@ template <typename T, int ROWS, int GROUPS, bool GRADIENT> __global__ __launch_b
     const uint32_t c = threadIdx.x * 4;
     if (c < F::kWeights && column0 + c < p.d_stride) {
       f32x4 all = {};
-      for (uint32_t i = 0; i < min(rows, (uint32_t)ROWS); i++) all += *(const f32x4 *)&sums[0][i][c];
-      *(f32x4 *)(p.sums + column0 + c) = all;
+      for (uint32_t i = 0; i < rows; i++) all += *(const f32x4 *)&sums[0][i][c];
+      *(f32x4 *)(p.sums + (uint64_t)blockIdx.y * p.d_stride + column0 + c) = all;
     }
   }
 }
 
 template <typename T, bool GRADIENT> void launch_items(ItemsProduct &p, int tile, hipStream_t s) {
   if (!tile) {
-    const auto launch = [&](auto kernel, int groups) {
+    const auto launch = [&](auto kernel, uint32_t rows, int groups) {
       p.column_tiles = div_up(p.items, 16 * groups);
-      hipLaunchKernelGGL(kernel, dim3(p.column_tiles), dim3(FewRows<T, 16, 2>::kThreads), 0, s, p);
+      hipLaunchKernelGGL(kernel, dim3(p.column_tiles, div_up(p.rows, rows)), dim3(FewRows<T, 16, 2>::kThreads), 0, s, p);
     };
     if (few_groups(p.rows, p.items) == 2) {
-      if (p.rows <= 16) launch(items_few<T, 16, 2, GRADIENT>, 2);
-      else launch(items_few<T, 32, 2, GRADIENT>, 2);
+      if (p.rows <= 16) launch(items_few<T, 16, 2, GRADIENT>, 16, 2);
+      else launch(items_few<T, 32, 2, GRADIENT>, 32, 2);
     } else {
-      if (p.rows <= 16) launch(items_few<T, 16, 4, GRADIENT>, 4);
-      else launch(items_few<T, 32, 4, GRADIENT>, 4);
+      if (p.rows <= 16) launch(items_few<T, 16, 4, GRADIENT>, 16, 4);
+      else launch(items_few<T, 32, 4, GRADIENT>, 32, 4);
     }
   } else {
     p.row_tiles = div_up(p.rows, tile), p.column_tiles = div_up(p.items, tile);
     HCTR_CHECK((uint64_t)p.row_tiles * p.column_tiles * 512 < (1ull << 32), "linear cross entropy: too many tiles");
     const dim3 blocks(p.row_tiles * p.column_tiles);
     if (tile == 256) hipLaunchKernelGGL((items_product<T, 256, GRADIENT>), blocks, dim3(512), 0, s, p);
-    else hipLaunchKernelGGL((items_product<T, 128, GRADIENT>), blocks, dim3(256), 0, s, p);
+    else if (tile == 128) hipLaunchKernelGGL((items_product<T, 128, GRADIENT>), blocks, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((items_product<T, 64, GRADIENT>), blocks, dim3(128), 0, s, p);
   }
   HCTR_HIP(hipGetLastError());
 }

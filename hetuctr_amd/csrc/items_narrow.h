@@ -121,7 +121,7 @@ template <typename T, int KS, Narrow MODE> __global__ __launch_bounds__(256, 2) 
   const auto load = [&](uint32_t tile, uint32_t stage) { n.load(other + (int64_t)tile * (N::kThrough * stride), stride, through - tile * N::kThrough, lds + stage * N::kBytes); };
   if (begin < end) load(begin, 0);
   for (uint32_t tile = begin; tile < end; tile++) {
-    tiles_ready();
+    tiles_ready<0>();
     const uint32_t stage = (tile - begin) & 1;
     uint32_t along = lds + stage * N::kBytes + N::along_at(), across = lds + stage * N::kBytes + N::across_at();
     asm("" : "+v"(along), "+v"(across));

@@ -44,15 +44,16 @@ __device__ __forceinline__ i32x4 buffer_at(const char *base) {
   const uint64_t b = (uint64_t)base;
   return i32x4{(int)__builtin_amdgcn_readfirstlane((int)b), (int)(__builtin_amdgcn_readfirstlane((int)(b >> 32)) & 0xffff), (int)kNowhere, 0x20000};
 }
-// everything this wave has under way is there, and so is that of the block's other waves
-__device__ __forceinline__ void tiles_ready() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// All but the last LEFT loads that this wave has under way are there, and so are those of the block's other waves
+template <int LEFT> __device__ __forceinline__ void tiles_ready() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory"); }
 
 // Where 16-byte piece `piece` of line `line` of a tile lies among the line's pieces.  A fragment takes one piece of each of 16 rows
 // (kAlong), or pieces of 16 rows from eight or four lines (kAcross): the order makes them lie in different banks.
-template <typename T, Lies L> __device__ __forceinline__ uint32_t placed(uint32_t line, uint32_t piece) {
+template <typename T, Lies L, int ROWS> __device__ __forceinline__ uint32_t placed(uint32_t line, uint32_t piece) {
   if constexpr (L == Lies::kAlong) return piece ^ (line >> 1 & 7);
-  else if constexpr (sizeof(T) == 2) return piece ^ ((line & 3) << 1 | (line >> 3 & 1) << 3);
-  else return piece ^ ((line >> 2 & 3) << 2);
+  else if constexpr (sizeof(T) == 4) return piece ^ ((line >> 2 & 3) << 2);
+  else if constexpr (ROWS == 64) return piece ^ ((line >> 1 & 1) << 1 | (line >> 3 & 1) << 2); // lines of eight pieces
+  else return piece ^ ((line & 3) << 1 | (line >> 3 & 1) << 3);
 }
 
 // One operand's tiles of ROWS rows, loaded by THREADS threads.
@@ -71,7 +72,7 @@ template <typename T, Lies L, Second S, int ROWS, int THREADS> struct Tiles {
     const uint32_t t = threadIdx.x;
     if constexpr (L == Lies::kAlong) {
       const uint32_t slot = t % 8, line = t / 8;
-      const uint32_t piece = placed<T, L>(line, slot);
+      const uint32_t piece = placed<T, L, ROWS>(line, slot);
       k_of[0] = piece * 16;
       const uint32_t first = S == Second::kPaired ? row0 / 2 : row0;
       base = o.base[0] + (int64_t)first * stride;
@@ -87,7 +88,7 @@ template <typename T, Lies L, Second S, int ROWS, int THREADS> struct Tiles {
       base2 = S == Second::kBehind ? o.base[1] + (int64_t)row0 * sizeof(T) : nullptr;
 #pragma unroll
       for (int i = 0; i < kPasses; i++) {
-        const uint32_t s = i * THREADS + t, line = s / kPieces, piece = placed<T, L>(line, s % kPieces);
+        const uint32_t s = i * THREADS + t, line = s / kPieces, piece = placed<T, L, ROWS>(line, s % kPieces);
         k_of[i] = line;
         offset[i] = row0 + piece * (16 / sizeof(T)) < o.rows ? line * (uint32_t)stride + piece * 16 : kNowhere;
       }
@@ -144,7 +145,7 @@ template <typename T, Lies L, int ROWS> __device__ __forceinline__ Fragment<T> f
   Fragment<T> f;
   if constexpr (L == Lies::kAlong) {
     const uint32_t r = r0 + l % 16;
-    f.v = *(const __attribute__((address_space(3))) typename Fragment<T>::type *)(uintptr_t)(lds + r * kStepBytes + placed<T, L>(r, kk * 4 + l / 16) * 16);
+    f.v = *(const __attribute__((address_space(3))) typename Fragment<T>::type *)(uintptr_t)(lds + r * kStepBytes + placed<T, L, ROWS>(r, kk * 4 + l / 16) * 16);
   } else if constexpr (sizeof(T) == 2) {
     // Lanes 4 i .. 4 i + 3 of each 16 point at the 16 rows of line i, and get four lines of one row each.
     typedef short s4 __attribute__((ext_vector_type(4)));
@@ -153,7 +154,7 @@ template <typename T, Lies L, int ROWS> __device__ __forceinline__ Fragment<T> f
     for (int j = 0; j < 2; j++) {
       const uint32_t line = kk * 32 + l / 16 * 8 + j * 4 + l % 16 / 4;
       const uint32_t row = r0 + l % 4 * 4;
-      const uint32_t at = lds + line * (ROWS * 2) + placed<T, L>(line, row / 8) * 16 + row % 8 * 2;
+      const uint32_t at = lds + line * (ROWS * 2) + placed<T, L, ROWS>(line, row / 8) * 16 + row % 8 * 2;
       h[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(uintptr_t)at);
     }
     f.v = __builtin_bit_cast(typename Fragment<T>::type, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
@@ -161,7 +162,7 @@ template <typename T, Lies L, int ROWS> __device__ __forceinline__ Fragment<T> f
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const uint32_t line = kk * 16 + l / 16 * 4 + j, row = r0 + l % 16;
-      f.v[j] = *(const __attribute__((address_space(3))) float *)(uintptr_t)(lds + line * (ROWS * 4) + placed<T, L>(line, row / 4) * 16 + row % 4 * 4);
+      f.v[j] = *(const __attribute__((address_space(3))) float *)(uintptr_t)(lds + line * (ROWS * 4) + placed<T, L, ROWS>(line, row / 4) * 16 + row % 4 * 4);
     }
   }
   return f;
@@ -182,7 +183,12 @@ template <typename T> __device__ __forceinline__ f32x4 multiply(const Fragment<T
 template <typename T, Lies LA, Lies LB, Second SB, int BM, int BN> struct Product {
   static constexpr int WM = BM / 2, WN = 64, kWaves = 2 * (BN / WN), kThreads = kWaves * kWave;
   static constexpr int kRowTiles = WM / 16, kColumnTiles = WN / 16;
-  static constexpr uint32_t kStageBytes = (BM + BN) * kStepBytes, kLdsBytes = 2 * kStageBytes;
+  // Tiles that LDS holds: the one that is read, and those under way.  Small ones, which are for products that leave a CU little else to do, have
+  // to wait out the memory by themselves (us, loss of 35 rows of 8086 columns and 712 items in bfloat16: 83 with two, 67 with four; its
+  // gradient for 259, 1149 and 3286 in float 177, 126).
+  static constexpr uint32_t kStages = BM == 64 ? 4 : 2;
+  static constexpr int kWavesEach = BM == 64 ? 1 : 2; // of a SIMD, at least
+  static constexpr uint32_t kStageBytes = (BM + BN) * kStepBytes, kLdsBytes = kStages * kStageBytes;
   typedef f32x4 Sums[kRowTiles][kColumnTiles];
 
   static __device__ __forceinline__ uint32_t wave_row() { return threadIdx.x / kWave / (BN / WN) * WM; }
@@ -239,9 +245,13 @@ template <typename T, Lies LA, Lies LB, Second SB, int BM, int BN> struct Produc
       __builtin_amdgcn_sched_group_barrier(0x8, kMultiplies - kReads * (kMultiplies / kReads), 0);
       __builtin_amdgcn_sched_barrier(0);
     };
-    load(k0, 0);
-    tiles_ready();
-    if (k0 + step < k1) load(k0 + step, 1);
+    constexpr int kLoads = Tiles<T, LA, Second::kNone, BM, kThreads>::kPasses + Tiles<T, LB, SB, BN, kThreads>::kPasses;
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < kStages; i++)
+      if (k0 + i * step < k1) load(k0 + i * step, i);
+    if (k0 + (kStages - 2) * step < k1) tiles_ready<(int)(kStages - 2) * kLoads>();
+    else tiles_ready<0>();
+    if (k0 + (kStages - 1) * step < k1) load(k0 + (kStages - 1) * step, kStages - 1);
     read(lds, first);
     uint32_t stage = 0, k = k0;
     for (; k + step < k1; k += step) {
@@ -249,9 +259,11 @@ template <typename T, Lies LA, Lies LB, Second SB, int BM, int BN> struct Produc
       read(lds + stage * kStageBytes, second);
       products(first);
       in_turn();
-      tiles_ready();
-      if (k + 2 * step < k1) load(k + 2 * step, stage);
-      stage ^= 1;
+      // (at the end there are fewer tiles under way)
+      if (kStages > 2 && k + (kStages - 1) * step < k1) tiles_ready<(int)(kStages - 2) * kLoads>();
+      else tiles_ready<0>();
+      if (k + kStages * step < k1) load(k + kStages * step, stage);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
       __builtin_amdgcn_sched_barrier(0);
       read(lds + stage * kStageBytes, first);
       products(second);

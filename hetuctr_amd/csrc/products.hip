@@ -5,21 +5,28 @@
 
 namespace hctr {
 
-// The tile and the number of parts along k that a product should take least time with, in us.  A tile of 256 x 256 has a CU for itself and takes
-// `large` us for a step of 128 bytes of k; of those of 128 x 128 two share a CU, and take `two` us a step together, or `one` alone.  Every
-// tile costs what it takes to begin and to end.  Parts are written and read again as floats, by a launch more.
+// The tile and the number of parts along k that a product should take least time with.  Of each tile up to `most` share a CU, and take
+// us[n - 1] for a step of 128 bytes of k while n of them do; every tile costs what it takes to begin and to end.  Parts are written and
+// read again as floats, by a launch more.
 Shape shape_of(size_t rows, size_t columns, size_t k, int size, bool paired, bool may_split) {
-  const double large = size == 2 ? 1.8 : 7.7, two = size == 2 ? 1.05 : 3.9, one = size == 2 ? 0.8 : 2.0, ends = 4.0;
+  struct Kind {
+    int tile, most;
+    double us[2];
+  };
+  static constexpr Kind kNarrowTypes[] = {{256, 1, {1.8}}, {128, 2, {0.8, 1.05}}, {64, 2, {0.4, 0.5}}};
+  static constexpr Kind kFloats[] = {{256, 1, {7.7}}, {128, 2, {2.0, 3.9}}, {64, 2, {1.0, 1.1}}};
+  const double ends = 4.0;
   const size_t cus = 256, steps = (k * size + kStepBytes - 1) / kStepBytes, wide = paired ? 2 * columns : columns;
   Shape best = {128, 1};
   double least = 1e30;
-  for (int tile : {256, 128}) {
-    const size_t tiles = ((rows + tile - 1) / tile) * ((wide + tile - 1) / tile);
+  for (const Kind &kind : size == 2 ? kNarrowTypes : kFloats) {
+    const size_t tiles = ((rows + kind.tile - 1) / kind.tile) * ((wide + kind.tile - 1) / kind.tile);
     for (uint32_t splits = 1; splits <= (may_split ? 32u : 1u) && (splits == 1 || steps / splits >= 4); splits++) {
       const size_t each = (steps + splits - 1) / splits, turns = (tiles * splits + cus - 1) / cus; // tiles that a CU has to do
-      double t = tile == 256 ? turns * (each * large + ends) : turns / 2 * (each * two + ends) + turns % 2 * (each * one + ends);
+      double t = turns / kind.most * (each * kind.us[kind.most - 1] + ends);
+      if (turns % kind.most) t += each * kind.us[turns % kind.most - 1] + ends;
       if (splits > 1) t += 4.0 + 0.5e-6 * parts_bytes(rows, wide, splits);
-      if (t < least) least = t, best = {tile, splits};
+      if (t < least) least = t, best = {kind.tile, splits};
     }
   }
   return best;

@@ -5,7 +5,7 @@
 namespace hctr {
 
 template <typename T, Lies LA, Lies LB, Second SB, int TILE>
-__global__ __launch_bounds__((Product<T, LA, LB, SB, TILE, TILE>::kThreads), 2) void product(ProductArgs p) {
+__global__ __launch_bounds__((Product<T, LA, LB, SB, TILE, TILE>::kThreads), (Product<T, LA, LB, SB, TILE, TILE>::kWavesEach)) void product(ProductArgs p) {
   typedef Product<T, LA, LB, SB, TILE, TILE> P;
   __shared__ __attribute__((aligned(1024))) char tiles[P::kLdsBytes];
   uint32_t row, column;
@@ -73,7 +73,8 @@ template <typename T, Lies LA, Lies LB, Second SB> void launch_product(ProductAr
   const dim3 blocks(p.row_tiles * p.column_tiles, p.splits);
   HCTR_CHECK((uint64_t)p.row_tiles * p.column_tiles * 512 < (1ull << 32), "product: too many tiles");
   if (tile == 256) hipLaunchKernelGGL((product<T, LA, LB, SB, 256>), blocks, dim3(512), 0, s, p);
-  else hipLaunchKernelGGL((product<T, LA, LB, SB, 128>), blocks, dim3(256), 0, s, p);
+  else if (tile == 128) hipLaunchKernelGGL((product<T, LA, LB, SB, 128>), blocks, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((product<T, LA, LB, SB, 64>), blocks, dim3(128), 0, s, p);
   HCTR_HIP(hipGetLastError());
 }
 template <typename T> void launch_forward_product(ProductArgs &p, int tile, hipStream_t s) {

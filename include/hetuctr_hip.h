@@ -318,7 +318,8 @@ size_t hctr_layer_norm_workspace(size_t rows, size_t width);
  * call says for the same arguments (whose stream and workspace it does not read; pointers it looks at, but does not follow;
  * (size_t)-1 where the call would refuse them for their sizes or types).
  * Products run on the matrix cores: 16-bit values are multiplied exactly, float values as floats; sums are held in 32 bits.
- * Matrices of weights are [columns of the result] x [columns of x], as rows.  rows and items < 2^31 - 65536; width, hidden <= 2^20.
+ * Matrices of weights are [columns of the result] x [columns of x], as rows.  rows and items < 2^31 - 65536 (rows of a
+ * cross entropy <= 2^26); width, hidden <= 2^20.
  *
  * hctr_gated_linear:  gate = x gate_weight^T + gate_bias,  up = x up_weight^T + up_bias,  h = f(gate) * up
  * rows x width times width x hidden, twice; all matrices are of type `dtype`, the biases (`hidden` elements each, NULL: none)

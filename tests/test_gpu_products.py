@@ -205,7 +205,7 @@ def test_reference_gradients_against_differences():
 
 # ---- cross entropy over many items ------------------------------------------------------------------------------------------
 ITEMS = [(1, 1, 1), (1, 16, 2), (1, 128, 1000), (3, 37, 5), (16, 32, 32), (17, 100, 100), (33, 8, 4097), (64, 333, 70), (65, 64, 129), (70, 37, 41),
-         (130, 200, 65), (300, 16, 5000), (257, 1000, 520), (2049, 48, 300), (1111, 39, 1001)]
+         (130, 200, 65), (300, 16, 5000), (257, 1000, 520), (2049, 48, 300), (1111, 39, 1001), (35, 4100, 70), (100, 2056, 300)]
 SHARES = [0.0, 0.3, 0.9]
 
 
@@ -402,6 +402,96 @@ def test_autograd_of_the_cross_entropy(rows, kind):
     torch.testing.assert_close(leaf.grad, same)
 
 
+# ---- far apart in memory ------------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("rows", [3, 70])
+def test_rows_further_apart_than_a_tile_can_count(rows):
+    apart = 2 ** 22 + 8                                            # floats: 16 MiB and a bit
+    space = torch.full((rows, apart), float("nan"), device="cuda")
+    _, near, gw, uw, _, _ = gated_inputs(rows, 40, 24, "f32", "none", 3)
+    x = space[:, 8:48]
+    x.copy_(near)
+    assert torch.equal(nn.gated_linear(x, gw, uw), nn.gated_linear(near, gw, uw))
+    target = torch.arange(rows, device="cuda") % 24
+    loss, lse = nn.linear_cross_entropy(near, gw, target, stats=True)
+    assert torch.equal(nn.linear_cross_entropy(x, gw, target), loss)
+    dloss = torch.ones(rows, device="cuda")
+    for a, b in zip(nn.linear_cross_entropy_backward(dloss, x, gw, target, lse)[:2], nn.linear_cross_entropy_backward(dloss, near, gw, target, lse)):
+        assert torch.equal(a, b)
+    # rows of weights that far apart, and in the other direction
+    weight = torch.full((24, apart), float("nan"), device="cuda")[:, 8:48]
+    weight.copy_(gw)
+    assert torch.equal(nn.gated_linear(near, weight, uw), nn.gated_linear(near, gw, uw))
+    assert torch.equal(nn.linear_cross_entropy(near, weight, target), loss)
+    del space, x, weight
+    torch.cuda.empty_cache()
+
+
+@gpu
+@pytest.mark.parametrize("rows, width, items", [(5, 64, 40_000_003), (40, 256, 9_000_001), (5, 200, 12_000_001)])
+def test_items_beyond_32_bits_of_bytes(rows, width, items):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(1)
+    w = torch.empty((items, width), dtype=torch.bfloat16, device="cuda")
+    for i in range(0, items, 1_000_000):
+        w[i:i + 1_000_000].normal_(0.0, 2 * width ** -0.5, generator=gen)
+    x = values((rows, width), "bf16", 2)
+    target = torch.tensor([items - 1, 0, items // 2, 2 ** 31 // width + 1, items - 2], device="cuda").repeat(rows // 5 + 1)[:rows]
+    loss, lse = nn.linear_cross_entropy(x, w, target, stats=True)
+    # the halves' sums, joined; the targets' logits from their own rows
+    half = items // 2
+    first = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    parts = [nn.linear_cross_entropy(x, part, first, stats=True)[1].double() for part in (w[:half], w[half:])]
+    want = torch.logaddexp(*parts)
+    assert (lse.double() - want).abs().max() < 1e-5
+    hit = (wide(x) * wide(w[target])).sum(1)
+    assert (loss.double() - (want - hit)).abs().max() < 1e-5
+    dloss = values(rows, "f32", 3)
+    dx, dw, _ = nn.linear_cross_entropy_backward(dloss, x, w, target, lse)
+    for at in (slice(0, 500), slice(items - 500, items), slice(2 ** 31 // width - 100, 2 ** 31 // width + 400)):
+        d = torch.exp(wide(x) @ wide(w[at]).T - wide(lse)[:, None])
+        for r in range(rows):
+            if at.start <= target[r] < at.stop:
+                d[r, target[r] - at.start] -= 1
+        d *= wide(dloss)[:, None]
+        got = wide(dw[at])
+        want = d.T @ wide(x)
+        # a rounding of d and one of the result, and what an exponential is off by (40 units), of the sizes
+        assert ((got - want).abs() <= (2 * 2.0 ** -8 + 40 * ref.U) * (d.abs().T @ wide(x).abs()) + 1e-12).all()
+    # dx: the pieces' slopes times the pieces, in 64 bits
+    want, size = torch.zeros((rows, width), dtype=torch.float64, device="cuda"), torch.zeros((rows, width), dtype=torch.float64, device="cuda")
+    for i in range(0, items, 1_000_000):
+        part = wide(w[i:i + 1_000_000])
+        d = torch.exp(wide(x) @ part.T - wide(lse)[:, None])
+        here = (target >= i) & (target < i + part.shape[0])
+        d[here, target[here] - i] -= 1
+        d *= wide(dloss)[:, None]
+        want += d @ part
+        size += d.abs() @ part.abs()
+    # the roundings of so many slopes do not add up all with one sign; that of the sum of n parts in 32 bits is some thousand units
+    assert ((wide(dx) - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 4096 * ref.U) * size).all()
+    del w, dw
+    torch.cuda.empty_cache()
+
+
+@gpu
+def test_a_gated_layer_beyond_32_bits_of_values():
+    rows, width, hidden = 140_001, 16, 16_384
+    x = values((rows, width), "bf16", 1)
+    gw, uw = values((hidden, width), "bf16", 2, 0.3), values((hidden, width), "bf16", 3, 0.3)
+    h, gate, up = nn.gated_linear(x, gw, uw, saved=True)
+    for at in (slice(0, 70), slice(rows - 70, rows), slice(2 ** 31 // hidden - 30, 2 ** 31 // hidden + 40)):
+        want = ref.gated(wide(x[at]), wide(gw), wide(uw), None, None, "silu")
+        for g, (value, slack) in zip((h, gate, up), want):
+            ref.check(g[at], value, slack, "rows from %d" % at.start)
+    dx, dgw, duw, _, _ = nn.gated_linear_backward(h, x, gate, up, gw, uw)
+    for at in (slice(0, 70), slice(rows - 70, rows)):
+        want = ref.gated_gradient(wide(h[at]), wide(x[at]), wide(gate[at]), wide(up[at]), wide(gw), wide(uw), "silu", x.dtype)
+        ref.check(dx[at], *want[0], "dx from %d" % at.start)
+    del h, gate, up
+    torch.cuda.empty_cache()
+
+
 # ---- together -----------------------------------------------------------------------------------------------------------------
 def small_step(x, weights, target, table):
     """Loss, gradients and their norm of one step: a gated layer and its way back, the next item among all, clipped"""
@@ -496,7 +586,7 @@ def test_the_c_entry_points_refuse_what_they_cannot_do():
 
     short = (4096, 7)
     for f, args, match in [
-            (gated, dict(rows=2 ** 31), "rows"), (gated, dict(width=0), "width"), (gated, dict(width=2 ** 20 + 1), "width"), (gated, dict(hidden=0), "hidden"),
+            (gated, dict(rows=2 ** 31), "rows"), (items, dict(rows=2 ** 26 + 1), "rows"), (gated, dict(width=0), "width"), (gated, dict(width=2 ** 20 + 1), "width"), (gated, dict(hidden=0), "hidden"),
             (gated, dict(hidden=2 ** 20 + 1), "hidden"), (gated, dict(types=(3, 0)), "type"), (gated, dict(f=4), "activation"), (gated, dict(f=-1), "activation"),
             (gated, dict(gb=4096, types=(bf16, f16)), "biases"), (gated, dict(x=none), "x: null"), (gated, dict(gw=none), "gate_weight: null"),
             (gated, dict(uw=none), "up_weight: null"), (gated, dict(h=none), "h: null"), (gated, dict(h=short), "h: .*overlap"), (gated, dict(gate=short), "gate: .*overlap"),
@@ -563,3 +653,45 @@ def test_the_functions_refuse_what_does_not_fit():
             f()
     with pytest.raises(TypeError):
         nn.linear_cross_entropy(x, w, target, ignore_index="none")
+
+
+# ---- with a table -------------------------------------------------------------------------------------------------------------
+def the_example():
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "examples", "train_next_item.py")
+    spec = importlib.util.spec_from_file_location("train_next_item", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    return example
+
+
+@gpu
+def test_the_example_runs():
+    example = the_example()
+    said = np.array(example.train(steps=6, samples=300))
+    assert said.shape == (6, 2) and np.isfinite(said).all() and (said > 0).all()
+
+
+@gpu
+def test_gradients_of_the_example():
+    # every gradient of its model against torch's own operators in 64 bits.  On the way to each there are about a dozen roundings to bfloat16, of
+    # values and of their gradients, each at most 2^-8 of what it rounds; in the 2-norm they are allowed all at once
+    example = the_example()
+    torch.manual_seed(1)
+    samples, model = 200, example.Model().cuda()
+    rows = values((samples * example.HISTORY, example.WIDTH), "f32", 1, 0.1).requires_grad_()
+    _, following = example.clicks(samples, np.random.default_rng(1))
+    target = torch.from_numpy(following).cuda()
+    names, leaves = zip(*model.named_parameters())
+    got = torch.autograd.grad(model(rows, samples, target).sum(), (*leaves, rows))
+    wide_leaves = {n: p.detach().double().requires_grad_() for n, p in zip(names, leaves)}
+    r = rows.detach().double().requires_grad_()
+    p = wide_leaves
+    h = torch.nn.functional.layer_norm(r, (example.WIDTH,), p["scale"], p["shift"]).view(samples, -1)
+    h = torch.nn.functional.silu(h @ p["gate"].T) * (h @ p["up"].T)
+    logits = h @ p["down"].T @ p["items"].T + p["popular"]
+    loss = torch.nn.functional.cross_entropy(logits, target, ignore_index=-100, reduction="sum")
+    want = torch.autograd.grad(loss, (*[p[n] for n in names], r))
+    for name, a, b in zip((*names, "rows"), got, want):
+        assert (a.double() - b).norm() <= 12 * 2.0 ** -8 * b.norm(), name
