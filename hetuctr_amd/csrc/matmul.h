@@ -178,6 +178,31 @@ template <typename T> __device__ __forceinline__ f32x4 multiply(const Fragment<T
   return c;
 }
 
+// A float is the sum of three bfloat16: the one nearest to it, the one nearest to what is left, and what is then left, which has eight bits at
+// most.  Of the nine products of two such sums the six largest are made; the others are below 2^-25 of the floats' product together.
+// They take six times a sixteenth of the matrix cores' time for floats, and five or six instructions for each float.  us, 8192 x 8192 x 2048 in
+// the three layouts: 2095, 2043 and 2098 with products of floats (131 to 135 TFLOP/s, of the 157 that the cores could do at most), 1573,
+// 1466 and 1476 so.  An infinity becomes a NaN on the way, a float below 2^-110 loses some of its bits, one beyond 2^128 - 2^119 is as
+// good as infinite.
+struct Split {
+  Fragment<bf16_t> part[3];
+};
+__device__ __forceinline__ Split split(const Fragment<float> &a, const Fragment<float> &b) {
+  Split s;
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = a.v[e], v[e + 4] = b.v[e];
+#pragma unroll
+  for (int p = 0; p < 3; p++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const bf16_t x = (bf16_t)v[e];
+      s.part[p].v[e] = x;
+      v[e] -= (float)x;
+    }
+  return s;
+}
+
 // The product of tiles: BM rows of a times BN rows of b, by waves of WM x WN each.  sum[i][j][e]: row i * 16 + lane % 16 of the wave's WM of a,
 // row j * 16 + lane / 16 * 4 + e of its WN of b: four neighbouring columns of the result in a lane.
 template <typename T, Lies LA, Lies LB, Second SB, int BM, int BN> struct Product {
@@ -194,6 +219,44 @@ template <typename T, Lies LA, Lies LB, Second SB, int BM, int BN> struct Produc
   static __device__ __forceinline__ uint32_t wave_row() { return threadIdx.x / kWave / (BN / WN) * WM; }
   static __device__ __forceinline__ uint32_t wave_column() { return threadIdx.x / kWave % (BN / WN) * WN; }
 
+  // The same for floats, in parts: a step's fragments of b are split, then those of a, 16 rows at a time, while the ones before are multiplied.
+  template <typename TA, typename TB>
+  static __device__ __forceinline__ void run_floats(const TA &ta, const TB &tb, uint32_t k0, uint32_t k1, uint32_t lds, Sums &sum) {
+    constexpr uint32_t step = kStep<T>;
+    constexpr int kLoads = TA::kPasses + TB::kPasses;
+    const auto load = [&](uint32_t k, uint32_t stage) {
+      ta.load(k, k1 - k, lds + stage * kStageBytes);
+      tb.load(k, k1 - k, lds + stage * kStageBytes + BM * kStepBytes);
+    };
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < kStages; i++)
+      if (k0 + i * step < k1) load(k0 + i * step, i);
+    uint32_t stage = 0;
+    for (uint32_t k = k0; k < k1; k += step) {
+      if (kStages > 2 && k + (kStages - 2) * step < k1) tiles_ready<(int)(kStages - 2) * kLoads>();
+      else tiles_ready<0>();
+      // (everyone has read the tile before this one)
+      if (k + (kStages - 1) * step < k1) load(k + (kStages - 1) * step, stage ? stage - 1 : kStages - 1);
+      const uint32_t here = lds + stage * kStageBytes;
+      Split b[kColumnTiles];
+#pragma unroll
+      for (int j = 0; j < kColumnTiles; j++)
+        b[j] = split(fragment<T, LB, BN>(here + BM * kStepBytes, wave_column() + j * 16, 0), fragment<T, LB, BN>(here + BM * kStepBytes, wave_column() + j * 16, 1));
+#pragma unroll
+      for (int i = 0; i < kRowTiles; i++) {
+        const Split a = split(fragment<T, LA, BM>(here, wave_row() + i * 16, 0), fragment<T, LA, BM>(here, wave_row() + i * 16, 1));
+        // the smallest first
+#pragma unroll
+        for (int both = 2; both >= 0; both--)
+#pragma unroll
+          for (int p = 0; p <= both; p++)
+#pragma unroll
+            for (int j = 0; j < kColumnTiles; j++) sum[i][j] = multiply<bf16_t>(b[j].part[both - p], a.part[p], sum[i][j]);
+      }
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+  }
+
   // k from k0 (a multiple of kStep) to k1
   static __device__ __forceinline__ void run(const Operand &a, const Operand &b, uint32_t row0, uint32_t column0, uint32_t k0, uint32_t k1,
                                              uint32_t lds, Sums &sum) {
@@ -207,6 +270,8 @@ template <typename T, Lies LA, Lies LB, Second SB, int BM, int BN> struct Produc
 #pragma unroll
       for (int j = 0; j < kColumnTiles; j++) sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (k0 >= k1) return;
+    // (a small tile would split each value too often: 8192 x 8192 x 2048 in 2774 us instead of 2315)
+    if constexpr (sizeof(T) == 4 && BM > 64) return run_floats(ta, tb, k0, k1, lds, sum);
     const auto load = [&](uint32_t k, uint32_t stage) {
       ta.load(k, k1 - k, lds + stage * kStageBytes);
       tb.load(k, k1 - k, lds + stage * kStageBytes + BM * kStepBytes);

@@ -14,7 +14,7 @@ Shape shape_of(size_t rows, size_t columns, size_t k, int size, bool paired, boo
     double us[2];
   };
   static constexpr Kind kNarrowTypes[] = {{256, 1, {1.8}}, {128, 2, {0.8, 1.05}}, {64, 2, {0.4, 0.5}}};
-  static constexpr Kind kFloats[] = {{256, 1, {7.7}}, {128, 2, {2.0, 3.9}}, {64, 2, {1.0, 1.1}}};
+  static constexpr Kind kFloats[] = {{256, 1, {5.9}}, {128, 2, {1.95, 3.2}}, {64, 2, {1.15, 1.25}}};
   const double ends = 4.0;
   const size_t cus = 256, steps = (k * size + kStepBytes - 1) / kStepBytes, wide = paired ? 2 * columns : columns;
   Shape best = {128, 1};
