@@ -1,5 +1,7 @@
 // The kernels of items.h for one type; items_*.hip build them side by side.
 #pragma once
+#include <algorithm>
+
 #include "few_rows.h"
 #include "items.h"
 #include "items_tail.h"
@@ -42,7 +44,8 @@ __global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kNo
   typedef Product<T, Lies::kAlong, Lies::kAlong, Second::kNone, TILE, TILE> P;
   __shared__ __attribute__((aligned(1024))) char tiles[P::kLdsBytes];
   uint32_t row, column;
-  tile_of(blockIdx.x, gridDim.x, p.row_tiles, p.column_tiles, p.band, row, column);
+  tile_of(blockIdx.x, gridDim.x, p.row_tiles, p.columns_here, p.band, row, column);
+  column += p.column_from;
   const uint32_t rows = *p.taken.count, row0 = row * TILE, column0 = column * TILE;
   if (row0 >= rows) return;
   typename P::Sums sum;
@@ -181,11 +184,16 @@ template <typename T, bool GRADIENT> void launch_items(ItemsProduct &p, int tile
     }
   } else {
     p.row_tiles = div_up(p.rows, tile), p.column_tiles = div_up(p.items, tile);
-    HCTR_CHECK((uint64_t)p.row_tiles * p.column_tiles * 512 < (1ull << 32), "linear cross entropy: too many tiles");
-    const dim3 blocks(p.row_tiles * p.column_tiles);
-    if (tile == 256) hipLaunchKernelGGL((items_product<T, 256, GRADIENT>), blocks, dim3(512), 0, s, p);
-    else if (tile == 128) hipLaunchKernelGGL((items_product<T, 128, GRADIENT>), blocks, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((items_product<T, 64, GRADIENT>), blocks, dim3(128), 0, s, p);
+    // (a launch has fewer than 2^32 threads; a million rows and a million items are more)
+    const uint32_t most = std::max<uint32_t>(1, ((1u << 23) - 1) / p.row_tiles);
+    for (p.column_from = 0; p.column_from < p.column_tiles; p.column_from += p.columns_here) {
+      p.columns_here = std::min(p.column_tiles - p.column_from, most);
+      const dim3 blocks(p.row_tiles * p.columns_here);
+      if (tile == 256) hipLaunchKernelGGL((items_product<T, 256, GRADIENT>), blocks, dim3(512), 0, s, p);
+      else if (tile == 128) hipLaunchKernelGGL((items_product<T, 128, GRADIENT>), blocks, dim3(256), 0, s, p);
+      else hipLaunchKernelGGL((items_product<T, 64, GRADIENT>), blocks, dim3(128), 0, s, p);
+      HCTR_HIP(hipGetLastError());
+    }
   }
   HCTR_HIP(hipGetLastError());
 }

@@ -475,6 +475,24 @@ def test_items_beyond_32_bits_of_bytes(rows, width, items):
 
 
 @gpu
+def test_more_tiles_than_a_launch_has():
+    rows, width, items = 300_000, 136, 8_000_000
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(1)
+    w = torch.empty((items, width), dtype=torch.bfloat16, device="cuda")
+    for i in range(0, items, 1_000_000):
+        w[i:i + 1_000_000].normal_(0.0, 2 * width ** -0.5, generator=gen)
+    x = torch.empty((rows, width), device="cuda").normal_(0.0, 1.0, generator=gen).bfloat16()
+    target = torch.randint(0, items, (rows,), device="cuda", generator=gen)
+    loss = nn.linear_cross_entropy(x, w, target)
+    for at in (slice(0, 32), slice(rows // 2, rows // 2 + 32), slice(rows - 32, rows)):
+        torch.testing.assert_close(loss[at], nn.linear_cross_entropy(x[at], w, target[at]), rtol=2e-6, atol=2e-5)
+    assert loss.isfinite().all()
+    del w, x
+    torch.cuda.empty_cache()
+
+
+@gpu
 def test_a_gated_layer_beyond_32_bits_of_values():
     rows, width, hidden = 140_001, 16, 16_384
     x = values((rows, width), "bf16", 1)
