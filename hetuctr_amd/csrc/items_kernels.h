@@ -43,11 +43,13 @@ template <typename T, int TILE, bool GRADIENT>
 __global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kNone, TILE, TILE>::kThreads), (Product<T, Lies::kAlong, Lies::kAlong, Second::kNone, TILE, TILE>::kWavesEach)) void items_product(ItemsProduct p) {
   typedef Product<T, Lies::kAlong, Lies::kAlong, Second::kNone, TILE, TILE> P;
   __shared__ __attribute__((aligned(1024))) char tiles[P::kLdsBytes];
+  // (the tiles of rows that are there are shared out among the XCDs, not those of all rows)
+  const uint32_t rows = *p.taken.count, row_tiles = (rows + TILE - 1) / TILE, live = row_tiles * p.columns_here;
+  if (blockIdx.x >= live) return;
   uint32_t row, column;
-  tile_of(blockIdx.x, gridDim.x, p.row_tiles, p.columns_here, p.band, row, column);
+  tile_of(blockIdx.x, live, row_tiles, p.columns_here, p.band, row, column);
   column += p.column_from;
-  const uint32_t rows = *p.taken.count, row0 = row * TILE, column0 = column * TILE;
-  if (row0 >= rows) return;
+  const uint32_t row0 = row * TILE, column0 = column * TILE;
   typename P::Sums sum;
   P::run(p.x, p.weight, row0, column0, 0, p.width, (uint32_t)(uintptr_t)(lds_char *)tiles, sum);
   const uint32_t l = lane_id(), wave_column = P::wave_column();

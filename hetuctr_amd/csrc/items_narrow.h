@@ -77,11 +77,12 @@ template <typename T, int KS, Narrow MODE> __global__ __launch_bounds__(256, 2) 
   __shared__ __attribute__((aligned(1024))) char tiles[2 * N::kBytes];
   const uint32_t lds = (uint32_t)(uintptr_t)(lds_char *)tiles, l = lane_id(), wave = threadIdx.x / kWave;
   const uint32_t count = min(p.rows, *p.taken.count);
-  uint32_t owner, range;
-  tile_of(blockIdx.x, gridDim.x, p.owners, p.ranges, p.owners, owner, range);
   const uint32_t owned = WEIGHT ? p.items : count, through = WEIGHT ? count : p.items;
+  const uint32_t owners = (owned + OI * 64 - 1) / (OI * 64), live = owners * p.ranges;
+  if (blockIdx.x >= live) return;
+  uint32_t owner, range;
+  tile_of(blockIdx.x, live, owners, p.ranges, owners, owner, range);
   const uint32_t first = owner * (OI * 64) + wave * (OI * 16);
-  if (owner * (OI * 64) >= owned) return;
   const char *own = WEIGHT ? p.weight : p.x, *other = WEIGHT ? p.x : p.weight;
   const int64_t own_stride = WEIGHT ? p.weight_stride : p.x_stride, stride = WEIGHT ? p.x_stride : p.weight_stride;
 
