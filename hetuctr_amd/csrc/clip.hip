@@ -8,8 +8,12 @@
 namespace hctr {
 namespace {
 
-constexpr int kBlock = 256, kLoads = 8;
-constexpr uint32_t kChunkBytes = kBlock * 16 * kLoads; // of one gradient, that a block takes at a time
+constexpr int kBlock = 256;
+// Pieces of 16 bytes that a thread has under way: a block takes a chunk of LOADS * 4 KiB of one gradient at a time.  Eight where there are few
+// chunks, whose blocks make the norm for themselves as well, four where there are many (us, 28.8 MB in 17 gradients 17.9 with eight, 20.8
+// with four; 4.1 GB 2130 and 2031).
+constexpr uint64_t chunk_bytes(int loads) { return (uint64_t)kBlock * 16 * loads; }
+constexpr int kFewLoads = 8, kManyLoads = 4;
 // Blocks of a call in all, which stay: each leaves one sum, and every block that scales adds them all up for itself, in the same order.
 constexpr uint32_t kMostBlocks = 2048;
 constexpr int kMostEntries = 128; // gradients that the arguments of one launch name
@@ -36,15 +40,15 @@ template <typename F> __device__ __forceinline__ void with_entry(const Entries &
   else f((const f16_t *)e.values[low], (f16_t *)e.into[low], e.count[low], in);
 }
 
-// f(piece, place, how many of its values are there) for the kLoads pieces of 16 bytes that a thread has of a chunk, all loaded first;
+// f(piece, place, how many of its values are there) for the LOADS pieces of 16 bytes that a thread has of a chunk, all loaded first;
 // meanwhile(): what is done while they are under way
-template <bool ONCE, typename T, typename M, typename F> __device__ __forceinline__ void pieces_of(const T *values, uint64_t count, uint32_t chunk, M &&meanwhile, F &&f) {
+template <int LOADS, bool ONCE, typename T, typename M, typename F> __device__ __forceinline__ void pieces_of(const T *values, uint64_t count, uint32_t chunk, M &&meanwhile, F &&f) {
   constexpr int V = kVec<T>;
   typedef typename Packed<T, V>::memory Loose;
-  const uint64_t base = (uint64_t)chunk * (kChunkBytes / sizeof(T)) + threadIdx.x * V;
-  typename Packed<T, V>::type v[kLoads];
+  const uint64_t base = (uint64_t)chunk * (chunk_bytes(LOADS) / sizeof(T)) + threadIdx.x * V;
+  typename Packed<T, V>::type v[LOADS];
 #pragma unroll
-  for (int i = 0; i < kLoads; i++) {
+  for (int i = 0; i < LOADS; i++) {
     const uint64_t at = base + (uint64_t)i * (kBlock * V);
     v[i] = (T)0;
     if (at + V <= count) {
@@ -57,7 +61,7 @@ template <bool ONCE, typename T, typename M, typename F> __device__ __forceinlin
   }
   meanwhile();
 #pragma unroll
-  for (int i = 0; i < kLoads; i++) {
+  for (int i = 0; i < LOADS; i++) {
     const uint64_t at = base + (uint64_t)i * (kBlock * V);
     if (at < count) f(v[i], at, at + V <= count ? (uint32_t)V : (uint32_t)(count - at));
   }
@@ -76,11 +80,11 @@ __device__ __forceinline__ double block_total(double v) {
   return v;
 }
 
-__global__ __launch_bounds__(kBlock) void sum_squares(Entries e, double *sums) {
+template <int LOADS> __global__ __launch_bounds__(kBlock) void sum_squares(Entries e, double *sums) {
   double sum = 0.0;
   for (uint32_t chunk = blockIdx.x; chunk < e.chunks; chunk += gridDim.x)
     with_entry(e, chunk, [&](const auto *values, auto *, uint64_t count, uint32_t in) {
-      pieces_of<false>(values, count, in, [] {}, [&](const auto &v, uint64_t, uint32_t) {
+      pieces_of<LOADS, false>(values, count, in, [] {}, [&](const auto &v, uint64_t, uint32_t) {
 #pragma unroll
         for (int j = 0; j < (int)(sizeof(v) / sizeof(*values)); j++) {
           const double d = (double)(float)v[j];
@@ -108,7 +112,7 @@ __global__ __launch_bounds__(kBlock) void finish_norm(const double *sums, uint32
 
 // The chunks are taken in the other direction than by sum_squares: what was read last is still in the last cache.  The norm is `given`, or
 // `whole`, or made of the sums by every block.
-__global__ __launch_bounds__(kBlock) void scale_gradients(Entries e, const double *sums, uint32_t count, const float *given, const double *whole, float max_norm, float *norm) {
+template <int LOADS> __global__ __launch_bounds__(kBlock) void scale_gradients(Entries e, const double *sums, uint32_t count, const float *given, const double *whole, float max_norm, float *norm) {
   bool known = false, same = false;
   float factor = 1.f;
   // (the block's first values are under way by then)
@@ -123,7 +127,7 @@ __global__ __launch_bounds__(kBlock) void scale_gradients(Entries e, const doubl
   for (uint32_t i = blockIdx.x; i < e.chunks; i += gridDim.x)
     with_entry(e, e.chunks - 1 - i, [&](const auto *values, auto *into, uint64_t total, uint32_t in) {
       if (same && values == into) return;
-      pieces_of<true>(values, total, in, find, [&](const auto &v, uint64_t at, uint32_t there) {
+      pieces_of<LOADS, true>(values, total, in, find, [&](const auto &v, uint64_t at, uint32_t there) {
         if (same && values == into) return;
         typedef std::remove_const_t<std::remove_pointer_t<decltype(into)>> T;
         constexpr int V = kVec<T>;
@@ -143,16 +147,24 @@ __global__ __launch_bounds__(kBlock) void scale_gradients(Entries e, const doubl
     });
 }
 
-uint64_t chunks_of(const hctr_gradient &g) { return (g.count * size_of(g.dtype) + kChunkBytes - 1) / kChunkBytes; }
+bool many(const hctr_clip_args &a) {
+  uint64_t bytes = 0;
+  for (size_t i = 0; i < a.count; i++) bytes += a.gradients[i].count * size_of(a.gradients[i].dtype);
+  return bytes > 4 * kMostBlocks * chunk_bytes(kFewLoads);
+}
+uint64_t chunks_of(const hctr_gradient &g, bool many) {
+  const uint64_t each = chunk_bytes(many ? kManyLoads : kFewLoads);
+  return (g.count * size_of(g.dtype) + each - 1) / each;
+}
 
 // Launches: of up to kMostEntries gradients and 2^31 chunks each
-template <typename F> void in_launches(const hctr_clip_args &a, F &&f) {
+template <typename F> void in_launches(const hctr_clip_args &a, bool many, F &&f) {
   Entries e;
   e.entries = e.chunks = 0;
   for (size_t i = 0; i < a.count; i++) {
     const hctr_gradient &g = a.gradients[i];
     if (!g.count) continue;
-    const uint64_t chunks = chunks_of(g);
+    const uint64_t chunks = chunks_of(g, many);
     if (e.entries == kMostEntries || (e.entries && e.chunks + chunks >= (1u << 31))) {
       f(e);
       e.entries = e.chunks = 0;
@@ -163,12 +175,12 @@ template <typename F> void in_launches(const hctr_clip_args &a, F &&f) {
   }
   if (e.entries) f(e);
 }
-size_t launches_of(const hctr_clip_args &a) {
+size_t launches_of(const hctr_clip_args &a, bool many) {
   size_t n = 0, entries = 0;
   uint64_t chunks = 0;
   for (size_t i = 0; i < a.count; i++) {
     if (!a.gradients[i].count) continue;
-    const uint64_t more = chunks_of(a.gradients[i]);
+    const uint64_t more = chunks_of(a.gradients[i], many);
     if (entries == kMostEntries || (entries && chunks + more >= (1u << 31))) n++, entries = 0, chunks = 0;
     entries++, chunks += more;
   }
@@ -216,7 +228,8 @@ void check_places(const hctr_clip_args &a) {
 
 size_t gradient_workspace(const hctr_clip_args &a) {
   check(a);
-  return (launches_of(a) * most_blocks(launches_of(a)) + 1) * sizeof(double); // the sums, and the norm
+  const size_t launches = launches_of(a, many(a));
+  return (launches * most_blocks(launches) + 1) * sizeof(double); // the sums, and the norm
 }
 
 void gradient_norm(const hctr_clip_args &a, bool clip) {
@@ -226,7 +239,8 @@ void gradient_norm(const hctr_clip_args &a, bool clip) {
   if (clip) check_places(a);
   else
     for (size_t i = 0; i < a.count; i++) HCTR_CHECK(!a.gradients[i].count || a.gradients[i].values, "gradient norm: null pointer");
-  const size_t launches = launches_of(a);
+  const bool much = many(a);
+  const size_t launches = launches_of(a, much);
   const bool sums_wanted = !clip || !a.given;
   if (sums_wanted) check_space(a.workspace, a.workspace_bytes, gradient_workspace(a), "clip gradients");
   const hipStream_t s = (hipStream_t)a.stream;
@@ -234,28 +248,30 @@ void gradient_norm(const hctr_clip_args &a, bool clip) {
   double *sums = (double *)a.workspace;
   uint32_t count = 0;
   if (sums_wanted)
-    in_launches(a, [&](const Entries &e) {
+    in_launches(a, much, [&](const Entries &e) {
       const uint32_t blocks = std::min(e.chunks, most);
-      hipLaunchKernelGGL(sum_squares, dim3(blocks), dim3(kBlock), 0, s, e, sums + count);
+      if (much) hipLaunchKernelGGL((sum_squares<kManyLoads>), dim3(blocks), dim3(kBlock), 0, s, e, sums + count);
+      else hipLaunchKernelGGL((sum_squares<kFewLoads>), dim3(blocks), dim3(kBlock), 0, s, e, sums + count);
       HCTR_HIP(hipGetLastError());
       count += blocks;
     });
   float *norm = a.norm == a.given ? nullptr : a.norm;
-  uint64_t chunks = 0;
-  for (size_t i = 0; i < a.count; i++) chunks += chunks_of(a.gradients[i]);
-  // Few chunks: the blocks that scale make the norm themselves, a launch less (28.8 MB in 17 gradients: FEW us, with three launches MANY).  Many:
-  // a block for each, without that work, moves more at a time than blocks that stay (4.1 GB: 1787 us, ONE EACH).
-  const bool many = chunks > 4 * kMostBlocks;
-  double *whole = clip && many && !a.given ? sums + launches * most : nullptr;
-  if (!clip || !launches || whole) {
-    if (norm || whole) hipLaunchKernelGGL(finish_norm, dim3(1), dim3(kBlock), 0, s, (const double *)sums, count, clip ? a.given : nullptr, norm, whole);
+  // Few chunks: the blocks that scale make the norm themselves, a launch less (28.8 MB in 17 gradients: 17.9 us, with three launches 20.6).  Many:
+  // a block for each, without that work, moves more at a time than blocks that stay (4.1 GB: 1787 us for blocks that stay, 1445).
+  double *whole = clip && much && !a.given ? sums + launches * most : nullptr;
+  if ((norm || whole) && (!clip || !launches || whole)) {
+    hipLaunchKernelGGL(finish_norm, dim3(1), dim3(kBlock), 0, s, (const double *)sums, count, clip ? a.given : nullptr, norm, whole);
     HCTR_HIP(hipGetLastError());
     if (whole) norm = nullptr;
   }
   if (!clip) return;
-  in_launches(a, [&](const Entries &e) {
-    const uint32_t blocks = many ? std::min(e.chunks, 1u << 23) : std::min(e.chunks, kMostBlocks);
-    hipLaunchKernelGGL(scale_gradients, dim3(blocks), dim3(kBlock), 0, s, e, (const double *)sums, count, a.given, (const double *)whole, a.max_norm, norm);
+  in_launches(a, much, [&](const Entries &e) {
+    if (much)
+      hipLaunchKernelGGL((scale_gradients<kManyLoads>), dim3(std::min(e.chunks, 1u << 23)), dim3(kBlock), 0, s, e, (const double *)sums, count, a.given, (const double *)whole,
+                         a.max_norm, norm);
+    else
+      hipLaunchKernelGGL((scale_gradients<kFewLoads>), dim3(std::min(e.chunks, kMostBlocks)), dim3(kBlock), 0, s, e, (const double *)sums, count, a.given, (const double *)whole,
+                         a.max_norm, norm);
     HCTR_HIP(hipGetLastError());
     norm = nullptr;
   });
