@@ -56,7 +56,9 @@ template <typename T> __device__ __forceinline__ void finish_gated(const GatedFo
 }
 
 // Both products in one: the rows of the two matrices of weights alternate in a tile, 32 by 32, so that a wave holds the same columns of
-// both, and makes h of them.
+// both, and makes h of them.  Bound by the matrix cores, at the clock that their power leaves (51 % of the cycles), and by the ends of tiles, which
+// nothing overlaps where a tile has the CU for itself: 8192 rows, 4096 x 16384 twice in bfloat16 1948 us with three results (1.13 PFLOP/s);
+// with h alone about 100 less.
 template <typename T, int TILE> __global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kPaired, TILE, TILE>::kThreads), (Product<T, Lies::kAlong, Lies::kAlong, Second::kPaired, TILE, TILE>::kWavesEach))
 void gated_product(GatedForward p) {
   typedef Product<T, Lies::kAlong, Lies::kAlong, Second::kPaired, TILE, TILE> P;
@@ -159,7 +161,9 @@ template <typename T, int ROWS, int GROUPS> __global__ __launch_bounds__((FewRow
   }
 }
 
-// dgate and dup of columns c .. c + V - 1 of a block's rows, and the sums over them.  Eight threads share out the rows of 32 pieces.
+// dgate and dup of columns c .. c + V - 1 of a block's rows, and the sums over them.  Eight threads share out the rows of 32 pieces.  Bound by
+// memory and, nearly as much, by the activation's arithmetic (86 % of the vector units' cycles with an exact exponential and quotient):
+// 8192 x 16384 in bfloat16, three matrices read and two written, 222 us, 6.0 TB/s.
 template <typename T, bool SUMS> __global__ __launch_bounds__(256) void gated_slopes(GatedSlopes p) {
   constexpr int V = kVec<T>, LANES = 32, GROUPS = 8;
   __shared__ float joined[SUMS ? GROUPS : 1][2][LANES * V];
