@@ -171,6 +171,9 @@ def test_memory_that_runs_out():
     w = values((4096, 1024), 2)
     with pytest.raises(torch.OutOfMemoryError):
         nn.gated_linear(x, w, w)
+    target = torch.zeros(1, dtype=torch.int64, device="cuda")
+    with pytest.raises(RuntimeError, match="too many rows"):
+        nn.linear_cross_entropy(x, w, target.expand(2 ** 30))
     with pytest.raises(torch.OutOfMemoryError):
-        nn.linear_cross_entropy(x, w, torch.zeros(1, dtype=torch.int64, device="cuda").expand(2 ** 30))
+        nn.linear_cross_entropy(values((1, 8192), 3).expand(2 ** 26, 8192), values((16, 8192), 4), target.expand(2 ** 26))     # 2 TiB
     assert nn.gated_linear(x[:3], w, w).isfinite().all()
