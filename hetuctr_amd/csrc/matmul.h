@@ -36,7 +36,8 @@ constexpr uint32_t kNowhere = 0x80000000u; // an offset behind every buffer: the
 template <typename T> constexpr int kStep = kStepBytes / (int)sizeof(T); // of k that a tile holds
 
 // 16 bytes per lane from base + offset to LDS, where a wave's lanes lie one behind the other from `lds`, the same address in all
-// lanes.  Not the builtin: the compiler would wait for every such load before any read of LDS.
+// lanes.  Not the builtin: the compiler would wait for every such load before any read of LDS.  (m0 is the compiler's own, which sets it right
+// before each use and keeps nothing there.)
 __device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t offset, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc) : "memory");
 }

@@ -277,6 +277,9 @@ def test_cross_entropy_of_any_layout(rows, kind):
         assert nn.linear_cross_entropy(x[:0], w, target[:0], b).shape == (0,)
         zero = nn.linear_cross_entropy_backward(dloss[:0], x[:0], w, target[:0], lse[:0], b)
         assert zero[0].shape == (0, width) and (zero[1] == 0).all() and (zero[2] == 0).all()
+        # one row, without a dimension for rows
+        one = nn.linear_cross_entropy(x[0], w, target[1], b, stats=True)
+        assert one[0].shape == () and nn.linear_cross_entropy_backward(dloss[0], x[0], w, target[1], one[1], b)[0].shape == (width,)
         # nothing takes part
         none = torch.full_like(target, -100)
         loss, lse = nn.linear_cross_entropy(x * float("nan"), w, none, b, stats=True)
@@ -522,18 +525,18 @@ def small_step(x, weights, target, table):
     return (loss.detach(), norm, *grads)
 
 
-def step_inputs(seed, rows=80):
+def step_inputs(seed, rows=80, width=32):
     gen = torch.Generator().manual_seed(seed)
     make = lambda *s: (torch.randn(*s, generator=gen) / s[-1] ** 0.5).bfloat16().cuda()
     target = torch.randint(0, 500, (rows,), generator=gen)
     target[::7] = -100
-    return make(rows, 32) * 5, [make(64, 32), make(64, 32), make(64, 32)], target.cuda(), make(500, 32)
+    return make(rows, width) * 5, [make(64, width), make(64, width), make(64, width)], target.cuda(), make(500, width)
 
 
 @gpu
-@pytest.mark.parametrize("rows", [40, 300])
-def test_steps_in_graphs_and_on_streams(rows):
-    x, weights, target, table = step_inputs(1, rows)
+@pytest.mark.parametrize("rows, width", [(40, 32), (300, 32), (20, 200), (300, 200), (40, 2048)])
+def test_steps_in_graphs_and_on_streams(rows, width):
+    x, weights, target, table = step_inputs(1, rows, width)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -543,7 +546,7 @@ def test_steps_in_graphs_and_on_streams(rows):
     with torch.cuda.graph(graph):
         outs = small_step(x, weights, target, table)
     for i in range(4):
-        new = step_inputs(10 + i, rows)
+        new = step_inputs(10 + i, rows, width)
         for to, t in zip((x, *weights, target, table), (new[0], *new[1], new[2], new[3])):
             to.copy_(t)
         graph.replay()
@@ -560,8 +563,9 @@ def test_steps_in_graphs_and_on_streams(rows):
 
 
 @gpu
-def test_two_graphs_do_not_share_what_they_work_in():
-    first, second = step_inputs(1, 300), step_inputs(2, 300)
+@pytest.mark.parametrize("width", [32, 200])
+def test_two_graphs_do_not_share_what_they_work_in(width):
+    first, second = step_inputs(1, 300, width), step_inputs(2, 300, width)
     small_step(*first)
     graphs, outs = [], []
     for given in (first, second):
