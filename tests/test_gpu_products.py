@@ -73,6 +73,27 @@ def test_gated_linear_gradient(rows, width, hidden, kind):
                 ref.check(g, value, slack, what + " " + f)
 
 
+# Sizes for which the larger tiles are chosen (128, 256), whole and in parts, with ends inside a tile in every direction
+MANY_GATED = [(4100, 2050, 1030), (5003, 300, 1001), (3000, 4100, 516), (9001, 130, 2050), (2500, 1030, 3070), (20000, 100, 300)]
+
+
+@gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows, width, hidden", MANY_GATED)
+def test_gated_linear_of_many_rows(rows, width, hidden, kind):
+    f = ACTIVATIONS[rows % 4]
+    dh, x, gw, uw, gb, ub = gated_inputs(rows, width, hidden, kind, "f32")
+    got = nn.gated_linear(x, gw, uw, gb, ub, f, saved=True)
+    for g, (value, slack), what in zip(got, ref.gated(wide(x), wide(gw), wide(uw), wide(gb), wide(ub), f), ("h", "gate", "up")):
+        ref.check(g, value, slack, what)
+    assert torch.equal(nn.gated_linear(x, gw, uw, gb, ub, f), got[0])
+    _, gate, up = got
+    back = nn.gated_linear_backward(dh, x, gate, up, gw, uw, gb, ub, f)
+    want = ref.gated_gradient(wide(dh), wide(x), wide(gate), wide(up), wide(gw), wide(uw), f, x.dtype)
+    for g, (value, slack), what in zip(back, want, ("dx", "dgate_weight", "dup_weight", "dgate_bias", "dup_bias")):
+        ref.check(g, value, slack, what)
+
+
 @gpu
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("rows", [5, 90])
@@ -253,6 +274,26 @@ def test_linear_cross_entropy_gradient(rows, width, items, kind):
                 assert g.dtype == like.dtype and g.shape == like.shape
                 ref.check(g, value, slack, what)
         assert (got[0][target == -100] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("share", [0.0, 0.4])
+@pytest.mark.parametrize("rows, width, items", [(4100, 200, 3001), (3000, 1030, 5003), (9001, 136, 2050), (600, 520, 40000), (5000, 128, 7001), (9000, 100, 700)])
+def test_cross_entropy_of_many_rows(rows, width, items, share, kind):
+    x, w, target, b = items_inputs(rows, width, items, kind, "f32", share)
+    clean = x.clone()
+    x[target == -100] = float("nan")
+    loss, lse = nn.linear_cross_entropy(x, w, target, b, stats=True)
+    want = ref.cross_entropy(wide(clean), wide(w), wide(b), target, -100)
+    ref.check(loss, *want[0], "loss")
+    ref.check(lse, *want[1], "lse")
+    dloss = values(rows, "f32", 9, 1e-3)
+    got = nn.linear_cross_entropy_backward(dloss, x, w, target, lse, b)
+    want = ref.cross_entropy_gradient(wide(dloss), wide(clean), wide(w), wide(b), target, wide(lse), -100, x.dtype)
+    for g, (value, slack), what in zip(got, want, ("dx", "dweight", "dbias")):
+        ref.check(g, value, slack, what)
+    assert (got[0][target == -100] == 0).all()
 
 
 @gpu
