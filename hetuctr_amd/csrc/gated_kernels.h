@@ -5,34 +5,44 @@
 
 namespace hctr {
 
-// sigmoid(v) and 1 - sigmoid(v), neither by cancellation
+// sigmoid(v) and 1 - sigmoid(v), neither by cancellation.  For 16-bit values by the machine's own exponential of two and reciprocal: its argument is off by
+// half a unit of itself, so that the value is by |v| * 2^-24 of it, far below their rounding where it is not nothing; a third of the instructions
+// (us, 8192 rows through 4096 x 16384 twice 1951 -> 1800, 65536 rows through 3328 x 512 469 -> 450).
 struct Sigmoid {
   float s, rest;
 };
-__device__ __forceinline__ Sigmoid sigmoid(float v) {
-  const float e = expf(-fabsf(v)), large = 1.f / (1.f + e), small = e * large;
+template <typename T> __device__ __forceinline__ Sigmoid sigmoid(float v) {
+  float e, large;
+  if constexpr (sizeof(T) == 2) {
+    e = __builtin_amdgcn_exp2f(fabsf(v) * -1.4426950408889634f);
+    large = __builtin_amdgcn_rcpf(1.f + e);
+  } else {
+    e = expf(-fabsf(v));
+    large = 1.f / (1.f + e);
+  }
+  const float small = e * large;
   return v >= 0.f || v != v ? Sigmoid{large, small} : Sigmoid{small, large};
 }
 // the normal distribution's integral
 __device__ __forceinline__ float normal_integral(float v) { return 0.5f * erfcf(v * -0.70710678118654752f); }
 
-__device__ __forceinline__ float activated(int f, float v) {
-  if (f == HCTR_SILU) return v * sigmoid(v).s;
+template <typename T> __device__ __forceinline__ float activated(int f, float v) {
+  if (f == HCTR_SILU) return v * sigmoid<T>(v).s;
   if (f == HCTR_GELU) return v * normal_integral(v);
   if (f == HCTR_RELU) return v > 0.f || v != v ? v : 0.f;
-  return sigmoid(v).s;
+  return sigmoid<T>(v).s;
 }
 // f(v) and f'(v)
 struct Slope {
   float value, slope;
 };
-__device__ __forceinline__ Slope slope_of(int f, float v) {
+template <typename T> __device__ __forceinline__ Slope slope_of(int f, float v) {
   if (f == HCTR_GELU) {
     const float whole = normal_integral(v);
     return {v * whole, whole + v * 0.39894228040143268f * expf(-0.5f * v * v)};
   }
   if (f == HCTR_RELU) return {v > 0.f || v != v ? v : 0.f, v > 0.f ? 1.f : 0.f};
-  const Sigmoid g = sigmoid(v);
+  const Sigmoid g = sigmoid<T>(v);
   if (f == HCTR_SILU) return {v * g.s, g.s + v * g.s * g.rest};
   return {g.s, g.s * g.rest};
 }
@@ -44,7 +54,7 @@ template <typename T> __device__ __forceinline__ f32x4 gated4(const GatedForward
   for (int e = 0; e < 4; e++) {
     gate[e] += bias_at<T>(p.gate_bias, p.narrow, column + e, p.hidden);
     up[e] += bias_at<T>(p.up_bias, p.narrow, column + e, p.hidden);
-    h[e] = activated(p.activation, gate[e]) * up[e];
+    h[e] = activated<T>(p.activation, gate[e]) * up[e];
   }
   return h;
 }
@@ -57,8 +67,7 @@ template <typename T> __device__ __forceinline__ void finish_gated(const GatedFo
 
 // Both products in one: the rows of the two matrices of weights alternate in a tile, 32 by 32, so that a wave holds the same columns of
 // both, and makes h of them.  Bound by the matrix cores, at the clock that their power leaves (51 % of the cycles), and by the ends of tiles, which
-// nothing overlaps where a tile has the CU for itself: 8192 rows, 4096 x 16384 twice in bfloat16 1948 us with three results (1.13 PFLOP/s);
-// with h alone about 100 less.
+// nothing overlaps where a tile has the CU for itself: 8192 rows, 4096 x 16384 twice in bfloat16 1800 us with three results (1.22 PFLOP/s).
 template <typename T, int TILE> __global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kPaired, TILE, TILE>::kThreads), (Product<T, Lies::kAlong, Lies::kAlong, Second::kPaired, TILE, TILE>::kWavesEach))
 void gated_product(GatedForward p) {
   typedef Product<T, Lies::kAlong, Lies::kAlong, Second::kPaired, TILE, TILE> P;
@@ -162,8 +171,7 @@ template <typename T, int ROWS, int GROUPS> __global__ __launch_bounds__((FewRow
 }
 
 // dgate and dup of columns c .. c + V - 1 of a block's rows, and the sums over them.  Eight threads share out the rows of 32 pieces.  Bound by
-// memory and, nearly as much, by the activation's arithmetic (86 % of the vector units' cycles with an exact exponential and quotient):
-// 8192 x 16384 in bfloat16, three matrices read and two written, 222 us, 6.0 TB/s.
+// memory: 8192 x 16384 in bfloat16, three matrices read and two written, 217 us, 6.2 TB/s.
 template <typename T, bool SUMS> __global__ __launch_bounds__(256) void gated_slopes(GatedSlopes p) {
   constexpr int V = kVec<T>, LANES = 32, GROUPS = 8;
   __shared__ float joined[SUMS ? GROUPS : 1][2][LANES * V];
@@ -178,7 +186,7 @@ template <typename T, bool SUMS> __global__ __launch_bounds__(256) void gated_sl
       Floats<V> d[2];
 #pragma unroll
       for (int e = 0; e < V; e++) {
-        const Slope s = slope_of(p.activation, gate.v[e]);
+        const Slope s = slope_of<T>(p.activation, gate.v[e]);
         d[0].v[e] = c + e < p.hidden ? dh.v[e] * up.v[e] * s.slope : 0.f;
         d[1].v[e] = c + e < p.hidden ? dh.v[e] * s.value : 0.f;
       }
