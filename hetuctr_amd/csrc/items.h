@@ -73,6 +73,9 @@ template <typename T> void launch_join_tails(const JoinTails &p, hipStream_t s);
 // Narrow matrices of 16-bit values: rows of up to kNarrow columns.  A block owns rows of one matrix, whose values it keeps in registers, and
 // goes through a range of the rows of the other.
 constexpr size_t kNarrow = 128;
+// Blocks that share a CU: three where the registers hold them (us, 4096 rows, a million items: forward of 64 columns 955 -> 889, of 32
+// 844 -> 777, dx of 32 985 -> 895, the weights' gradient 987 -> 985; forward of 128 would spill, 1373 -> 1403).
+constexpr int narrow_share(size_t width, bool gradient) { return width <= 64 && (!gradient || width <= 32) ? 3 : 2; }
 struct ItemsNarrow {
   const char *x, *weight;
   int64_t x_stride, weight_stride; // bytes

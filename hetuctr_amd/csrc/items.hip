@@ -301,10 +301,10 @@ template <typename A> void check(const A &a) {
 
 } // namespace
 
-// As many blocks as the card holds at a time, two a CU, of eight tiles of 64 rows at least.
+// As many blocks as the card holds at a time, of eight tiles of 64 rows at least.
 uint32_t narrow_ranges(size_t owned, size_t through, size_t width, bool gradient) {
   const size_t owners = (owned + 255) / (gradient && width > 64 ? 192 : 256), tiles = (through + 63) / 64;
-  return (uint32_t)std::max<size_t>(1, std::min(512 / std::max<size_t>(1, owners), tiles / 8));
+  return (uint32_t)std::max<size_t>(1, std::min((size_t)256 * narrow_share(width, gradient) / std::max<size_t>(1, owners), tiles / 8));
 }
 
 size_t linear_cross_entropy_workspace(const hctr_items_args &a) {

@@ -9,7 +9,7 @@
 //
 // Bound by the vector units: forward an exponential (a quarter of the others' rate) and four instructions a logit, 73 % of the cycles beside 35 %
 // in the matrix cores.  4096 rows, a million items of 128 bfloat16: 1.27 ms (0.83 PFLOP/s), by tiles, each of which joins lanes and waves
-// for itself, 2.75; dx 2.0 and the weights' gradient 2.1, with d in memory 8.9 together.  Of 32 columns 0.84, 0.99 and 0.99.
+// for itself, 2.75; dx 2.0 and the weights' gradient 2.1, with d in memory 8.9 together.  Of 32 columns 0.78, 0.90 and 0.99.
 #pragma once
 #include "items.h"
 #include "items_tail.h"
@@ -74,7 +74,8 @@ template <typename T, int KS> struct NarrowTiles {
 // SIMD's registers, so that two waves can share it, and one's exponentials run beside the other's products.
 template <int KS, Narrow MODE> constexpr int kOwned = MODE != Narrow::kForward && KS == 4 ? 3 : 4;
 
-template <typename T, int KS, Narrow MODE> __global__ __launch_bounds__(256, 2) void items_narrow(ItemsNarrow p) {
+template <typename T, int KS, Narrow MODE>
+__global__ __launch_bounds__(256, narrow_share(KS * 32, MODE != Narrow::kForward)) void items_narrow(ItemsNarrow p) {
   typedef NarrowTiles<T, KS> N;
   constexpr int OI = kOwned<KS, MODE>, J = MODE == Narrow::kForward ? 4 : 2;
   constexpr bool WEIGHT = MODE == Narrow::kDweight;
@@ -90,7 +91,7 @@ template <typename T, int KS, Narrow MODE> __global__ __launch_bounds__(256, 2) 
   const char *own = WEIGHT ? p.weight : p.x, *other = WEIGHT ? p.x : p.weight;
   const int64_t own_stride = WEIGHT ? p.weight_stride : p.x_stride, stride = WEIGHT ? p.x_stride : p.weight_stride;
 
-  // Of the two waves that share a SIMD one goes first, so that they do not do the same at the same time: by the number that the hardware gave it
+  // Of two waves that share a SIMD one goes first, so that they do not do the same at the same time: by the number that the hardware gave it
   // (us, weights' gradient: 4096 rows and a million items 2236 -> 2136, 65536 and 20000 956 -> 865; the others the same or 1 % slower).
   if (WEIGHT && __builtin_amdgcn_s_getreg(3 << 11 | 4) & 1) __builtin_amdgcn_s_setprio(1);
   Fragment<T> mine[OI][KS];
