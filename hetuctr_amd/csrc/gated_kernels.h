@@ -66,7 +66,7 @@ template <typename T> __device__ __forceinline__ void finish_gated(const GatedFo
 }
 
 // Both products in one: the rows of the two matrices of weights alternate in a tile, 32 by 32, so that a wave holds the same columns of
-// both, and makes h of them.  Bound by the matrix cores, at the clock that their power leaves (51 % of the cycles), and by the ends of tiles, which
+// both, and makes h of them.  Bound by the matrix cores, at the clock that their power leaves (56 % of the cycles), and by the ends of tiles, which
 // nothing overlaps where a tile has the CU for itself: 8192 rows, 4096 x 16384 twice in bfloat16 1800 us with three results (1.22 PFLOP/s).
 template <typename T, int TILE> __global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kPaired, TILE, TILE>::kThreads), (Product<T, Lies::kAlong, Lies::kAlong, Second::kPaired, TILE, TILE>::kWavesEach))
 void gated_product(GatedForward p) {
