@@ -23,12 +23,28 @@ template <typename T> __device__ __forceinline__ Sigmoid sigmoid(float v) {
   const float small = e * large;
   return v >= 0.f || v != v ? Sigmoid{large, small} : Sigmoid{small, large};
 }
-// the normal distribution's integral
-__device__ __forceinline__ float normal_integral(float v) { return 0.5f * erfcf(v * -0.70710678118654752f); }
+// The normal distribution's integral up to v, and exp(-v^2 / 2).  For 16-bit values by one exponential, which the slope takes too: below zero the integral
+// is that exponential times t P(t), t = 1 / (1 + 0.28 |v|), with P of degree eight by least squares, weighted anew until its largest relative error
+// was smallest, 1.7e-7, over all v; the exponential's argument, rounded, adds v^2 2^-24 (us, against the library's erfcf and expf: 65536 rows through 3328 x 512 twice with three results 1026 -> 865,
+// its gradient 1328 -> 1258; 8192 through 4096 x 16384 1905 -> 1791).
+struct Normal {
+  float whole, e;
+};
+template <typename T> __device__ __forceinline__ Normal normal(float v) {
+  if constexpr (sizeof(T) == 2) {
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.28f, fabsf(v), 1.f)), e = __builtin_amdgcn_exp2f(v * v * -0.72134752044448170f);
+    float q = 0.0247199624463723f;
+    for (float c : {-0.09359308485038127f, 0.0924280603918132f, -0.0064491364459287335f, 0.07277499335202713f, 0.08363079551306478f, 0.10308466407569232f,
+                    0.11169980273233898f, 0.11170385755238264f})
+      q = __builtin_fmaf(q, t, c);
+    const float rest = q * t * e;
+    return {v < 0.f ? rest : 1.f - rest, e};
+  } else return {0.5f * erfcf(v * -0.70710678118654752f), expf(-0.5f * v * v)};
+}
 
 template <typename T> __device__ __forceinline__ float activated(int f, float v) {
   if (f == HCTR_SILU) return v * sigmoid<T>(v).s;
-  if (f == HCTR_GELU) return v * normal_integral(v);
+  if (f == HCTR_GELU) return v * normal<T>(v).whole;
   if (f == HCTR_RELU) return v > 0.f || v != v ? v : 0.f;
   return sigmoid<T>(v).s;
 }
@@ -38,8 +54,8 @@ struct Slope {
 };
 template <typename T> __device__ __forceinline__ Slope slope_of(int f, float v) {
   if (f == HCTR_GELU) {
-    const float whole = normal_integral(v);
-    return {v * whole, whole + v * 0.39894228040143268f * expf(-0.5f * v * v)};
+    const Normal n = normal<T>(v);
+    return {v * n.whole, n.whole + v * 0.39894228040143268f * n.e};
   }
   if (f == HCTR_RELU) return {v > 0.f || v != v ? v : 0.f, v > 0.f ? 1.f : 0.f};
   const Sigmoid g = sigmoid<T>(v);

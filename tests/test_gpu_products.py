@@ -168,6 +168,30 @@ def test_steep_and_flat_ends_of_the_activations():
 
 
 @gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_activations_between_their_ends(kind):
+    # Values one by one from where the result is next to nothing, as products with one, which are exact.  Besides what FUNCTION counts the argument of an
+    # exponential or of the normal distribution's integral is rounded twice and made with a rounded factor, three halves of a unit of itself: a
+    # value of exp(-|v|) is off by 1.5 |v| units for it, one of exp(-v^2 / 2) or of the integral by 1.5 v^2 at most.
+    x = torch.cat([torch.linspace(-12.5, 8, 1536), torch.linspace(-0.1, 0.1, 256)]).to(TYPES[kind]).cuda()[:, None].contiguous()
+    one, flat = torch.ones((1, 1), dtype=TYPES[kind], device="cuda"), torch.zeros((1, 1), dtype=TYPES[kind], device="cuda")
+    bias = torch.ones(1, device="cuda")                     # the second product is 0 x + 1
+    v = wide(x)
+    units = ref.FUNCTION + 1.5 * ref.U * torch.maximum(v * v, v.abs())
+    # (torch.special.ndtr is 1 + erf over 2: nothing is left of it below -8)
+    sigmoid, integral, density = torch.sigmoid(v), torch.special.erfc(v.cpu() * -0.5 ** 0.5).cuda() / 2, torch.exp(-v * v / 2) / (2 * np.pi) ** 0.5
+    sizes = {"silu": sigmoid * (1 + v.abs() * (1 - sigmoid)), "gelu": integral + v.abs() * density, "relu": 0 * v, "sigmoid": sigmoid * (1 - sigmoid)}
+    for f in ACTIVATIONS:
+        value, slope = (v * integral, integral + v * density) if f == "gelu" else ref.activation(f, v)
+        h, gate, up = nn.gated_linear(x, one, flat, None, bias, activation=f, saved=True)
+        assert torch.equal(gate, x) and torch.equal(up, torch.ones_like(x))
+        ref.check(h, value, units * value.abs(), f)
+        dx = nn.gated_linear_backward(torch.ones_like(h), x, gate, up, one, flat, None, bias, activation=f)[0]       # dgate, rounded twice
+        slack = 2 * units * sizes[f]                        # two factors
+        ref.check(dx, slope, slack + ref.rounding(slope.abs() + slack, TYPES[kind]), f + "'")
+
+
+@gpu
 @pytest.mark.parametrize("rows", [3, 200])
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_autograd_of_the_gated_layer(rows, kind):
