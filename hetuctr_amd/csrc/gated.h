@@ -24,9 +24,14 @@ struct GatedSlopes {
   int64_t dh_stride, gate_stride, up_stride;
   void *slopes;         // [rows][2 * padded]: dgate, dup, zeros behind each
   float *sums;          // [blocks][2 * padded] sums over a block's rows, or null
+  float *sizes;         // half: [blocks along the rows][blocks along the columns] the largest |dgate|, |dup|; or null: not scaled
+  float *guess;         // half: [kGuesses] the largest that some blocks found in some of the rows; or null: they are not scaled at first
+  float *scale;         // half: [2] what dgate and dup were multiplied by before they were rounded, and 1 / that
   uint32_t rows, hidden, padded, rows_each; // rows of a block
   int activation;
 };
+constexpr uint32_t kGuesses = 256;
+inline uint32_t slope_columns(int size) { return 32 * (16 / size); } // of a block
 template <typename T> void launch_slopes(const GatedSlopes &p, hipStream_t s);
 
 // The entry points of the C ABI behind their guard

@@ -79,8 +79,8 @@ template <typename T> void forward(const hctr_gated_args &a) {
 struct BackwardPlan {
   size_t padded, row_blocks, rows_each;
   Shape dx, dweight;
-  size_t slopes, sums, x, gate, up, parts, bytes;
-  bool products, weights;
+  size_t slopes, sums, sizes, x, gate, up, parts, bytes;
+  bool weights;
 };
 BackwardPlan plan_of(const hctr_gated_grad_args &a) {
   BackwardPlan p = {};
@@ -89,11 +89,12 @@ BackwardPlan plan_of(const hctr_gated_grad_args &a) {
   p.weights = a.dgate_weight.data || a.dup_weight.data;
   p.slopes = up(a.rows * 2 * padded * size, 256);
   // blocks for about eight rounds of the card, of 8 to 256 rows each
-  const size_t across = div_up(padded, 32 * (16 / size));
+  const size_t across = div_up(padded, slope_columns((int)size));
   p.rows_each = std::min<size_t>(256, std::max<size_t>(8, up(a.rows * across / 8192 + 1, 8)));
   p.rows_each = std::max(p.rows_each, up((a.rows + 65534) / 65535, 8));
   p.row_blocks = div_up(a.rows, p.rows_each);
   if (a.dgate_bias || a.dup_bias) p.sums = up(p.row_blocks * 2 * padded * sizeof(float), 256);
+  if (a.dtype == HCTR_F16 && a.rows && (a.dx.data || p.weights)) p.sizes = up((kGuesses + 2 + p.row_blocks * across) * sizeof(float), 256);
   if (a.dx.data && a.rows) {
     p.dx = shape_of(a.rows, a.width, 2 * padded, (int)size, false, true);
     if (p.dx.splits > 1) p.parts = parts_bytes(a.rows, a.width, p.dx.splits);
@@ -109,7 +110,7 @@ BackwardPlan plan_of(const hctr_gated_grad_args &a) {
     p.x = laid_out_bytes(a.x, a.rows, a.width, size);
   }
   p.parts = up(p.parts, 256);
-  p.bytes = p.slopes + p.sums + p.parts + p.x + p.gate + p.up;
+  p.bytes = p.slopes + p.sums + p.sizes + p.parts + p.x + p.gate + p.up;
   return p;
 }
 
@@ -118,13 +119,21 @@ template <typename T> void backward(const hctr_gated_grad_args &a) {
   const hipStream_t s = (hipStream_t)a.stream;
   const size_t size = sizeof(T), padded = plan.padded;
   char *space = (char *)a.workspace, *slopes = space, *parts = slopes + plan.slopes;
-  float *sums = (float *)(parts + plan.parts);
-  space = (char *)sums + plan.sums;
+  float *sums = (float *)(parts + plan.parts), *scale = plan.sizes ? (float *)((char *)sums + plan.sums) : nullptr;
+  const float *back = scale ? scale + 1 : nullptr;
+  space = (char *)sums + plan.sums + plan.sizes;
 
   GatedSlopes p = {};
   p.dh = a.dh.data, p.gate = a.gate.data, p.up = a.up.data;
   p.dh_stride = a.dh.stride, p.gate_stride = a.gate.stride, p.up_stride = a.up.stride;
   p.slopes = slopes, p.sums = plan.sums ? sums : nullptr;
+  p.scale = scale;
+  if (scale) {
+    // (us of the gradient, 65536 rows through 3328 x 512 twice, slopes of 1e-3: 1748 without a guess, as they are all made twice; 1310 with one.  Where there are
+    // few slopes a launch takes longer than making them again.)
+    p.guess = (uint64_t)a.rows * a.hidden >= (1u << 22) ? scale + 2 : nullptr;
+    p.sizes = scale + 2 + kGuesses;
+  }
   p.rows = (uint32_t)a.rows, p.hidden = (uint32_t)a.hidden, p.padded = (uint32_t)padded, p.rows_each = (uint32_t)plan.rows_each;
   p.activation = a.activation;
   if (a.rows) launch_slopes<T>(p, s);
@@ -151,7 +160,7 @@ template <typename T> void backward(const hctr_gated_grad_args &a) {
     q.rows = (uint32_t)a.rows, q.columns = (uint32_t)a.width, q.k = (uint32_t)(2 * padded);
     q.splits = plan.dx.splits, q.band = 8;
     q.partial = q.splits > 1 ? (float *)parts : nullptr;
-    q.result = {{a.dx.data, nullptr}, {a.dx.stride, 0}, q.rows, q.columns, ~0u, nullptr, nullptr};
+    q.result = {{a.dx.data, nullptr}, {a.dx.stride, 0}, q.rows, q.columns, ~0u, back, nullptr};
     launch_forward_product<T>(q, plan.dx.tile, s);
     if (q.partial) launch_join<T>(q, s);
   }
@@ -166,7 +175,7 @@ template <typename T> void backward(const hctr_gated_grad_args &a) {
     q.splits = plan.dweight.splits, q.band = 8;
     q.partial = q.splits > 1 ? (float *)parts : nullptr;
     const hctr_matrix &first = gate ? a.dgate_weight : a.dup_weight, &second = a.dup_weight;
-    q.result = {{first.data, both ? second.data : nullptr}, {first.stride, second.stride}, (uint32_t)a.hidden, q.columns, (uint32_t)padded, nullptr,
+    q.result = {{first.data, both ? second.data : nullptr}, {first.stride, second.stride}, (uint32_t)a.hidden, q.columns, (uint32_t)padded, back,
                 nullptr};
     launch_across_product<T>(q, plan.dweight.tile, s);
     if (q.partial) launch_join<T>(q, s);

@@ -186,33 +186,63 @@ template <typename T, int ROWS, int GROUPS> __global__ __launch_bounds__((FewRow
   }
 }
 
-// dgate and dup of columns c .. c + V - 1 of a block's rows, and the sums over them.  Eight threads share out the rows of 32 pieces.  Bound by
-// memory: 8192 x 16384 in bfloat16, three matrices read and two written, 217 us, 6.2 TB/s.
-template <typename T, bool SUMS> __global__ __launch_bounds__(256) void gated_slopes(GatedSlopes p) {
+// dgate and dup of columns c .. c + V - 1 of a row
+template <typename T, int V> __device__ __forceinline__ void slopes_at(const GatedSlopes &p, uint32_t r, uint32_t c, Floats<V> (&d)[2]) {
+  const Floats<V> dh = load_columns<V, Rows::kLong, true>((const T *)p.dh + (int64_t)r * p.dh_stride, c, p.hidden);
+  const Floats<V> gate = load_columns<V, Rows::kLong, true>((const T *)p.gate + (int64_t)r * p.gate_stride, c, p.hidden);
+  const Floats<V> up = load_columns<V, Rows::kLong, true>((const T *)p.up + (int64_t)r * p.up_stride, c, p.hidden);
+#pragma unroll
+  for (int e = 0; e < V; e++) {
+    const Slope s = slope_of<T>(p.activation, gate.v[e]);
+    d[0].v[e] = c + e < p.hidden ? dh.v[e] * up.v[e] * s.slope : 0.f;
+    d[1].v[e] = c + e < p.hidden ? dh.v[e] * s.value : 0.f;
+  }
+}
+// the largest of them, leaving out what is not finite
+template <int V> __device__ __forceinline__ float largest(const Floats<V> (&d)[2], float most) {
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+#pragma unroll
+    for (int e = 0; e < V; e++) most = fmaxf(most, fabsf(d[i].v[e]) < __builtin_inff() ? fabsf(d[i].v[e]) : 0.f);
+  return most;
+}
+// the largest of a block's values, which are not negative, the same in all threads
+__device__ __forceinline__ float block_most(float v) {
+  __shared__ float waves[256 / kWave];
+#pragma unroll
+  for (int mask = 32; mask; mask /= 2) v = fmaxf(v, __shfl_xor(v, mask));
+  __syncthreads(); // what was there before is read
+  if (lane_id() == 0) waves[threadIdx.x / kWave] = v;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 256 / kWave; i++) v = fmaxf(v, waves[i]);
+  return v;
+}
+
+// dgate and dup, as the operands of the products: rounded to the type, since the matrix cores take both of a product's in one.  Eight threads share
+// out the rows of 32 pieces, block `across` along the columns, `down` along the rows.  SUMS: the sums over a block's rows, of what was neither
+// scaled nor rounded.  Returns, if SIZE, the largest that the thread made, before it was scaled.
+template <typename T, bool SUMS, bool SIZE> __device__ __forceinline__ float slopes_of(const GatedSlopes &p, uint32_t across, uint32_t down, float scale) {
   constexpr int V = kVec<T>, LANES = 32, GROUPS = 8;
   __shared__ float joined[SUMS ? GROUPS : 1][2][LANES * V];
-  const uint32_t x = threadIdx.x % LANES, y = threadIdx.x / LANES, c = (blockIdx.x * LANES + x) * V;
-  const uint32_t first = blockIdx.y * p.rows_each, last = min(p.rows, first + p.rows_each);
+  const uint32_t x = threadIdx.x % LANES, y = threadIdx.x / LANES, c = (across * LANES + x) * V;
+  const uint32_t first = down * p.rows_each, last = min(p.rows, first + p.rows_each);
   Floats<V> sums[2] = {};
+  float most = 0.f;
   if (c < p.padded)
     for (uint32_t r = first + y; r < last; r += GROUPS) {
-      const Floats<V> dh = load_columns<V, Rows::kLong, true>((const T *)p.dh + (int64_t)r * p.dh_stride, c, p.hidden);
-      const Floats<V> gate = load_columns<V, Rows::kLong, true>((const T *)p.gate + (int64_t)r * p.gate_stride, c, p.hidden);
-      const Floats<V> up = load_columns<V, Rows::kLong, true>((const T *)p.up + (int64_t)r * p.up_stride, c, p.hidden);
       Floats<V> d[2];
-#pragma unroll
-      for (int e = 0; e < V; e++) {
-        const Slope s = slope_of<T>(p.activation, gate.v[e]);
-        d[0].v[e] = c + e < p.hidden ? dh.v[e] * up.v[e] * s.slope : 0.f;
-        d[1].v[e] = c + e < p.hidden ? dh.v[e] * s.value : 0.f;
-      }
+      slopes_at<T>(p, r, c, d);
+      if (SIZE) most = largest(d, most);
       T *to = (T *)p.slopes + (uint64_t)r * (2 * p.padded) + c;
 #pragma unroll
       for (int i = 0; i < 2; i++) {
-        *(typename Packed<T, V>::type *)(to + i * p.padded) = rounded<T>(d[i]);
         if (SUMS)
 #pragma unroll
           for (int e = 0; e < V; e++) sums[i].v[e] += d[i].v[e];
+#pragma unroll
+        for (int e = 0; e < V; e++) d[i].v[e] *= scale;
+        *(typename Packed<T, V>::type *)(to + i * p.padded) = rounded<T>(d[i]);
       }
     }
   if constexpr (SUMS) {
@@ -222,13 +252,58 @@ template <typename T, bool SUMS> __global__ __launch_bounds__(256) void gated_sl
       for (int e = 0; e < V; e++) joined[y][i][e * LANES + x] = sums[i].v[e];
     __syncthreads();
     for (uint32_t t = threadIdx.x; t < 2 * LANES * V; t += 256) {
-      const uint32_t i = t / (LANES * V), at = t % (LANES * V), column = blockIdx.x * LANES * V + at;
+      const uint32_t i = t / (LANES * V), at = t % (LANES * V), column = across * LANES * V + at;
       float sum = 0.f;
 #pragma unroll
       for (int g = 0; g < GROUPS; g++) sum += joined[g][i][at % V * LANES + at / V];
-      if (column < p.padded) p.sums[(uint64_t)blockIdx.y * (2 * p.padded) + i * p.padded + column] = sum;
+      if (column < p.padded) p.sums[(uint64_t)down * (2 * p.padded) + i * p.padded + column] = sum;
     }
   }
+  return most;
+}
+
+// Half precision does not hold every slope: beyond 65504 they are infinite, and below 2^-14 they lose bits.  So they are multiplied by a power of
+// two, by which the products' sums are divided, where that keeps the largest of them in 1 .. 2^15: then those above 2^-14 of it have
+// all their bits, and none is off by more than 2^-25 of it.  The power is that which takes the largest of some rows to 2^8 .. 2^9, one if there
+// are few; a launch behind finds the largest of all, and makes them again, it being in 2^13 .. 2^14, where it was not in that range.
+__device__ __forceinline__ int power_to(int to, float most) { return most > 0.f ? min(to - ilogbf(most), 126) : 0; } // (a factor that is a float, and so is 1 / it)
+__device__ __forceinline__ int guessed_power(const GatedSlopes &p) { return p.guess ? power_to(8, block_most(p.guess[threadIdx.x])) : 0; }
+
+template <typename T> __global__ __launch_bounds__(256) void gated_guess(GatedSlopes p, uint32_t some) {
+  constexpr uint32_t V = kVec<T>;
+  const uint32_t pieces = (p.hidden + V - 1) / V;
+  float most = 0.f;
+  for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < some * pieces; i += kGuesses * 256) {
+    Floats<V> d[2];
+    slopes_at<T>(p, (uint32_t)((uint64_t)(i / pieces) * p.rows / some), i % pieces * V, d);
+    most = largest(d, most);
+  }
+  most = block_most(most);
+  if (threadIdx.x == 0) p.guess[blockIdx.x] = most;
+}
+
+// Bound by memory: 8192 x 16384 in bfloat16, three matrices read and two written, 217 us, 6.2 TB/s.
+template <typename T, bool SUMS> __global__ __launch_bounds__(256) void gated_slopes(GatedSlopes p) {
+  if constexpr (std::is_same_v<T, f16_t>) {
+    const float most = block_most(slopes_of<T, SUMS, true>(p, blockIdx.x, blockIdx.y, ldexpf(1.f, guessed_power(p))));
+    if (p.sizes && threadIdx.x == 0) p.sizes[blockIdx.y * gridDim.x + blockIdx.x] = most;
+  } else {
+    slopes_of<T, SUMS, false>(p, blockIdx.x, blockIdx.y, 1.f);
+  }
+}
+
+template <typename T> __global__ __launch_bounds__(256) void gated_rescale(GatedSlopes p, uint32_t across, uint32_t blocks) {
+  float most = 0.f;
+  for (uint32_t i = threadIdx.x; i < blocks; i += 256) most = fmaxf(most, p.sizes[i]);
+  most = block_most(most);
+  int by = guessed_power(p);
+  const float was = ldexpf(most, by);
+  const bool fits = most == 0.f || (was >= 1.f && was < 32768.f);
+  if (!fits) by = power_to(13, most);
+  const float scale = ldexpf(1.f, by);
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.scale[0] = scale, p.scale[1] = ldexpf(1.f, -by);
+  if (fits) return;
+  for (uint32_t i = blockIdx.x; i < blocks; i += gridDim.x) slopes_of<T, false, false>(p, i % across, i / across, scale);
 }
 
 template <typename T> void launch_gated(GatedForward &p, int tile, hipStream_t s) {
@@ -259,10 +334,20 @@ template <typename T> void launch_gated_few(const GatedForward &p, hipStream_t s
   HCTR_HIP(hipGetLastError());
 }
 template <typename T> void launch_slopes(const GatedSlopes &p, hipStream_t s) {
-  const dim3 blocks(div_up(p.padded, 32 * kVec<T>), div_up(p.rows, p.rows_each));
+  const dim3 blocks(div_up(p.padded, slope_columns(sizeof(T))), div_up(p.rows, p.rows_each));
+  if constexpr (std::is_same_v<T, f16_t>)
+    if (p.guess) {
+      hipLaunchKernelGGL((gated_guess<T>), dim3(kGuesses), dim3(256), 0, s, p, min(p.rows, 64u));
+      HCTR_HIP(hipGetLastError());
+    }
   if (p.sums) hipLaunchKernelGGL((gated_slopes<T, true>), blocks, dim3(256), 0, s, p);
   else hipLaunchKernelGGL((gated_slopes<T, false>), blocks, dim3(256), 0, s, p);
   HCTR_HIP(hipGetLastError());
+  if constexpr (std::is_same_v<T, f16_t>)
+    if (p.sizes) {
+      hipLaunchKernelGGL((gated_rescale<T>), dim3(min(blocks.x * blocks.y, 2048u)), dim3(256), 0, s, p, blocks.x, blocks.x * blocks.y);
+      HCTR_HIP(hipGetLastError());
+    }
 }
 
 } // namespace hctr

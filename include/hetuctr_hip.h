@@ -342,7 +342,8 @@ size_t hctr_gated_linear_workspace(const hctr_gated_args *a);
 /* Its gradient, given that of h and the products gate and up that the forward pass left:
  *     dgate = dh * up * f'(gate),  dup = dh * f(gate)
  *     dx = dgate gate_weight + dup up_weight,  dgate_weight = dgate^T x,  dup_weight = dup^T x,  dgate_bias, dup_bias: their sums over the rows
- * dgate and dup are rounded to dtype before the products, not for the biases.  f' of max(v, 0) is 0 at 0.  Any result may be missing (data
+ * dgate and dup are rounded to dtype before the products, not for the biases (to half after a power of two that takes the largest of them to 1 .. 2^15,
+ * by which the results are divided).  f' of max(v, 0) is 0 at 0.  Any result may be missing (data
  * NULL); gate_weight and up_weight are read for dx alone, x for the weights' gradients alone. */
 typedef struct hctr_gated_grad_args {
   size_t rows, width, hidden;

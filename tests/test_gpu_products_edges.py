@@ -1,0 +1,124 @@
+"""Ends of the ranges of the gated linear layer and of cross entropy over many items, against their definitions in 64 bits
+(tests/products_reference.py)."""
+import math
+
+import pytest
+import torch
+
+from hetuctr_amd import nn
+from tests import products_reference as ref
+from tests.test_gpu_products import ACTIVATIONS, TYPES, gated_inputs, values, wide
+
+gpu = pytest.mark.gpu
+
+
+# ---- slopes of half precision ---------------------------------------------------------------------------------------------
+def gated_gradient_in_range(dh, x, gate, up, gate_weight, up_weight, f, many=None):
+    """ref.gated_gradient for half precision, where dgate and dup are multiplied by a power of two before they are rounded.  Few: by none if the largest is in
+    1 .. 2^15, else that which takes it to 2^13 at least.  Many: one that takes it to 2^8 at least.  As if dh were larger by half of that
+    power, for which values become subnormal no later."""
+    value, slope = ref.activation(f, wide(gate))
+    d = torch.stack((wide(dh) * slope * wide(up), wide(dh) * value)).abs()
+    most = d[d.isfinite()].max().item()
+    many = dh.numel() >= 2 ** 22 if many is None else many
+    by = 1.0 if 1 <= most < 2 ** 15 and not many else 2.0 ** ((7 if many else 12) - math.floor(math.log2(most)))
+    want = ref.gated_gradient(wide(dh) * by, wide(x), wide(gate), wide(up), wide(gate_weight), wide(up_weight), f, torch.float16)
+    return [(v / by, s / by) for v, s in want]
+
+
+def check_half(got, value, slack, what):
+    """As ref.check; a result that lies beyond the type's largest number is infinite"""
+    inside, beyond = value.abs() + slack < 65504, value.abs() - slack > 65520
+    ref.check(got[inside], value[inside], slack[inside], what)
+    assert torch.equal(got[beyond].double(), value[beyond].sign() * math.inf)
+
+
+# dh, up, x and weights: the slopes lie beyond 65504, or below the smallest half, and the results in between
+SLOPES = {"beyond the largest half": (1e3, 100.0, 3e-4, 3e-4), "below the smallest half": (1e-6, 1e-2, 1e3, 1e3), "among the smallest halves": (1e-4, 1.0, 10.0, 10.0)}
+
+
+@gpu
+@pytest.mark.parametrize("sizes", SLOPES)
+@pytest.mark.parametrize("rows, width, hidden", [(1, 40, 24), (5, 64, 40), (65, 37, 41), (300, 130, 300), (2000, 96, 136), (5003, 300, 1001)])
+def test_slopes_of_any_size_in_half_precision(rows, width, hidden, sizes):
+    dh_size, up_size, x_size, weight_size = SLOPES[sizes]
+    dh, x, gw, uw, gb, ub = gated_inputs(rows, width, hidden, "f16", "f32", 9)
+    dh, x = values((rows, hidden), "f16", 30, dh_size), values((rows, width), "f16", 31, x_size)
+    gw, uw = (values((hidden, width), "f16", 32 + i, weight_size) for i in range(2))
+    gate, up = values((rows, hidden), "f16", 34, 2.0), values((rows, hidden), "f16", 35, up_size)
+    for f in ACTIVATIONS if rows < 5000 else ACTIVATIONS[:2]:
+        got = nn.gated_linear_backward(dh, x, gate, up, gw, uw, gb, ub, f)
+        assert all(g.isfinite().all() for g in got) and all(g.count_nonzero() > g.numel() // 8 for g in got)
+        want = gated_gradient_in_range(dh, x, gate, up, gw, uw, f)
+        for g, (value, slack), what in zip(got, want, ("dx", "dgate_weight", "dup_weight", "dgate_bias", "dup_bias")):
+            ref.check(g, value, slack, what + " " + f)
+        # some of the results, in the same call as another's scale
+        only = nn.gated_linear_backward(dh[:1], x[:1], gate[:1], up[:1], gw, uw, None, None, f)
+        want = gated_gradient_in_range(dh[:1], x[:1], gate[:1], up[:1], gw, uw, f)
+        for g, (value, slack), what in zip(only, want, ("dx", "dgate_weight", "dup_weight")):
+            ref.check(g, value, slack, what + " of one row " + f)
+
+
+@gpu
+def test_slopes_in_half_precision_beside_a_row_that_is_not_finite():
+    rows, width, hidden = 150, 72, 40
+    _, x, gw, uw, _, _ = gated_inputs(rows, width, hidden, "f16", "none", 3)
+    gw, uw = gw * 1e-3, uw * 1e-3
+    dh, gate, up = values((rows, hidden), "f16", 40, 1e3), values((rows, hidden), "f16", 41), values((rows, hidden), "f16", 42, 100.0)
+    want = gated_gradient_in_range(dh, x, gate, up, gw, uw, "silu")[0]
+    keep = torch.arange(rows, device="cuda") != 7
+    for odd in (float("nan"), float("inf"), -float("inf")):
+        bad = dh.clone()
+        bad[7, 3] = odd
+        dx = nn.gated_linear_backward(bad, x, gate, up, gw, uw)[0]
+        assert not dx[7].isfinite().all()
+        ref.check(dx[keep], want[0][keep], want[1][keep], "dx")
+
+
+@gpu
+@pytest.mark.parametrize("seen, others", [(1e-4, 1e3), (1e3, 1e-4), (0.0, 1e3), (0.0, 1e-6), (0.0, 0.0), (1.0, float("inf"))])
+def test_many_slopes_in_half_precision_that_a_look_at_some_rows_misses(seen, others):
+    # every 65th row, and the first, are of one size, the others of another: the scale that some rows suggest is far from what all need, or there is none
+    rows, width, hidden = 64 * 65, 72, 1024
+    _, x, gw, uw, _, _ = gated_inputs(rows, width, hidden, "f16", "none", 3)
+    x, gw, uw = x * 1e-3, gw * 1e-3, uw * 1e-3
+    gate, up = values((rows, hidden), "f16", 41), values((rows, hidden), "f16", 42, 100.0)
+    some = torch.arange(rows, device="cuda") % 65 == 0
+    dh = torch.where(some[:, None], seen, others) * values((rows, hidden), "f32", 40)
+    dh = dh.nan_to_num(0.0, math.inf, -math.inf).half()
+    got = nn.gated_linear_backward(dh, x, gate, up, gw, uw)
+    if seen == others == 0:
+        assert all((g == 0).all() for g in got[:3])
+        return
+    keep = some if others == math.inf else torch.ones_like(some)
+    want = gated_gradient_in_range(dh[keep], x[keep], gate[keep], up[keep], gw, uw, "silu", True)
+    for g, (value, slack), what in list(zip(got, want, ("dx", "dgate_weight", "dup_weight")))[:1 if others == math.inf else 3]:
+        ref.check(g[keep] if what == "dx" else g, value, slack, what)
+
+
+@gpu
+def test_a_captured_gradient_finds_its_scale_again():
+    # the largest slope is another one at each replay: beyond the range, within it, below it
+    rows, width, hidden = 90, 64, 48
+    _, x, gw, uw, _, _ = gated_inputs(rows, width, hidden, "f16", "none", 4)
+    gw, uw = gw * 1e-2, uw * 1e-2
+    dh, gate, up = (values((rows, hidden), "f16", 50 + i) for i in range(3))
+    step = lambda: nn.gated_linear_backward(dh, x, gate, up, gw, uw)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i, size in enumerate((1e3, 1.0, 1e-5, 300.0, 1e-3)):
+        dh.copy_(values((rows, hidden), "f16", 60 + i, size))
+        up.copy_(values((rows, hidden), "f16", 70 + i, 100.0))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out[:3]]
+        for g, w in zip(got, step()):
+            assert torch.equal(g, w)
+        for g, (value, slack) in zip(got, gated_gradient_in_range(dh, x, gate, up, gw, uw, "silu")):
+            check_half(g, value, slack, "size %g" % size)
