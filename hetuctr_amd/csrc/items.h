@@ -11,6 +11,7 @@ struct Taken {
   uint32_t *row_of;   // [rows] where each one lies among all rows
   uint32_t *target;   // its item; kNoItem: that is none
   float *dloss, *lse; // of the gradient
+  float *hits;        // of the forward pass, in lse's place: a row's logit of its target, in units of log 2
   float *bias;        // [items] in units of log 2
 };
 constexpr uint32_t kNoItem = 0xffffffffu;
@@ -58,18 +59,6 @@ struct ItemsProduct {
 };
 template <typename T> void launch_items_forward(ItemsProduct &p, int tile, hipStream_t s);  // tile 0: few rows
 template <typename T> void launch_items_gradient(ItemsProduct &p, int tile, hipStream_t s);
-// The parts of the rows joined: loss and lse
-struct JoinTails {
-  const float2 *parts;
-  uint32_t tiles, rows, width;
-  const void *x, *weight; // the rows that take part; the weight as it is given
-  uint32_t x_stride;
-  int64_t weight_stride;
-  Taken taken;
-  float *loss, *lse;
-};
-template <typename T> void launch_join_tails(const JoinTails &p, hipStream_t s);
-
 // Narrow matrices of 16-bit values: rows of up to kNarrow columns.  A block owns rows of one matrix, whose values it keeps in registers, and
 // goes through a range of the rows of the other.
 constexpr size_t kNarrow = 128;

@@ -29,6 +29,40 @@ __global__ __launch_bounds__(256) void count_rows(const int64_t *target, int64_t
   if (threadIdx.x == 0) chunks[blockIdx.x] = make_uint2(counts[0] + counts[1] + counts[2] + counts[3], max(max(sizes[0], sizes[1]), max(sizes[2], sizes[3])));
 }
 
+// The tiles' parts of ROWS rows joined by the other threads, each of which takes every so many tiles' parts of a row; then theirs, in pairs.  The target's
+// logit is one of those that went into the sum, to the bit, and the largest adds 1 to it: no loss is below zero.
+struct JoinTails {
+  const float2 *parts;
+  uint32_t tiles, rows;
+  Taken taken;
+  float *loss, *lse;
+};
+template <uint32_t ROWS> __global__ __launch_bounds__(256) void join_tails(JoinTails p) {
+  constexpr uint32_t GROUPS = 256 / ROWS, LOADS = 8;
+  __shared__ Tail tails[GROUPS][ROWS];
+  const uint32_t there = *p.taken.count, x = threadIdx.x % ROWS, y = threadIdx.x / ROWS, row0 = blockIdx.x * ROWS, r = row0 + x;
+  if (row0 >= there) return;
+  Tail t = {kLowest, 0.f};
+  for (uint32_t i = y; i < p.tiles; i += GROUPS * LOADS) {
+    float2 v[LOADS];
+#pragma unroll
+    for (uint32_t k = 0; k < LOADS; k++) v[k] = r < there && i + k * GROUPS < p.tiles ? p.parts[(uint64_t)(i + k * GROUPS) * p.rows + r] : make_float2(kLowest, 0.f);
+#pragma unroll
+    for (uint32_t k = 0; k < LOADS; k++) t = join(t, Tail{v[k].x, v[k].y});
+  }
+  tails[y][x] = t;
+  for (uint32_t n = GROUPS / 2; n; n /= 2) {
+    __syncthreads();
+    if (y < n) tails[y][x] = join(tails[y][x], tails[y + n][x]);
+  }
+  if (y || r >= there) return;
+  t = tails[0][x];
+  const float log_sum = log2f(t.sum), hit = p.taken.target[r] == kNoItem ? __builtin_nanf("") : p.taken.hits[r];
+  const uint32_t to = p.taken.row_of[r];
+  p.loss[to] = (log_sum + (t.most - hit)) * kLog2;
+  if (p.lse) p.lse[to] = hit != hit ? hit : (log_sum + t.most) * kLog2;
+}
+
 // of the workspace
 struct RowsSpace {
   size_t each, taken, chunks, x, bias, bytes; // each: of a number for every row
@@ -55,7 +89,7 @@ template <typename T, typename A> TakeRows take(const A &a, const float *dloss, 
   t.bias = a.bias, t.narrow = a.bias_dtype != HCTR_F32;
   t.rows = (uint32_t)rows, t.width = (uint32_t)width, t.items = (uint32_t)items;
   char *at = space + 256;
-  t.taken = {(uint32_t *)space, (float *)space + 4, (uint32_t *)at, (uint32_t *)(at + each), (float *)(at + 2 * each), (float *)(at + 3 * each),
+  t.taken = {(uint32_t *)space, (float *)space + 4, (uint32_t *)at, (uint32_t *)(at + each), (float *)(at + 2 * each), (float *)(at + 3 * each), (float *)(at + 3 * each),
              (float *)(space + need.taken + need.chunks + need.x)};
   t.to = space + need.taken + need.chunks;
   t.to_stride = (uint32_t)(up(width * sizeof(T), 16) / sizeof(T));
@@ -136,7 +170,11 @@ template <typename T> void forward(const hctr_items_args &a) {
     p.weight = {{w.at, nullptr}, w.stride, p.items, 0, 0};
     launch_items_forward<T>(p, plan.tile, s);
   }
-  launch_join_tails<T>({parts, (uint32_t)plan.tiles, t.rows, t.width, t.to, a.weight.data, t.to_stride, a.weight.stride, t.taken, a.loss, a.lse}, s);
+  // (few rows: more blocks)
+  const JoinTails j = {parts, (uint32_t)plan.tiles, t.rows, t.taken, a.loss, a.lse};
+  if (t.rows <= 1024) hipLaunchKernelGGL((join_tails<2>), dim3(div_up(t.rows, 2)), dim3(256), 0, s, j);
+  else hipLaunchKernelGGL((join_tails<8>), dim3(div_up(t.rows, 8)), dim3(256), 0, s, j);
+  HCTR_HIP(hipGetLastError());
 }
 
 // What is held of d at a time: large enough for every product to fill the card, and to make the sums that dx is joined from a small part

@@ -4,5 +4,4 @@ namespace hctr {
 template void launch_items_forward<float>(ItemsProduct &, int, hipStream_t);
 template void launch_items_gradient<float>(ItemsProduct &, int, hipStream_t);
 template void launch_take_rows<float>(const TakeRows &, hipStream_t);
-template void launch_join_tails<float>(const JoinTails &, hipStream_t);
 } // namespace hctr

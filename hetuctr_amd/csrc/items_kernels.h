@@ -73,6 +73,13 @@ __global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kNo
       t = join_lanes(t, 16);
       t = join_lanes(t, 32);
       if (l < 16) tails[wave_column / 64 * TILE + in] = t;
+      const uint32_t aim = (row0 + in < rows ? p.taken.target[row0 + in] : kNoItem) - (column0 + wave_column);
+      if (__ballot(aim < 64))
+#pragma unroll
+        for (int j = 0; j < P::kColumnTiles; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (aim == j * 16 + l / 16 * 4 + e) p.taken.hits[row0 + in] = sum[i][j][e];
     }
     __syncthreads();
     const uint32_t r = threadIdx.x;
@@ -155,6 +162,10 @@ template <typename T, int ROWS, int GROUPS, bool GRADIENT> __global__ __launch_b
 #pragma unroll
       for (uint32_t mask = 1; mask < QUADS; mask *= 2) tail = join_lanes(tail, mask);
       if (c == 0 && r < rows) p.parts[(uint64_t)blockIdx.x * p.rows + row0 + r] = make_float2(tail.most, tail.sum);
+      const uint32_t aim = (r < rows ? p.taken.target[row0 + r] : kNoItem) - (column0 + c);
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (aim == (uint32_t)e) p.taken.hits[row0 + r] = logit[0][e];
     } else {
       f32x4 d = {};
       if (r < rows) {
@@ -304,61 +315,6 @@ template <typename T> void launch_take_rows(const TakeRows &p, hipStream_t s) {
   const auto launch = [&](auto kernel, uint32_t rows) { hipLaunchKernelGGL(kernel, dim3(div_up(p.rows, rows) + div_up(p.items, kFilled)), dim3(256), 0, s, p); };
   if (p.rows <= kChunk) launch(take_rows<T, 2>, 2);
   else launch(take_rows<T, 8>, 8);
-  HCTR_HIP(hipGetLastError());
-}
-
-// The tiles' parts of ROWS rows joined by the other threads, each of which takes every so many tiles' parts of a row; then theirs, in pairs.  The
-// block's four waves multiply the rows with their targets' weights, for the logits that the losses are less by.
-template <typename T, uint32_t ROWS> __global__ __launch_bounds__(256) void join_tails(JoinTails p) {
-  constexpr uint32_t GROUPS = 256 / ROWS, LOADS = 8, WAVES = ROWS < 4 ? 4 / ROWS : 1; // waves for a row
-  constexpr int V = kVec<T>;
-  __shared__ Tail tails[GROUPS][ROWS];
-  __shared__ float hits[WAVES][ROWS];
-  const uint32_t there = *p.taken.count, x = threadIdx.x % ROWS, y = threadIdx.x / ROWS, row0 = blockIdx.x * ROWS, r = row0 + x;
-  if (row0 >= there) return;
-  for (uint32_t w = threadIdx.x / kWave; w < ROWS * WAVES; w += 4) {
-    const uint32_t i = w % ROWS, share = w / ROWS, item = row0 + i < there ? p.taken.target[row0 + i] : kNoItem;
-    float sum = 0.f;
-    if (item != kNoItem) {
-      const T *a = (const T *)p.x + (uint64_t)(row0 + i) * p.x_stride, *b = (const T *)p.weight + (int64_t)item * p.weight_stride;
-#pragma unroll 4
-      for (uint32_t c = (share * kWave + lane_id()) * V; c < p.width; c += WAVES * kWave * V) {
-        const Floats<V> u = floats<V>(*(const typename Packed<T, V>::type *)(a + c)), w = load_columns<V, Rows::kLong, false>(b, c, p.width);
-#pragma unroll
-        for (int e = 0; e < V; e++) sum = __builtin_fmaf(u.v[e], w.v[e], sum);
-      }
-    }
-#pragma unroll
-    for (int mask = 32; mask; mask /= 2) sum += __shfl_xor(sum, mask);
-    if (lane_id() == 0) hits[share][i] = item == kNoItem ? __builtin_nanf("") : share ? sum * kLog2E : __builtin_fmaf(sum, kLog2E, p.taken.bias[item]);
-  }
-  Tail t = {kLowest, 0.f};
-  for (uint32_t i = y; i < p.tiles; i += GROUPS * LOADS) {
-    float2 v[LOADS];
-#pragma unroll
-    for (uint32_t k = 0; k < LOADS; k++) v[k] = r < there && i + k * GROUPS < p.tiles ? p.parts[(uint64_t)(i + k * GROUPS) * p.rows + r] : make_float2(kLowest, 0.f);
-#pragma unroll
-    for (uint32_t k = 0; k < LOADS; k++) t = join(t, Tail{v[k].x, v[k].y});
-  }
-  tails[y][x] = t;
-  for (uint32_t n = GROUPS / 2; n; n /= 2) {
-    __syncthreads();
-    if (y < n) tails[y][x] = join(tails[y][x], tails[y + n][x]);
-  }
-  if (y || r >= there) return;
-  t = tails[0][x];
-  float hit = hits[0][x];
-#pragma unroll
-  for (uint32_t w = 1; w < WAVES; w++) hit += hits[w][x];
-  const float log_sum = log2f(t.sum);
-  const uint32_t to = p.taken.row_of[r];
-  p.loss[to] = (log_sum + (t.most - hit)) * kLog2;
-  if (p.lse) p.lse[to] = hit != hit ? hit : (log_sum + t.most) * kLog2;
-}
-template <typename T> void launch_join_tails(const JoinTails &p, hipStream_t s) {
-  // (few rows: more blocks)
-  if (p.rows <= 1024) hipLaunchKernelGGL((join_tails<T, 2>), dim3(div_up(p.rows, 2)), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((join_tails<T, 8>), dim3(div_up(p.rows, 8)), dim3(256), 0, s, p);
   HCTR_HIP(hipGetLastError());
 }
 

@@ -8,7 +8,7 @@
 // one.  That is the same tile in LDS, read across.
 //
 // Bound by the vector units: forward an exponential (a quarter of the others' rate) and four instructions a logit, 73 % of the cycles beside 35 %
-// in the matrix cores.  4096 rows, a million items of 128 bfloat16: 1.27 ms (0.83 PFLOP/s), by tiles, each of which joins lanes and waves
+// in the matrix cores.  4096 rows, a million items of 128 bfloat16: 1.19 ms (0.88 PFLOP/s), by tiles, each of which joins lanes and waves
 // for itself, 2.75; dx 2.0 and the weights' gradient 2.1, with d in memory 8.9 together.  Of 32 columns 0.78, 0.90 and 0.99.
 #pragma once
 #include "items.h"
@@ -244,6 +244,25 @@ __global__ __launch_bounds__(256, narrow_share(KS * 32, MODE != Narrow::kForward
       const uint32_t r = first + i * 16 + l;
       if (l < 16 && r < owned) p.parts[(uint64_t)range * p.rows + r] = make_float2(t.most, t.sum);
     }
+    // The logits of the rows' targets, once more: the products of the rows with the 16 items that they aim at, by the same instructions in the same
+    // order, so that they are the logits above to the bit; what a row has of its own lies on the diagonal.  (Picked out in the loop they would
+    // cost two instructions a logit where there are few items.)
+    if (range == 0)
+#pragma unroll
+      for (int i = 0; i < OI; i++) {
+        const uint32_t r = first + i * 16 + l % 16, item = r < owned ? p.taken.target[r] : kNoItem;
+        f32x4 sum = {};
+#pragma unroll
+        for (int kk = 0; kk < KS; kk++) {
+          const uint32_t c = (kk * 4 + l / 16) * 8;
+          Fragment<T> f;
+          f.v = (T)0;
+          if (item != kNoItem && c < p.width) f.v = *(const typename Fragment<T>::type *)(p.weight + (int64_t)item * p.weight_stride + c * 2);
+          sum = multiply<T>(f, mine[i][kk], sum);
+        }
+        const float own = l % 4 == 0 ? sum[0] : l % 4 == 1 ? sum[1] : l % 4 == 2 ? sum[2] : sum[3];
+        if (l % 16 / 4 == l / 16 && item != kNoItem) p.taken.hits[r] = __builtin_fmaf(own, kLog2E, p.taken.bias[item]);
+      }
   } else {
     const float back = p.partial ? 1.f : p.taken.scale[1];
     const uint32_t columns = (p.width + 3) / 4 * 4;

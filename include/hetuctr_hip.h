@@ -359,7 +359,7 @@ size_t hctr_gated_linear_backward_workspace(const hctr_gated_grad_args *a);
 
 /* Softmax cross entropy over `items`: with l = x weight^T + bias, rows x items, which is never stored,
  *     lse[r] = log(sum over the items of exp(l[r])),   loss[r] = lse[r] - l[r][target[r]]
- * A row whose target is ignore_index takes no part, whatever x holds there: its loss and lse are 0.  One whose target is neither that nor
+ * loss is not below zero, not by rounding either.  A row whose target is ignore_index takes no part, whatever x holds there: its loss and lse are 0.  One whose target is neither that nor
  * an item gets NaN for both.  x and weight are of `dtype`, bias (`items` elements, NULL: none) is HCTR_F32 or dtype.  An
  * item whose bias is -infinity does not count; if none is left, lse is -infinity and loss NaN.  lse may be NULL. */
 typedef struct hctr_items_args {

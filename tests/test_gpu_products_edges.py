@@ -122,3 +122,27 @@ def test_a_captured_gradient_finds_its_scale_again():
             assert torch.equal(g, w)
         for g, (value, slack) in zip(got, gated_gradient_in_range(dh, x, gate, up, gw, uw, "silu")):
             check_half(g, value, slack, "size %g" % size)
+
+
+# ---- losses next to nothing ------------------------------------------------------------------------------------------------
+# rows, width, items: narrow rows of 16 bits, few rows, few but long ones, tiles of each size
+CERTAIN = [(1, 24, 7), (20, 64, 900), (700, 128, 3000), (3000, 33, 5000), (3, 300, 2000), (32, 1000, 700), (40, 4096, 100), (90, 200, 700), (1500, 260, 1500),
+           (6000, 520, 6000)]
+
+
+@gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows, width, items", CERTAIN)
+def test_a_loss_is_never_below_zero(rows, width, items, kind):
+    # rows that are all but certain of their target: its logit is some hundreds, and the loss the little that the others add
+    weight = values((items, width), kind, 80, width ** -0.5)
+    target = torch.randint(0, items, (rows,), generator=torch.Generator().manual_seed(81)).cuda()
+    x = (wide(weight)[target] * torch.linspace(1, 400, rows, device="cuda", dtype=torch.float64)[:, None]).to(TYPES[kind])
+    for bias in (None, values(items, "f32", 82)):
+        loss, lse = nn.linear_cross_entropy(x, weight, target, bias, stats=True)
+        assert (loss >= 0).all()
+        for got, (value, slack), what in zip((loss, lse), ref.cross_entropy(wide(x), wide(weight), wide(bias), target, -100), ("loss", "lse")):
+            ref.check(got, value, slack, what)
+        # of one item there is nothing to lose, whatever its logit
+        one = nn.linear_cross_entropy(x, weight[:1], torch.zeros_like(target), None if bias is None else bias[:1])
+        assert (one == 0).all()
