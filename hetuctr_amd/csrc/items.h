@@ -50,7 +50,7 @@ struct ItemsProduct {
   uint32_t few_stride;
   uint32_t rows, width, items, first; // items first .. first + items - 1 of all
   uint32_t row_tiles, column_tiles, band;
-  uint32_t column_from, columns_here; // the tiles of a launch
+  uint32_t column_from, columns_here; // the tiles of a launch (few rows: from where on)
   Taken taken;
   float2 *parts; // forward: [column tiles][rows]: the largest logit and the sum of exponentials less it, both in units of log 2
   void *d;       // gradient: [rows][d_stride]

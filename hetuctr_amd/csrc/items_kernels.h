@@ -5,6 +5,7 @@
 #include "few_rows.h"
 #include "items.h"
 #include "items_tail.h"
+#include "launch_cut.h"
 
 namespace hctr {
 
@@ -138,7 +139,7 @@ template <typename T, int ROWS, int GROUPS, bool GRADIENT> __global__ __launch_b
   typedef FewRows<T, ROWS, GROUPS> F;
   constexpr uint32_t QUADS = F::kWeights / 4; // of a row
   __shared__ typename F::Sums sums[F::kSums];
-  const uint32_t count = *p.taken.count, row0 = blockIdx.y * ROWS, column0 = blockIdx.x * F::kWeights;
+  const uint32_t count = *p.taken.count, row0 = blockIdx.y * ROWS, column = p.column_from + blockIdx.x, column0 = column * F::kWeights;
   if (row0 >= count) return;
   const uint32_t rows = min(count - row0, (uint32_t)ROWS);
   const T *groups[F::kGroups];
@@ -161,7 +162,7 @@ template <typename T, int ROWS, int GROUPS, bool GRADIENT> __global__ __launch_b
       Tail tail = tail_of(logit);
 #pragma unroll
       for (uint32_t mask = 1; mask < QUADS; mask *= 2) tail = join_lanes(tail, mask);
-      if (c == 0 && r < rows) p.parts[(uint64_t)blockIdx.x * p.rows + row0 + r] = make_float2(tail.most, tail.sum);
+      if (c == 0 && r < rows) p.parts[(uint64_t)column * p.rows + row0 + r] = make_float2(tail.most, tail.sum);
       const uint32_t aim = (r < rows ? p.taken.target[row0 + r] : kNoItem) - (column0 + c);
 #pragma unroll
       for (int e = 0; e < 4; e++)
@@ -190,7 +191,11 @@ template <typename T, bool GRADIENT> void launch_items(ItemsProduct &p, int tile
   if (!tile) {
     const auto launch = [&](auto kernel, uint32_t rows, int groups) {
       p.column_tiles = div_up(p.items, 16 * groups);
-      hipLaunchKernelGGL(kernel, dim3(p.column_tiles, div_up(p.rows, rows)), dim3(FewRows<T, 16, 2>::kThreads), 0, s, p);
+      const uint32_t threads = FewRows<T, 16, 2>::kThreads, most = most_blocks(threads);
+      for (p.column_from = 0; p.column_from < p.column_tiles; p.column_from += most) {
+        hipLaunchKernelGGL(kernel, dim3(std::min(p.column_tiles - p.column_from, most), div_up(p.rows, rows)), dim3(threads), 0, s, p);
+        HCTR_HIP(hipGetLastError());
+      }
     };
     if (few_groups(p.rows, p.items) == 2) {
       if (p.rows <= 16) launch(items_few<T, 16, 2, GRADIENT>, 16, 2);
@@ -201,8 +206,8 @@ template <typename T, bool GRADIENT> void launch_items(ItemsProduct &p, int tile
     }
   } else {
     p.row_tiles = div_up(p.rows, tile), p.column_tiles = div_up(p.items, tile);
-    // (a launch has fewer than 2^32 threads; a million rows and a million items are more)
-    const uint32_t most = std::max<uint32_t>(1, ((1u << 23) - 1) / p.row_tiles);
+    // (a million rows and a million items are more tiles than a launch has)
+    const uint32_t most = std::max<uint32_t>(1, most_blocks(512) / p.row_tiles);
     for (p.column_from = 0; p.column_from < p.column_tiles; p.column_from += p.columns_here) {
       p.columns_here = std::min(p.column_tiles - p.column_from, most);
       const dim3 blocks(p.row_tiles * p.columns_here);
@@ -212,7 +217,6 @@ template <typename T, bool GRADIENT> void launch_items(ItemsProduct &p, int tile
       HCTR_HIP(hipGetLastError());
     }
   }
-  HCTR_HIP(hipGetLastError());
 }
 template <typename T> void launch_items_forward(ItemsProduct &p, int tile, hipStream_t s) { launch_items<T, false>(p, tile, s); }
 template <typename T> void launch_items_gradient(ItemsProduct &p, int tile, hipStream_t s) { launch_items<T, true>(p, tile, s); }

@@ -5,6 +5,10 @@
 
 namespace hctr {
 
+// The most blocks along one dimension of a launch, which has fewer than 2^32 threads there; a multiple of eight, so that a block's XCD is the same
+// whether its number is counted from a launch's beginning or from that of the launch before.
+constexpr uint32_t most_blocks(uint32_t threads) { return (uint32_t)(((1ull << 32) - 1) / threads / 8 * 8); }
+
 // Record k has blocks first[k] .. first[k] + blocks[k) of the launch, as many as its own batch needs.  (Cut for the largest batch
 // times the records instead, a launch for one large batch beside seven small ones is seven eighths idle blocks, and may
 // exceed the 2^32 threads a launch can have where a launch per record did not.  Eight shards, one batch of 1.7 M keys x 128

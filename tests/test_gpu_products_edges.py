@@ -146,3 +146,29 @@ def test_a_loss_is_never_below_zero(rows, width, items, kind):
         # of one item there is nothing to lose, whatever its logit
         one = nn.linear_cross_entropy(x, weight[:1], torch.zeros_like(target), None if bias is None else bias[:1])
         assert (one == 0).all()
+
+
+# ---- more blocks than a launch has -------------------------------------------------------------------------------------------
+@gpu
+def test_few_rows_and_more_items_than_a_launch_has_blocks():
+    # one row of one column, whose logits are 0 but for a few items, at both ends and where one launch ends and the next begins
+    items = 2 ** 29 + 70
+    weight = torch.zeros((items, 1), device="cuda")
+    places = torch.tensor([0, 2 ** 29 - 512, 2 ** 29 - 1, 2 ** 29, 2 ** 29 + 69], device="cuda")
+    logits = torch.tensor([15.0, 16.0, 14.0, 15.5, 16.5], device="cuda")
+    weight[places, 0] = logits
+    x = torch.ones((1, 1), device="cuda")
+    total = items - len(places) + wide(logits).exp().sum().item()
+    for place, logit in zip(places.tolist(), logits.tolist()):
+        loss, lse = nn.linear_cross_entropy(x, weight, torch.tensor([place], device="cuda"), stats=True)
+        # (sums of 2^29 terms, most of them 1: whole numbers below 2^24, then joined in pairs)
+        assert abs(lse.item() - math.log(total)) < 128 * ref.U * math.log(total) and abs(loss.item() - (math.log(total) - logit)) < 128 * ref.U * math.log(total)
+    dx, dweight, _ = nn.linear_cross_entropy_backward(torch.ones(1, device="cuda"), x, weight, torch.tensor([place], device="cuda"), lse)
+    p = wide(logits).exp() / total
+    p_slack = p * (16 + 4 * 20 + 128 * 20) * ref.U          # an exponential of up to 20, and lse as it was given
+    assert abs(dx.item() - ((p * wide(logits)).sum().item() - logit)) < (p_slack * wide(logits)).sum().item() + 256 * ref.U * logit
+    hit = torch.zeros_like(p)
+    hit[-1] = 1
+    ref.check(dweight[places, 0], p - hit, p_slack + 2 * ref.U, "dweight")
+    rest = dweight[1:2 ** 29 - 512]
+    assert rest.min() == rest.max() and dweight[-2] == rest[0] and abs(rest[0].item() * total - 1) < 2656 * ref.U
