@@ -308,11 +308,10 @@ template <typename T> __global__ __launch_bounds__(256) void gated_rescale(Gated
 
 template <typename T> void launch_gated(GatedForward &p, int tile, hipStream_t s) {
   p.row_tiles = div_up(p.rows, tile), p.column_tiles = div_up(p.hidden, tile / 2);
-  HCTR_CHECK((uint64_t)p.row_tiles * p.column_tiles * 512 < (1ull << 32), "gated linear: too many tiles");
-  const dim3 blocks(p.row_tiles * p.column_tiles, p.splits);
-  if (tile == 256) hipLaunchKernelGGL((gated_product<T, 256>), blocks, dim3(512), 0, s, p);
-  else if (tile == 128) hipLaunchKernelGGL((gated_product<T, 128>), blocks, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((gated_product<T, 64>), blocks, dim3(128), 0, s, p);
+  const dim3 blocks(p.row_tiles * p.column_tiles, p.splits), threads(tile_threads(p.row_tiles, p.column_tiles, tile, "gated linear"));
+  if (tile == 256) hipLaunchKernelGGL((gated_product<T, 256>), blocks, threads, 0, s, p);
+  else if (tile == 128) hipLaunchKernelGGL((gated_product<T, 128>), blocks, threads, 0, s, p);
+  else hipLaunchKernelGGL((gated_product<T, 64>), blocks, threads, 0, s, p);
   HCTR_HIP(hipGetLastError());
   if (p.partial) {
     const uint64_t quads = (uint64_t)p.rows * ((p.hidden + 3) / 4);

@@ -1,5 +1,7 @@
 // What the operators made of matrix products share: results and partial sums, the choice of tiles, and the kernels around the products.
 #pragma once
+#include <string>
+
 #include "../../include/hetuctr_hip.h"
 #include "matmul.h"
 
@@ -62,6 +64,12 @@ template <typename T> void launch_forward_product(ProductArgs &p, int tile, hipS
 // both kAcross
 template <typename T> void launch_across_product(ProductArgs &p, int tile, hipStream_t s);
 template <typename T> void launch_join(const ProductArgs &p, hipStream_t s);
+// The threads of a block that makes a tile.  A launch has fewer than 2^32: two for each row and column of tiles, so that only results that no card
+// holds have too many (of a gated layer, whose tiles of 128 are 64 columns of the result, 2^37 values).
+inline uint32_t tile_threads(uint32_t row_tiles, uint32_t column_tiles, int tile, const char *what) {
+  HCTR_CHECK((uint64_t)row_tiles * column_tiles * (2 * tile) < (1ull << 32), std::string(what) + ": too many tiles");
+  return 2 * tile;
+}
 
 // ---- matrices that do not begin, or end their rows, at a multiple of 16 bytes, are laid out once more -------------------------
 struct Layout {

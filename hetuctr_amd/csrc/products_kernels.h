@@ -73,11 +73,10 @@ template <typename T> __global__ __launch_bounds__(256) void join_parts(const fl
 
 template <typename T, Lies LA, Lies LB, Second SB> void launch_product(ProductArgs &p, int tile, hipStream_t s) {
   p.row_tiles = div_up(p.rows, tile), p.column_tiles = div_up(p.columns, tile);
-  const dim3 blocks(p.row_tiles * p.column_tiles, p.splits);
-  HCTR_CHECK((uint64_t)p.row_tiles * p.column_tiles * 512 < (1ull << 32), "product: too many tiles");
-  if (tile == 256) hipLaunchKernelGGL((product<T, LA, LB, SB, 256>), blocks, dim3(512), 0, s, p);
-  else if (tile == 128) hipLaunchKernelGGL((product<T, LA, LB, SB, 128>), blocks, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((product<T, LA, LB, SB, 64>), blocks, dim3(128), 0, s, p);
+  const dim3 blocks(p.row_tiles * p.column_tiles, p.splits), threads(tile_threads(p.row_tiles, p.column_tiles, tile, "product"));
+  if (tile == 256) hipLaunchKernelGGL((product<T, LA, LB, SB, 256>), blocks, threads, 0, s, p);
+  else if (tile == 128) hipLaunchKernelGGL((product<T, LA, LB, SB, 128>), blocks, threads, 0, s, p);
+  else hipLaunchKernelGGL((product<T, LA, LB, SB, 64>), blocks, threads, 0, s, p);
   HCTR_HIP(hipGetLastError());
 }
 template <typename T> void launch_forward_product(ProductArgs &p, int tile, hipStream_t s) {

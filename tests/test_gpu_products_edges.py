@@ -172,3 +172,39 @@ def test_few_rows_and_more_items_than_a_launch_has_blocks():
     ref.check(dweight[places, 0], p - hit, p_slack + 2 * ref.U, "dweight")
     rest = dweight[1:2 ** 29 - 512]
     assert rest.min() == rest.max() and dweight[-2] == rest[0] and abs(rest[0].item() * total - 1) < 2656 * ref.U
+
+
+@gpu
+@pytest.mark.parametrize("rows, width, hidden", [(2 ** 30 + 5, 8, 8), (2 ** 31 - 65536 - 50, 1, 1)])
+def test_more_rows_of_a_gated_layer_than_large_tiles_are_in_a_launch(rows, width, hidden):
+    # tiles of 64 rows, and of 128: with the threads that they have they are a launch, with the 512 that a tile of 256 has they would be 2^32 threads and
+    # more.  A row's results hang on nothing but the row, so that a few at a time say what all have to be.
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 80 GiB of free memory")
+    x = torch.empty((rows, width), dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(5))
+    gw, uw = values((hidden, width), "bf16", 6), values((hidden, width), "bf16", 7)
+    h = nn.gated_linear(x, gw, uw)
+    for first in (0, 2 ** 23, 2 ** 29 - 3000, 2 ** 30 - 777, rows // 2, 2 ** 31 - 2 ** 20, rows - 4000):
+        assert torch.equal(h[first:first + 4000], nn.gated_linear(x[first:first + 4000], gw, uw))
+    del h, x
+    torch.cuda.empty_cache()
+
+
+@gpu
+def test_more_rows_of_a_gated_gradient_than_large_tiles_are_in_a_launch():
+    # 2^23 tiles of 64 rows: 2^32 threads if each had 512
+    rows = 2 ** 29 + 100
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 180 << 30:
+        pytest.skip("needs 180 GiB of free memory")
+    dh = torch.empty((rows, 1), dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(8))
+    gw, uw, gate, up = (values((1, 1), "bf16", 9 + i) for i in range(4))
+    every = lambda t, n: t.expand(n, 1)                     # one row again and again
+    dx, dgate_weight, dup_weight, _, _ = nn.gated_linear_backward(dh, every(gw * 0, rows), every(gate, rows), every(up, rows), gw, uw)
+    for first in (0, 2 ** 23 - 5, 2 ** 28, rows - 4000):
+        want = nn.gated_linear_backward(dh[first:first + 4000], every(gw, 4000), every(gate, 4000), every(up, 4000), gw, uw)[0]
+        assert torch.equal(dx[first:first + 4000], want) and want.count_nonzero() > 3000
+    assert (dgate_weight == 0).all() and (dup_weight == 0).all()
+    del dh, dx
+    torch.cuda.empty_cache()
