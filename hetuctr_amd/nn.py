@@ -107,11 +107,14 @@ class _LayerNorm(torch.autograd.Function):
         ctx.drop = drop
         ctx.save_for_backward(x, weight, bias, mean, rstd, step_tensor)
         ctx.mark_non_differentiable(mean, rstd)
+        ctx.set_materialize_grads(False)        # or zeros are made for mean and rstd
         return y, mean, rstd
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, _mean, _rstd):
+        if dy is None:
+            return (None,) * 7
         x, weight, bias, mean, rstd, _ = ctx.saved_tensors
         dx, dweight, dbias = _run(_native.backward, x, False, dy, None, x, mean, rstd, weight, bias, ctx.drop, True,
                                   *ctx.needs_input_grad[1:3])
@@ -190,11 +193,14 @@ class _GatedLinear(torch.autograd.Function):
         ctx.activation = activation
         ctx.save_for_backward(x, gate, up, gate_weight, up_weight, gate_bias, up_bias)
         ctx.mark_non_differentiable(gate, up)
+        ctx.set_materialize_grads(False)        # or matrices of zeros are made for gate and up
         return h, gate, up
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh, _gate, _up):
+        if dh is None:
+            return (None,) * 6
         return (*_run(_native.gated_backward, dh, dh, *ctx.saved_tensors, ctx.activation, *ctx.needs_input_grad[:5]), None)
 
 
@@ -226,11 +232,14 @@ class _LinearCrossEntropy(torch.autograd.Function):
         ctx.ignore_index = ignore_index
         ctx.save_for_backward(x, weight, target, lse, bias)
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return loss, lse
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss, _lse):
+        if dloss is None:
+            return (None,) * 5
         x, weight, target, lse, bias = ctx.saved_tensors
         dx, dweight, dbias = _run(_native.items_backward, dloss, dloss, x, weight, target, lse, bias, ctx.ignore_index,
                                   *(ctx.needs_input_grad[i] for i in (0, 1, 3)))

@@ -208,3 +208,43 @@ def test_more_rows_of_a_gated_gradient_than_large_tiles_are_in_a_launch():
     assert (dgate_weight == 0).all() and (dup_weight == 0).all()
     del dh, dx
     torch.cuda.empty_cache()
+
+
+# ---- what autograd makes besides --------------------------------------------------------------------------------------------
+def memory_of(f):
+    """The most memory that f takes on top of what there was"""
+    f()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    f()
+    return torch.cuda.max_memory_allocated() - before
+
+
+@gpu
+def test_autograd_takes_no_more_memory_than_the_calls():
+    # gate and up are of 16 MiB each, lse, mean and rstd of 4 MiB: none is the place for zeros that stand for a gradient that there is not
+    dh, *inputs = gated_inputs(2048, 64, 4096, "bf16", "none")[:4]
+    h, gate, up = nn.gated_linear(*inputs, saved=True)
+    direct = memory_of(lambda: nn.gated_linear_backward(dh, inputs[0], gate, up, *inputs[1:]))
+    leaves = [t.requires_grad_() for t in inputs]
+    for saved in (False, True):
+        out = nn.gated_linear(*leaves, saved=saved)
+        out = out[0] if saved else out
+        assert memory_of(lambda: torch.autograd.grad(out, leaves, dh, retain_graph=True)) < direct + (1 << 20)
+    x, weight = values((1 << 20, 8), "bf16", 90), values((64, 8), "bf16", 91)
+    target = torch.arange(1 << 20, device="cuda") % 64
+    loss, lse = nn.linear_cross_entropy(x, weight, target, stats=True)
+    dloss = torch.ones_like(loss)
+    direct = memory_of(lambda: nn.linear_cross_entropy_backward(dloss, x, weight, target, lse))
+    leaves = [x.requires_grad_(), weight.requires_grad_()]
+    for stats in (False, True):
+        out = nn.linear_cross_entropy(*leaves, target, stats=stats)
+        out = out[0] if stats else out
+        assert memory_of(lambda: torch.autograd.grad(out, leaves, dloss, retain_graph=True)) < direct + (1 << 20)
+    x = values((1 << 20, 8), "f32", 92)
+    y, mean, rstd = nn.layer_norm(x, stats=True)
+    direct = memory_of(lambda: nn.layer_norm_backward(x, x, mean, rstd))
+    leaf = x.clone().requires_grad_()
+    out = nn.layer_norm(leaf)
+    assert memory_of(lambda: torch.autograd.grad(out, leaf, x, retain_graph=True)) < direct + (1 << 20)
