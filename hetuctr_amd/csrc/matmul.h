@@ -1,4 +1,4 @@
-// Products of matrices on the matrix cores, as the kernels of matmul_*.hip build them: tiles that go from memory to LDS past the
+// Products of matrices on the matrix cores, as the kernels of gated_kernels.h, items_kernels.h and products_kernels.h build them: tiles that go from memory to LDS past the
 // registers, fragments from there, sums in 32 bits, and an epilogue that takes them.
 #pragma once
 #include <type_traits>
@@ -36,8 +36,9 @@ constexpr uint32_t kNowhere = 0x80000000u; // an offset behind every buffer: the
 template <typename T> constexpr int kStep = kStepBytes / (int)sizeof(T); // of k that a tile holds
 
 // 16 bytes per lane from base + offset to LDS, where a wave's lanes lie one behind the other from `lds`, the same address in all
-// lanes.  Not the builtin: the compiler would wait for every such load before any read of LDS.  (m0 is the compiler's own, which sets it right
-// before each use and keeps nothing there.)
+// lanes.  Not the builtin: the compiler would wait for every such load before any read of LDS.  The list of what is overwritten cannot name m0, which
+// is not a register that the compiler gives to values (it warns, and builds the same code): nothing of it may be kept there across this, which
+// tests/test_kernel_m0.py reads from the built library.
 __device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t offset, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc) : "memory");
 }
