@@ -181,7 +181,7 @@ template <typename T> __device__ __forceinline__ f32x4 multiply(const Fragment<T
 }
 
 // A float is the sum of three bfloat16: the one nearest to it, the one nearest to what is left, and what is then left, which has eight bits at
-// most.  Of the nine products of two such sums the six largest are made; the others are below 2^-25 of the floats' product together.
+// most.  Of the nine products of two such sums the six largest are made; the others are below 2^-24 of the floats' product together (at most 0.9932 of that, over all of them).
 // They take six times a sixteenth of the matrix cores' time for floats, and five or six instructions for each float.  us, 8192 x 8192 x 2048 in
 // the three layouts: 2095, 2043 and 2098 with products of floats (131 to 135 TFLOP/s, of the 157 that the cores could do at most), 1573,
 // 1466 and 1476 so.  An infinity becomes a NaN on the way, a float below 2^-110 loses some of its bits, one beyond 2^128 - 2^119 is as

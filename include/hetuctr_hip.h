@@ -317,7 +317,7 @@ size_t hctr_layer_norm_workspace(size_t rows, size_t width);
  * are device memory, 16-byte aligned, in use until the work is done, and of as many bytes as the function beside each
  * call says for the same arguments (whose stream and workspace it does not read; pointers it looks at, but does not follow;
  * (size_t)-1 where the call would refuse them for their sizes or types).
- * Products run on the matrix cores: 16-bit values are multiplied exactly, floats to 25 bits or better (as sums of three bfloat16: not below
+ * Products run on the matrix cores: 16-bit values are multiplied exactly, floats to 2^-24 of the product (as sums of three bfloat16: not below
  * 2^-110, and an infinity may make a NaN); sums are held in 32 bits.
  * Matrices of weights are [columns of the result] x [columns of x], as rows.  rows and items < 2^31 - 65536 (rows of a
  * cross entropy <= 2^26); width, hidden <= 2^20.
