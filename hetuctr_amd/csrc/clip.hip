@@ -199,28 +199,29 @@ void check(const hctr_clip_args &a) {
   }
 }
 
-// No result may lie where another result or another gradient does.
+// No result, the norm among them, may lie where another result, another gradient or the norm that is given does: blocks read these while others write.
 void check_places(const hctr_clip_args &a) {
   struct Span {
     uintptr_t from, to;
-    size_t of;
     bool written;
   };
   std::vector<Span> spans;
-  spans.reserve(2 * a.count);
+  spans.reserve(2 * a.count + 2);
   for (size_t i = 0; i < a.count; i++) {
     const hctr_gradient &g = a.gradients[i];
     if (!g.count) continue;
     HCTR_CHECK(g.values && g.into, "clip gradients: null pointer");
     const size_t bytes = g.count * size_of(g.dtype);
-    spans.push_back({(uintptr_t)g.into, (uintptr_t)g.into + bytes, i, true});
-    if (g.values != g.into) spans.push_back({(uintptr_t)g.values, (uintptr_t)g.values + bytes, i, false});
+    spans.push_back({(uintptr_t)g.into, (uintptr_t)g.into + bytes, true});
+    if (g.values != g.into) spans.push_back({(uintptr_t)g.values, (uintptr_t)g.values + bytes, false});
   }
+  if (a.given) spans.push_back({(uintptr_t)a.given, (uintptr_t)a.given + sizeof(float), false});
+  if (a.norm && a.norm != a.given) spans.push_back({(uintptr_t)a.norm, (uintptr_t)a.norm + sizeof(float), true});
   const auto before = [](const Span &x, const Span &y) { return x.from < y.from; };
   if (!std::is_sorted(spans.begin(), spans.end(), before)) std::sort(spans.begin(), spans.end(), before);
   uintptr_t read = 0, written = 0; // where what was seen so far ends
   for (const Span &s : spans) {
-    HCTR_CHECK(s.from >= written && (!s.written || s.from >= read), "clip gradients: a result lies where another gradient or result does");
+    HCTR_CHECK(s.from >= written && (!s.written || s.from >= read), "clip gradients: a result lies where another gradient or result, or the norm, does");
     if (s.written) written = std::max(written, s.to);
     else read = std::max(read, s.to);
   }

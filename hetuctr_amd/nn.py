@@ -276,7 +276,7 @@ def gradient_norm(gradients):
 def clip_gradients(gradients, max_norm, *, norm=None, into=None):
     """Multiplies every gradient by min(1, max_norm / norm), in place or `into` tensors of the same types and shapes, and returns the norm: that
     of gradient_norm, or the one that is given (a float32 on the GPU: where several GPUs hold a part of the gradients
-    each).  No result may lie where another gradient or result does; each holds its values one behind the other.  Where the norm is
+    each).  No result may lie where another gradient or result, or `norm`, does; each holds its values one behind the other.  Where the norm is
     not finite, what is multiplied is not either, or zero."""
     gradients = list(gradients)
     into = gradients if into is None else list(into)

@@ -399,7 +399,7 @@ size_t hctr_linear_cross_entropy_backward_workspace(const hctr_items_grad_args *
 
 /* norm = the 2-norm of all `count` gradients together (squares and their sums in 64 bits), a float in device memory.
  * hctr_clip_gradients also writes each gradient times min(1, max_norm / norm) to its `into`, which may be the gradient's own place (where
- * nothing is written if nothing changes) but may not overlap any other; if `given` is not NULL, the norm is taken from there (device memory; as
+ * nothing is written if nothing changes) but may not overlap any other, nor a norm; if `given` is not NULL, the norm is taken from there (device memory; as
  * when several GPUs hold a part each), and norm may be NULL.  A norm that is not finite makes every result so or zero, as the product says.
  * values: elements, one behind the other; into: of the same type.  The array of hctr_gradient is host memory, read before the call returns. */
 typedef struct hctr_gradient {
