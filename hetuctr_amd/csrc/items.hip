@@ -177,9 +177,9 @@ template <typename T> void forward(const hctr_items_args &a) {
   HCTR_HIP(hipGetLastError());
 }
 
-// What is held of d at a time: large enough for every product to fill the card, and to make the sums that dx is joined from a small part
-// of what is moved.
-constexpr size_t kPieceBytes = (size_t)512 << 20;
+// What is held of d at a time, at most: large enough for every product to fill the card, and to make the sums that dx is joined from a small part
+// of what is moved.  For that it is d of kPieceItems items at least, however many rows there are.
+constexpr size_t kPieceItems = 2048, kPieceBytes = (size_t)512 << 20;
 
 struct BackwardPlan {
   Way way;
@@ -204,7 +204,7 @@ BackwardPlan plan_of(const hctr_items_grad_args &a) {
     p.bytes = p.rows + p.acc + p.parts + p.sums + p.weight;
     return p;
   }
-  p.piece = std::min(up(a.items, 64), std::min<size_t>(kMaxStride / size, std::max<size_t>(2048, kPieceBytes / (rows * size) / 256 * 256)));
+  p.piece = std::min(up(a.items, 64), std::min<size_t>(kMaxStride / size, std::max<size_t>(kPieceItems, kPieceBytes / (rows * size) / 256 * 256)));
   p.pieces = (a.items + p.piece - 1) / p.piece;
   p.d_stride = p.piece;
   const size_t some = std::min(a.items, p.piece);

@@ -250,7 +250,8 @@ def linear_cross_entropy(x, weight, target, bias=None, *, ignore_index=-100, sta
     """The softmax cross entropy of x @ weight.T + bias with the items that `target` names, float32, one for each row, without a matrix of
     logits in memory.  weight is [items, width], of the type of x; bias is float32 or of that type; target is int64, of
     the shape of the result.  Rows whose target is `ignore_index` take no part, whatever x holds there: their loss is 0.  A
-    target that is neither that nor an item gives NaN.  With `stats` returns (loss, log of the sum of exponentials)."""
+    target that is neither that nor an item gives NaN.  An item whose bias is below -1e30 does not count.  With `stats` returns (loss, log of the
+    sum of exponentials)."""
     if _wants_gradient(x, weight, bias):
         out = _LinearCrossEntropy.apply(x, weight, target, bias, ignore_index)
     else:

@@ -361,7 +361,8 @@ size_t hctr_gated_linear_backward_workspace(const hctr_gated_grad_args *a);
  *     lse[r] = log(sum over the items of exp(l[r])),   loss[r] = lse[r] - l[r][target[r]]
  * loss is not below zero, not by rounding either.  A row whose target is ignore_index takes no part, whatever x holds there: its loss and lse are 0.  One whose target is neither that nor
  * an item gets NaN for both.  x and weight are of `dtype`, bias (`items` elements, NULL: none) is HCTR_F32 or dtype.  An
- * item whose bias is -infinity does not count; if none is left, lse is -infinity and loss NaN.  lse may be NULL. */
+ * item whose bias is -infinity, or below -1e30, does not count; if none is left, lse is -infinity and loss NaN.  Logits of more than 2^127 are infinite.
+ * lse may be NULL. */
 typedef struct hctr_items_args {
   size_t rows, width, items;
   hctr_matrix x, weight;
@@ -380,7 +381,8 @@ size_t hctr_linear_cross_entropy_workspace(const hctr_items_args *a);
 /* Its gradient, given that of loss and the lse that the forward pass left:
  *     d = (exp(l - lse) - [item is the target]) * dloss,   dx = d weight,  dweight = d^T x,  dbias: the sums of d over the rows
  * in pieces of the items, of which d is held, rounded to dtype (to 16 bits after a factor that brings the largest dloss to 2^13, by which the
- * results are divided).  Ignored rows have zeros in dx and no part in the others.  Any result may be missing (data NULL). */
+ * results are divided).  A piece is 512 MiB of d at most, or 2048 items where these are more.  Ignored rows have zeros in dx and no part in the
+ * others.  Any result may be missing (data NULL). */
 typedef struct hctr_items_grad_args {
   size_t rows, width, items;
   hctr_matrix x, weight, dx, dweight;
