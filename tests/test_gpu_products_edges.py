@@ -248,3 +248,29 @@ def test_autograd_takes_no_more_memory_than_the_calls():
     leaf = x.clone().requires_grad_()
     out = nn.layer_norm(leaf)
     assert memory_of(lambda: torch.autograd.grad(out, leaf, x, retain_graph=True)) < direct + (1 << 20)
+
+
+# ---- slopes of the cross entropy in half precision -----------------------------------------------------------------------------
+# dloss, x and weights: slopes that would be below the smallest half, or beyond the largest, if they were not scaled, and of dx or dweight, or both, results in between
+DLOSSES = {"small, for dx": (1e-7, 1e-3, 1e3), "small, for dweight": (1e-7, 1e3, 1e-3), "smaller": (1e-11, 300.0, 3e-3), "large, for dx": (1e6, 1.0, 1e-3), "large, for dweight": (1e6, 1e-3, 1.0),
+           "larger": (1e9, 3e-5, 1e-4)}
+
+
+@gpu
+@pytest.mark.parametrize("sizes", DLOSSES)
+@pytest.mark.parametrize("rows, width, items", [(20, 64, 900), (700, 128, 3000), (3000, 33, 500), (3, 300, 2000), (40, 4096, 100), (90, 200, 700), (1500, 260, 1500)])
+def test_gradients_of_a_cross_entropy_of_any_size_in_half_precision(rows, width, items, sizes):
+    dloss_size, x_size, weight_size = DLOSSES[sizes]
+    x, weight = values((rows, width), "f16", 100, x_size), values((items, width), "f16", 101, weight_size)
+    target = torch.randint(0, items, (rows,), generator=torch.Generator().manual_seed(102)).cuda()
+    target[1::7] = -100
+    dloss = values(rows, "f32", 103, dloss_size)
+    _, lse = nn.linear_cross_entropy(x, weight, target, stats=True)
+    dx, dweight, _ = nn.linear_cross_entropy_backward(dloss, x, weight, target, lse)
+    want = ref.cross_entropy_gradient(wide(dloss), wide(x), wide(weight), None, target, wide(lse), -100, torch.float16)
+    for got, (value, slack), what in zip((dx, dweight), want, ("dx", "dweight")):
+        check_half(got, value, slack, what)
+    # what the case is there for (results below half of the smallest half are zeros whatever the slopes)
+    for got, (value, _), name in zip((dx, dweight), want, ("dx", "dweight")):
+        if name in sizes:
+            assert got.isfinite().all() and (got != 0).sum() >= (value.abs() > 2.0 ** -24).sum() > 50
