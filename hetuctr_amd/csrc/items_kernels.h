@@ -41,7 +41,8 @@ __device__ __forceinline__ f32x4 slope4(f32x4 sum, f32x4 bias, float lse, float 
 }
 
 // A tile of logits.  Forward: the rows' tails over the tile's items, in registers, then over the lanes that share a row, then over the waves.
-// Gradient: d, rounded, and its sums over the tile's rows for the bias.  An exponential and four to six instructions a logit stand behind
+// Gradient: d, rounded to the type, since the matrix cores take both operands of the products behind it in one, and its sums over the tile's
+// rows for the bias, from before that.  An exponential and four to six instructions a logit stand behind
 // width / 32 products of 16 x 16 x 32: from some hundred columns on the matrix cores bound it (6144 rows and 65537 items of 4096 bfloat16:
 // gradient 3.1 ms, 1.06 PFLOP/s).
 template <typename T, int TILE, bool GRADIENT>
@@ -65,6 +66,13 @@ __global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kNo
   if constexpr (!GRADIENT) {
     constexpr int ACROSS = TILE / 64;
     Tail *tails = (Tail *)tiles; // [ACROSS][TILE]
+    // (all loaded before any hit is written, which might change them for all that the compiler knows)
+    uint32_t aims[P::kRowTiles]; // the targets' places among the wave's columns
+#pragma unroll
+    for (int i = 0; i < P::kRowTiles; i++) {
+      const uint32_t r = row0 + P::wave_row() + i * 16 + l % 16;
+      aims[i] = (r < rows ? p.taken.target[r] : kNoItem) - (column0 + wave_column);
+    }
 #pragma unroll
     for (int i = 0; i < P::kRowTiles; i++) {
       const uint32_t in = P::wave_row() + i * 16 + l % 16;
@@ -74,7 +82,7 @@ __global__ __launch_bounds__((Product<T, Lies::kAlong, Lies::kAlong, Second::kNo
       t = join_lanes(t, 16);
       t = join_lanes(t, 32);
       if (l < 16) tails[wave_column / 64 * TILE + in] = t;
-      const uint32_t aim = (row0 + in < rows ? p.taken.target[row0 + in] : kNoItem) - (column0 + wave_column);
+      const uint32_t aim = aims[i];
       if (__ballot(aim < 64))
 #pragma unroll
         for (int j = 0; j < P::kColumnTiles; j++)

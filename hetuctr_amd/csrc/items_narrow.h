@@ -7,9 +7,9 @@
 // owned row and 4 + 4 of the others, which the second product takes as its k, in whatever order, if the other operand comes in the same
 // one.  That is the same tile in LDS, read across.
 //
-// Bound by the vector units: forward an exponential (a quarter of the others' rate) and four instructions a logit, 73 % of the cycles beside 35 %
-// in the matrix cores.  4096 rows, a million items of 128 bfloat16: 1.19 ms (0.88 PFLOP/s), by tiles, each of which joins lanes and waves
-// for itself, 2.75; dx 2.0 and the weights' gradient 2.1, with d in memory 8.9 together.  Of 32 columns 0.78, 0.90 and 0.99.
+// Bound by the vector units: forward an exponential (a quarter of the others' rate) and four instructions a logit, 81 % of the cycles beside 40 %
+// in the matrix cores.  4096 rows, a million items of 128 bfloat16: 1.17 ms (0.89 PFLOP/s), by tiles, each of which joins lanes and waves
+// for itself, 2.75; dx 2.0 and the weights' gradient 2.1, with d in memory 8.9 together.  Of 32 columns 0.77, 0.90 and 0.99.
 #pragma once
 #include "items.h"
 #include "items_tail.h"
@@ -23,7 +23,9 @@ template <typename T, int KS> struct NarrowTiles {
   static constexpr int kThrough = 64, kLine = KS * 64, kPieces = KS * 4, kPasses = kThrough * kPieces / 256;
   static_assert(kPasses >= 1);
   static constexpr uint32_t kBytes = kThrough * kLine;
-  // 16 rows' pieces, and 32 bytes of 16 rows, lie in different banks
+  // 16 rows' pieces lie in different banks.  32 bytes of 16 rows, read across, do two by two in the same ones: neighbours have the same two pieces, which
+  // costs a third of the cycles with reads in the gradients.  (With the row's bits rotated by one none would, and took as long: 4096 rows, a
+  // million items, 128 columns 4066 to 4087 us either way, 64 columns 2651 and 2674.)
   static __device__ __forceinline__ uint32_t placed(uint32_t row, uint32_t piece) { return piece ^ (row / (4 / KS) & (kPieces - 1)); }
   uint32_t offset; // the order of a row's pieces is that of the rows kRows further down
   static constexpr uint32_t kRows = 256 / kPieces;
@@ -219,6 +221,7 @@ __global__ __launch_bounds__(256, narrow_share(KS * 32, MODE != Narrow::kForward
 #pragma unroll
                 for (int e = 0; e < 4; e++) total[i] += sum[i][j][e];
         }
+        // (rounded: the matrix cores take both operands in one type)
         Fragment<T> d[OI];
 #pragma unroll
         for (int i = 0; i < OI; i++) {
@@ -247,7 +250,7 @@ __global__ __launch_bounds__(256, narrow_share(KS * 32, MODE != Narrow::kForward
     // The logits of the rows' targets, once more: the products of the rows with the 16 items that they aim at, by the same instructions in the same
     // order, so that they are the logits above to the bit; what a row has of its own lies on the diagonal.  (Picked out in the loop they would
     // cost two instructions a logit where there are few items.)
-    if (range == 0)
+    if (range == p.ranges - 1) // which has the fewest tiles
 #pragma unroll
       for (int i = 0; i < OI; i++) {
         const uint32_t r = first + i * 16 + l % 16, item = r < owned ? p.taken.target[r] : kNoItem;

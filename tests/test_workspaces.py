@@ -1,4 +1,4 @@
-"""How much memory cross entropy over many items works in, as INTEGRATION.md and include/hetuctr_hip.h say: no GPU is needed to ask."""
+"""How much memory cross entropy over many items works in (include/hetuctr_hip.h): no GPU is needed to ask."""
 import os
 
 import pytest
